@@ -27,9 +27,13 @@ GLUE_SRC = os.path.join(CSRC, "dg_torch_glue.cpp")
 GLUE_PATH = os.path.join(PKG_DIR, "deepgemm", "_glue.so")
 GLUE_STAMP = GLUE_PATH + ".stamp"
 
-SOURCES = ["dg_api.cu"]
-HEADERS = ["dg_ptx.cuh", "dg_grouped_gemm.cuh", "dg_grouped_gemm_pair.cuh", "dg_grouped_gemm_w4.cuh", "dg_grouped_gemm_w4s.cuh",
-           "dg_pack.cuh", "dg_quant_group.cuh", "dg_moe_chain.cuh", "dg_ep.cuh"]
+# Translation units and the headers each of them includes (a unit is recompiled when one changes).
+SOURCES = {
+    "dg_api.cu": ["dg_host.h", "dg_ptx.cuh", "dg_grouped_gemm.cuh", "dg_grouped_gemm_pair.cuh", "dg_grouped_gemm_w4.cuh",
+                  "dg_grouped_gemm_w4s.cuh", "dg_pack.cuh", "dg_quant_group.cuh", "dg_moe_chain.cuh", "dg_ep.cuh"],
+    "dg_train_api.cu": ["dg_host.h", "dg_rows.cuh", "dg_token_sort.cuh", "dg_checkpoint.cuh"],
+}
+OBJ_DIR = os.path.join(PKG_DIR, "build")
 
 
 def _nvcc() -> str:
@@ -39,9 +43,9 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found (set NVCC or put it on PATH)")
 
 
-def _digest() -> str:
+def _digest(source: str) -> str:
     h = hashlib.sha256()
-    files = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
+    files = [os.path.join(CSRC, f) for f in [source] + SOURCES[source]]
     files.append(os.path.join(REPO_DIR, "include", "deepgemm_b200.h"))
     files.append(os.path.abspath(__file__))
     for f in files:
@@ -50,20 +54,22 @@ def _digest() -> str:
     return h.hexdigest()
 
 
-def nvcc_command(verbose: bool = False) -> list[str]:
+def nvcc_command(source: str, obj: str, verbose: bool = False) -> list[str]:
     cmd = [
         _nvcc(),
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-O3", "-std=c++17", "-lineinfo",
-        "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-        "-cudart", "static",
+        "-c", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
         "-I", os.path.join(REPO_DIR, "include"), "-I", CSRC,
     ]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
-    cmd += ["-o", LIB_PATH]
-    return cmd
+    return cmd + [os.path.join(CSRC, source), "-o", obj]
+
+
+def link_command(objs: list[str]) -> list[str]:
+    return [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompiler", "-fPIC",
+            "-cudart", "static"] + objs + ["-o", LIB_PATH]
 
 
 def glue_command() -> list[str]:
@@ -122,21 +128,43 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles the library (and the host glue) if their sources changed; returns the path of
     libdeepgemm_b200.so."""
     os.makedirs(LIB_DIR, exist_ok=True)
-    digest = _digest()
-    fresh = False
-    if not force and os.path.exists(LIB_PATH) and os.path.exists(STAMP_PATH):
-        with open(STAMP_PATH) as fh:
-            fresh = fh.read().strip() == digest
-    if not fresh:
-        cmd = nvcc_command(verbose)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+
+    def read(path):
+        if not os.path.exists(path):
+            return ""
+        with open(path) as fh:
+            return fh.read().strip()
+
+    digests = {s: _digest(s) for s in SOURCES}
+    whole = hashlib.sha256("".join(digests[s] for s in sorted(SOURCES)).encode()).hexdigest()
+    if force or not os.path.exists(LIB_PATH) or read(STAMP_PATH) != whole:
+        running = []
+        for s, digest in digests.items():
+            obj = os.path.join(OBJ_DIR, s + ".o")
+            if not force and not verbose and os.path.exists(obj) and read(obj + ".stamp") == digest:
+                continue
+            cmd = nvcc_command(s, obj, verbose)
+            running.append((digest, obj, cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+        failed = []
+        for digest, obj, cmd, proc in running:
+            output, _ = proc.communicate()
+            if verbose or proc.returncode != 0:
+                sys.stderr.write(output)
+            if proc.returncode != 0:
+                failed.append(" ".join(cmd))
+                continue
+            with open(obj + ".stamp", "w") as fh:
+                fh.write(digest)
+        if failed:
+            raise RuntimeError("nvcc failed building libdeepgemm_b200.so:\n" + "\n".join(failed))
+        cmd = link_command([os.path.join(OBJ_DIR, s + ".o") for s in SOURCES])
         proc = subprocess.run(cmd, capture_output=True, text=True)
-        if verbose or proc.returncode != 0:
-            sys.stderr.write(proc.stdout)
-            sys.stderr.write(proc.stderr)
         if proc.returncode != 0:
-            raise RuntimeError("nvcc failed building libdeepgemm_b200.so:\n" + " ".join(cmd))
+            sys.stderr.write(proc.stdout + proc.stderr)
+            raise RuntimeError("linking libdeepgemm_b200.so failed:\n" + " ".join(cmd))
         with open(STAMP_PATH, "w") as fh:
-            fh.write(digest)
+            fh.write(whole)
     build_glue(force=force, verbose=verbose)
     return LIB_PATH
 

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "deepgemm_b200.h"
+#include "dg_host.h"
 #include "dg_grouped_gemm.cuh"
 #include "dg_grouped_gemm_pair.cuh"
 #include "dg_grouped_gemm_w4.cuh"
@@ -18,28 +19,24 @@
 #include "dg_ep.cuh"
 
 namespace {
-
 using namespace dg;
-
 thread_local int tl_last_cuda_error = 0;
 std::atomic<long long> g_launch_count{0};
+}  // namespace
+
+namespace dg {
+namespace host {
 
 int cuda_fail(cudaError_t e) {
   tl_last_cuda_error = static_cast<int>(e);
   return DG_ERR_CUDA;
 }
 
+void count_launches(int n) { g_launch_count.fetch_add(n, std::memory_order_relaxed); }
+
 // ---- per-device cache (filled once; the reference queries device properties per call,
 //      csrc/arch/gfx936_gfx938_shared/m_grouped_w8a8_gemm_nt_masked.cu:85-89)
-constexpr int kMaxDevices = 64;
-struct DeviceInfo {
-  std::once_flag once;
-  int status = DG_ERR_NO_DEVICE;
-  int sm_count = 0;
-  int max_smem = 0;
-  int cc = 0;
-};
-DeviceInfo g_dev[kMaxDevices];
+static DeviceInfo g_dev[kMaxDevices];
 
 int device_info(const DeviceInfo** out) {
   int dev = -1;
@@ -67,6 +64,13 @@ int device_info(const DeviceInfo** out) {
   *out = &d;
   return d.status;
 }
+
+}  // namespace host
+}  // namespace dg
+
+namespace {
+
+using namespace dg::host;
 
 // ---- cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link)
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -110,8 +114,10 @@ struct MapSlot {
 constexpr int kMapSlots = 256;
 std::atomic<unsigned long long> g_map_hits{0}, g_map_misses{0};
 
+}  // namespace
+
 // rank-2 or rank-3 tiled map; dims/strides innermost first, strides in bytes for dims 1..
-int encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base,
+int dg::host::encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base,
                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
                CUtensorMapSwizzle swizzle) {
   EncodeTiledFn enc = get_encode();
@@ -168,6 +174,8 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* b
   encoded_ok = true;
   return DG_OK;
 }
+
+namespace {
 
 // ---- kernel instantiations: (kind, BN) -> stages so the ring holds ~192-200 KB
 template <int KIND, int BN>
@@ -643,8 +651,6 @@ int launch_w4_smem(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return DG_OK;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int validate_and_launch(Problem& pr, cudaStream_t stream) {
   if (pr.kind < DG_KIND_I8 || pr.kind > DG_KIND_BF16) return DG_ERR_BAD_KIND;

@@ -1,0 +1,111 @@
+// Rows of bf16 / fp16 / fp32 values as the memory-bound kernels of a training step handle them:
+// eight values of a row per thread, through 16-byte accesses where every row starts on a 16-byte
+// boundary and ends on one, value by value where not.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "deepgemm_b200.h"
+
+namespace dg {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight values of the 8 * LANES columns that begin at column c0, held by lane `lane` of LANES:
+// VEC: columns c0 + 8 * lane + i (c0, the row length and the row's address are multiples of 16
+// bytes); otherwise columns c0 + lane + LANES * i, so that a warp's accesses stay side by side.
+template <class T, bool VEC, int LANES>
+struct Eight {
+  union {
+    uint4 raw[sizeof(T) / 2];
+    T val[8];
+  };
+  __device__ __forceinline__ Eight() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  static __device__ __forceinline__ int col(int c0, int lane, int i) {
+    return VEC ? c0 + 8 * lane + i : c0 + lane + LANES * i;
+  }
+  // columns at or beyond `cols` are left at zero
+  __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols) {
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      if (c < cols) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + lane + LANES * i;
+        if (c < cols) val[i] = row[c];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int c0, int lane, int cols) const {
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      if (c < cols) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) *(reinterpret_cast<uint4*>(row + c) + i) = raw[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + lane + LANES * i;
+        if (c < cols) row[c] = val[i];
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return to_f32(val[i]); }
+  __device__ __forceinline__ void set(int i, float v) { val[i] = from_f32<T>(v); }  // round to nearest even
+};
+
+// The same for 8-bit codes: one 8-byte access, or byte by byte.
+template <bool VEC, int LANES>
+struct EightBytes {
+  union {
+    uint2 raw;
+    uint8_t val[8];
+  };
+  __device__ __forceinline__ EightBytes() { raw = make_uint2(0u, 0u); }
+  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols) {
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      if (c < cols) raw = __ldg(reinterpret_cast<const uint2*>(row + c));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + lane + LANES * i;
+        if (c < cols) val[i] = row[c];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* row, int c0, int lane, int cols) const {
+    if constexpr (VEC) {
+      const int c = c0 + 8 * lane;
+      if (c < cols) *reinterpret_cast<uint2*>(row + c) = raw;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + lane + LANES * i;
+        if (c < cols) row[c] = val[i];
+      }
+    }
+  }
+};
+
+}  // namespace dg

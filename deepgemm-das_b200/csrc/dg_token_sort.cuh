@@ -1,0 +1,439 @@
+// Tokens sorted by expert and back.
+//
+// A router names top_k experts for each of T tokens; pair p = t * top_k + j.  With
+//   count[e]  = #{p : id[p] = e},        offset[e] = sum_{e' < e} roundup(count[e'], align),
+//   dest[p]   = offset[id[p]] + #{p' < p : id[p'] = id[p]}
+// the sorted layout holds row dest[p] = x[t], m_indices[dest[p]] = id[p], and m_indices = -1 in
+// rows that stand for no pair (an expert's padding, everything behind the last expert).  The way
+// back and the gradients:
+//   out[t]     = sum_j w[t][j] * y[dest[t][j]]
+//   dy[dest]   = w[t][j] * dout[t]           dw[t][j] = <dout[t], y[dest[t][j]]>
+//   dx[t]      = sum_j drows[dest[t][j]]     (the way back without weights)
+// A pair whose id is negative (an expert that lives elsewhere) has dest = -1 and contributes
+// nothing; an id >= G is treated the same and reported in the status words.
+//
+// All of it moves rows and is bound by HBM; sums are held in fp32 in the order j = 0, 1, ..., so
+// no result depends on the launch shape, and nothing uses an atomic on a floating-point value.
+#pragma once
+
+#include "dg_rows.cuh"
+
+namespace dg {
+
+struct TokenSortParams {
+  const void* x;
+  const void* ids;      // int32 or int64 [T][top_k]
+  int ids64;
+  int T, top_k, G, align, cap;
+  int row_bytes;        // bytes of a row
+  long long x_stride;   // bytes between rows of x
+  void* rows;           // [cap] rows
+  int32_t* dest;        // [T][top_k]
+  int32_t* m_indices;   // [cap]
+  int32_t* counts;      // [G]
+  int32_t* offsets;     // [G]
+  int32_t* m_total;     // [1]
+  int32_t* status;
+  const int32_t* hist;  // NULL, or [chunks + 1][G]: pairs of each expert before each block's chunk, then totals
+  int tokens_per_block;
+  int clear;            // write zeros into rows that stand for no pair
+  int rep;              // copies of the shared-memory histogram (fewer lanes meet at one address)
+};
+
+constexpr int kSortThreads = 512;
+constexpr int kSortMaxChunk = 2048;  // pairs of one block
+
+__device__ __forceinline__ int sort_id(const TokenSortParams& p, long long i) {
+  if (p.ids64) {
+    const long long v = static_cast<const long long*>(p.ids)[i];
+    return v < 0 ? -1 : (v >= p.G ? p.G : static_cast<int>(v));
+  }
+  const int v = static_cast<const int32_t*>(p.ids)[i];
+  return v < 0 ? -1 : (v >= p.G ? p.G : v);
+}
+
+// Pairs of each expert in each block's chunk (more pairs than one block should count by itself).
+__global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(const TokenSortParams p, int32_t* hist) {
+  extern __shared__ int32_t cnt[];
+  for (int e = threadIdx.x; e < p.G; e += kSortThreads) cnt[e] = 0;
+  __syncthreads();
+  const long long p0 = (long long)blockIdx.x * p.tokens_per_block * p.top_k;
+  const long long p1 = min(p0 + (long long)p.tokens_per_block * p.top_k, (long long)p.T * p.top_k);
+  for (long long i = p0 + threadIdx.x; i < p1; i += kSortThreads) {
+    const int e = sort_id(p, i);
+    if (e >= 0 && e < p.G) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.G; e += kSortThreads) hist[(size_t)blockIdx.x * p.G + e] = cnt[e];
+}
+
+// Running sums over the chunks, one warp per expert; entry [chunks] is the total.
+__global__ void __launch_bounds__(256) sort_scan_kernel(int32_t* hist, int chunks, int G) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (e >= G) return;
+  int running = 0;
+  for (int c0 = 0; c0 < chunks; c0 += 32) {
+    const int c = c0 + lane;
+    const int v = c < chunks ? hist[(size_t)c * G + e] : 0;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (c < chunks) hist[(size_t)c * G + e] = running + x - v;
+    running += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) hist[(size_t)chunks * G + e] = running;
+}
+
+template <int VB>
+struct BytesOf;
+template <>
+struct BytesOf<16> { using type = uint4; };
+template <>
+struct BytesOf<4> { using type = uint32_t; };
+template <>
+struct BytesOf<2> { using type = uint16_t; };
+
+// Plan and copy in one launch.  Every block counts all pairs itself (their ids stay in L2: 32768
+// pairs are 128 KB), so no block waits for another; it then places the pairs of its own tokens and
+// copies their rows, each read once and written top_k times.  blockIdx.y splits the columns of a
+// row when there are few tokens.
+template <int VB>
+__global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSortParams p) {
+  using V = typename BytesOf<VB>::type;
+  extern __shared__ int32_t sm[];
+  int32_t* before = sm;               // [G] pairs of e before this block's (then: placed so far)
+  int32_t* count = before + p.G;      // [G]
+  int32_t* offset = count + p.G;      // [G + 1]
+  int32_t* dest_s = offset + p.G + 1; // [tokens_per_block * top_k]
+  int32_t* hist = dest_s + p.tokens_per_block * p.top_k;  // [2][G][rep]
+  __shared__ int bad_s, list_n;
+  __shared__ int list[kSortThreads];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long R = (long long)p.T * p.top_k;
+  const int t0 = blockIdx.x * p.tokens_per_block;
+  const int nt = min(p.tokens_per_block, p.T - t0);
+  const long long p0 = (long long)t0 * p.top_k;
+  const int np = nt * p.top_k;
+  const bool first = blockIdx.y == 0;
+
+  if (tid == 0) bad_s = 0;
+  if (p.hist == nullptr) {
+    for (int i = tid; i < 2 * p.G * p.rep; i += kSortThreads) hist[i] = 0;
+    __syncthreads();
+    const int mine = lane & (p.rep - 1);
+    auto note = [&](int e, long long i) {
+      if (e < 0) return;
+      if (e >= p.G) {
+        bad_s = 1;
+        return;
+      }
+      atomicAdd(&hist[((i < p0 ? 0 : p.G) + e) * p.rep + mine], 1);
+    };
+    if (!p.ids64 && (reinterpret_cast<uintptr_t>(p.ids) & 15u) == 0) {
+      const int4* v = static_cast<const int4*>(p.ids);
+      const long long nv = R / 4;
+#pragma unroll 4
+      for (long long i = tid; i < nv; i += kSortThreads) {
+        const int4 q = __ldg(v + i);
+        note(min(q.x, p.G), 4 * i);
+        note(min(q.y, p.G), 4 * i + 1);
+        note(min(q.z, p.G), 4 * i + 2);
+        note(min(q.w, p.G), 4 * i + 3);
+      }
+      for (long long i = 4 * nv + tid; i < R; i += kSortThreads) note(sort_id(p, i), i);
+    } else {
+#pragma unroll 4
+      for (long long i = tid; i < R; i += kSortThreads) note(sort_id(p, i), i);
+    }
+    __syncthreads();
+    for (int e = tid; e < p.G; e += kSortThreads) {
+      int b = 0, r = 0;
+      for (int c = 0; c < p.rep; ++c) {
+        b += hist[e * p.rep + c];
+        r += hist[(p.G + e) * p.rep + c];
+      }
+      before[e] = b;
+      count[e] = b + r;
+    }
+  } else {
+    for (int e = tid; e < p.G; e += kSortThreads) {
+      before[e] = p.hist[(size_t)blockIdx.x * p.G + e];
+      count[e] = p.hist[(size_t)gridDim.x * p.G + e];
+    }
+    __syncthreads();  // bad_s is zero before the ids below are looked at
+    for (long long i = p0 + tid; i < p0 + np; i += kSortThreads)
+      if (sort_id(p, i) >= p.G) bad_s = 1;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int running = 0;
+    for (int e0 = 0; e0 < p.G; e0 += 32) {
+      const int e = e0 + lane;
+      const int v = e < p.G ? (count[e] + p.align - 1) / p.align * p.align : 0;
+      int x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (e < p.G) offset[e] = running + x - v;
+      running += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) offset[p.G] = running;
+    __syncwarp();
+    // stable places of this block's pairs, 32 at a time
+    for (int i0 = 0; i0 < np; i0 += 32) {
+      const int i = i0 + lane;
+      const int e = i < np ? sort_id(p, p0 + i) : -1;
+      const bool in = e >= 0 && e < p.G;
+      const unsigned same = __match_any_sync(0xffffffffu, in ? e : -1);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      int d = -1;
+      if (in) d = offset[e] + before[e] + rank;
+      __syncwarp();
+      if (in && rank == 0) before[e] += __popc(same);
+      __syncwarp();
+      if (i < np) {
+        dest_s[i] = d;
+        if (first) p.dest[p0 + i] = d;
+      }
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && first) {
+    for (int e = tid; e < p.G; e += kSortThreads) {
+      p.counts[e] = count[e];
+      p.offsets[e] = offset[e];
+    }
+    if (tid == 0) *p.m_total = offset[p.G];
+  }
+  if (tid == 0 && first && bad_s && p.status != nullptr) atomicCAS(p.status, DG_DEV_OK, DG_DEV_BAD_GROUP_INDEX);
+
+  // rows: a warp takes 4 x 32 vectors of one token at a time
+  const int nv = p.row_bytes / VB;
+  constexpr int kSeg = 128;
+  const int segs_all = (nv + kSeg - 1) / kSeg;
+  const int segs_per = (segs_all + gridDim.y - 1) / gridDim.y;
+  const int seg0 = blockIdx.y * segs_per, seg1 = min(seg0 + segs_per, segs_all);
+  const int segs = max(seg1 - seg0, 0);
+  char* rows = static_cast<char*>(p.rows);
+  for (int u = warp; u < nt * segs; u += kSortThreads / 32) {
+    const int t = u / segs, v0 = (seg0 + u - t * segs) * kSeg + lane;
+    const V* src = reinterpret_cast<const V*>(static_cast<const char*>(p.x) + (long long)(t0 + t) * p.x_stride);
+    V v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (v0 + 32 * i < nv) v[i] = __ldg(src + v0 + 32 * i);
+    for (int j = 0; j < p.top_k; ++j) {
+      const int d = dest_s[t * p.top_k + j];
+      if (d < 0) continue;
+      V* dst = reinterpret_cast<V*>(rows + (size_t)d * p.row_bytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v0 + 32 * i < nv) dst[v0 + 32 * i] = v[i];
+    }
+  }
+
+  // m_indices, and zeros in the rows that stand for no pair
+  const int per = (p.cap + gridDim.x - 1) / gridDim.x;
+  const long long r1 = min((long long)(blockIdx.x + 1) * per, (long long)p.cap);
+  for (long long rb = (long long)blockIdx.x * per; rb < r1; rb += kSortThreads) {
+    if (tid == 0) list_n = 0;
+    __syncthreads();
+    const long long r = rb + tid;
+    if (r < r1) {
+      int lo = 0, hi = p.G;  // the last expert that begins at or before r (empty ones begin where the next does)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (offset[mid] <= r) lo = mid; else hi = mid;
+      }
+      const bool used = r < (long long)offset[lo] + count[lo];
+      if (first) p.m_indices[r] = used ? lo : -1;
+      if (!used && p.clear) list[atomicAdd(&list_n, 1)] = static_cast<int>(r);
+    }
+    __syncthreads();
+    const int n = list_n;
+    for (int u = warp; u < n * segs; u += kSortThreads / 32) {
+      const int i = u / segs, v0 = (seg0 + u - i * segs) * kSeg + lane;
+      V* dst = reinterpret_cast<V*>(rows + (size_t)list[i] * p.row_bytes);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (v0 + 32 * k < nv) dst[v0 + 32 * k] = V{};
+    }
+    __syncthreads();
+  }
+}
+
+struct TokenUnsortParams {
+  const void* y;         // [rows] rows of H values
+  const int32_t* dest;   // [T][top_k]
+  const float* weights;  // [T][top_k] or NULL
+  void* out;             // [T][H]
+  int T, top_k, H, rows;
+  long long y_stride;    // values between rows of y
+};
+
+// out[t] = sum_j w * y[dest]: a warp takes 256 columns of one token; the rows of its pairs are
+// fetched together (up to eight in flight) and added in order.
+constexpr int kUnsortThreads = 256;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kUnsortThreads) token_unsort_kernel(const TokenUnsortParams p) {
+  const int lane = threadIdx.x & 31;
+  const int segs = (p.H + 255) / 256;
+  const long long units = (long long)p.T * segs;
+  const long long step = (long long)gridDim.x * (kUnsortThreads / 32);
+  for (long long u = (long long)blockIdx.x * (kUnsortThreads / 32) + (threadIdx.x >> 5); u < units; u += step) {
+    const long long t = u / segs;
+    const int c0 = static_cast<int>(u - t * segs) * 256;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+      int d = -1;
+      float w = 1.0f;
+      if (lane < 8 && j0 + lane < p.top_k) {
+        d = p.dest[t * p.top_k + j0 + lane];
+        if (d >= p.rows) d = -1;
+        if (p.weights) w = p.weights[t * p.top_k + j0 + lane];
+      }
+      Eight<T, VEC, 32> v[8];
+      int dj[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dj[j] = __shfl_sync(0xffffffffu, d, j);
+        if (dj[j] >= 0) v[j].load(static_cast<const T*>(p.y) + (size_t)dj[j] * p.y_stride, c0, lane, p.H);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        if (dj[j] >= 0) {  // a pair without a row adds nothing, whatever its weight is
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = fmaf(wj, v[j].get(i), acc[i]);
+        }
+      }
+    }
+    Eight<T, VEC, 32> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.set(i, acc[i]);
+    o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0, lane, p.H);
+  }
+}
+
+struct TokenUnsortGradParams {
+  const void* dout;          // [T] rows
+  const void* y;             // [rows] rows
+  const int32_t* dest;       // [T][top_k]
+  const float* weights;      // or NULL (weights of one; dw is not written)
+  const int32_t* m_indices;  // [rows]; with clear: rows with m_indices < 0 are set to zero
+  void* dy;                  // [rows][H]
+  float* dw;                 // [T][top_k] or NULL
+  int T, top_k, H, rows;
+  long long y_stride, dout_stride;
+  int per;                   // pairs of a token that one block takes
+  int clear_blocks;          // blocks behind those of the tokens that clear rows
+};
+
+// Sets rows with m_indices < 0 to zero: block `b` of `nb`.
+template <class T, bool VEC, int THREADS>
+__device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indices, int rows, int H, int b, int nb) {
+  const int lane = threadIdx.x & 31;
+  const int per = (rows + nb - 1) / nb;
+  const long long r1 = min((long long)(b + 1) * per, (long long)rows);
+  // a warp looks at 32 rows at a time and clears the ones that stand for nothing together
+  for (long long rb = (long long)b * per + (threadIdx.x >> 5) * 32; rb < r1; rb += THREADS) {
+    const bool free_row = rb + lane < r1 && m_indices[rb + lane] < 0;
+    unsigned mask = __ballot_sync(0xffffffffu, free_row);
+    while (mask) {
+      const int i = __ffs(mask) - 1;
+      mask &= mask - 1;
+      T* row = out + (size_t)(rb + i) * H;
+      const Eight<T, VEC, 32> zero;
+      for (int c0 = 0; c0 < H; c0 += 256) zero.store(row, c0, lane, H);
+    }
+  }
+}
+
+// One block takes `per` pairs of one token: dout[t] stays in registers (2048 columns at a time)
+// while the rows of y go by; each row's product with dout is summed over the block in a fixed
+// order.
+constexpr int kUnsortGradThreads = 128;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kUnsortGradThreads) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
+  constexpr int kWarps = kUnsortGradThreads / 32;
+  __shared__ float part[kWarps][32];
+  const int splits = (p.top_k + p.per - 1) / p.per;
+  const long long token_blocks = (long long)p.T * splits;
+  if ((long long)blockIdx.x >= token_blocks) {
+    clear_rows_block<T, VEC, kUnsortGradThreads>(static_cast<T*>(p.dy), p.m_indices, p.rows, p.H,
+                                                 static_cast<int>(blockIdx.x - token_blocks), p.clear_blocks);
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = blockIdx.x / splits;
+  const int j_begin = static_cast<int>(blockIdx.x - t * splits) * p.per;
+  const int j_end = min(j_begin + p.per, p.top_k);
+  const T* dout = static_cast<const T*>(p.dout) + (size_t)t * p.dout_stride;
+  for (int j0 = j_begin; j0 < j_end; j0 += 32) {
+    const int nj = min(32, j_end - j0);
+    float dot = 0.0f;  // lane j: this warp's part of pair j0 + j
+    constexpr int kPass = 2;
+    for (int base = 0; base < p.H; base += kPass * kWarps * 256) {
+      Eight<T, VEC, 32> g[kPass];
+#pragma unroll
+      for (int k = 0; k < kPass; ++k) g[k].load(dout, base + (k * kWarps + warp) * 256, lane, p.H);
+#pragma unroll 2
+      for (int j = 0; j < nj; ++j) {
+        const int d = p.dest[t * p.top_k + j0 + j];
+        if (d < 0 || d >= p.rows) continue;
+        const float w = p.weights ? p.weights[t * p.top_k + j0 + j] : 1.0f;
+        const T* yr = static_cast<const T*>(p.y) + (size_t)d * p.y_stride;
+        T* dr = static_cast<T*>(p.dy) + (size_t)d * p.H;
+        float s = 0.0f;
+        if (p.dw != nullptr) {
+          Eight<T, VEC, 32> v[kPass];
+#pragma unroll
+          for (int k = 0; k < kPass; ++k) v[k].load(yr, base + (k * kWarps + warp) * 256, lane, p.H);
+#pragma unroll
+          for (int k = 0; k < kPass; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              s = fmaf(g[k].get(i), v[k].get(i), s);  // columns behind the row's end hold zeros
+        }
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) {
+          Eight<T, VEC, 32> o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.set(i, w * g[k].get(i));
+          o.store(dr, base + (k * kWarps + warp) * 256, lane, p.H);
+        }
+        if (p.dw != nullptr) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (lane == j) dot += s;
+        }
+      }
+    }
+    if (p.dw != nullptr) {
+      part[warp][lane] = dot;
+      __syncthreads();
+      if (threadIdx.x < nj) {
+        float s = part[0][lane];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) s += part[w][lane];
+        p.dw[t * p.top_k + j0 + lane] = s;  // zero for a pair without a row
+      }
+      __syncthreads();
+    }
+  }
+}
+
+constexpr int kClearThreads = 128;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kClearThreads) clear_rows_kernel(T* out, const int32_t* m_indices, int rows, int H) {
+  clear_rows_block<T, VEC, kClearThreads>(out, m_indices, rows, H, blockIdx.x, gridDim.x);
+}
+
+}  // namespace dg

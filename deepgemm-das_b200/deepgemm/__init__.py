@@ -65,6 +65,10 @@ from .legacy_compat import *  # noqa: F401,F403  (old names, as the reference re
 from .quant_group import quant_group_capacity, quantize_group_rows
 from .moe_marlin_prefill import assert_moe_prefill_down_fp8_shapes, moe_w8a8_marlin_prefill_down_fp8
 from .moe_chain import combine_rows, expert_mlp_contiguous, moe_forward, silu_mul_quant
+from .token_sort import (TokenPlan, clear_padding_rows, sort_capacity, sort_tokens, sort_tokens_grad, unsort_tokens,
+                         unsort_tokens_grad)
+from .activation_checkpoint import (Checkpoint, checkpoint_rows, restore_rows, silu_mul, silu_mul_checkpoint,
+                                    silu_mul_checkpoint_grad)
 from .print_size import install_op_size_printer
 from ._core import check_device_status
 

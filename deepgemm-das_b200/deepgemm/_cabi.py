@@ -37,6 +37,16 @@ EXPORTED_SYMBOLS = (
     "dg_ep_plan",
     "dg_ep_push",
     "dg_ep_barrier",
+    "dg_token_sort_capacity",
+    "dg_token_sort_scratch_bytes",
+    "dg_token_sort",
+    "dg_token_unsort",
+    "dg_token_unsort_grad",
+    "dg_clear_padding_rows",
+    "dg_checkpoint_rows",
+    "dg_restore_rows",
+    "dg_act_checkpoint",
+    "dg_act_checkpoint_grad",
     "dg_pack_weight",
     "dg_unpack_weight",
     "dg_query",
@@ -304,6 +314,116 @@ class EpBarrierArgs(C.Structure):
     ]
 
 
+MAX_GROUPS, MAX_TOP_K = 1024, 128
+
+
+class TokenSortArgs(C.Structure):
+    _fields_ = [
+        ("elem_bytes", C.c_int32),
+        ("ids64", C.c_int32),
+        ("num_tokens", C.c_int32),
+        ("top_k", C.c_int32),
+        ("num_groups", C.c_int32),
+        ("hidden", C.c_int32),
+        ("align", C.c_int32),
+        ("cap", C.c_int32),
+        ("x_stride", C.c_int64),
+        ("x", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("rows", C.c_void_p),
+        ("dest", C.c_void_p),
+        ("m_indices", C.c_void_p),
+        ("counts", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("m_total", C.c_void_p),
+        ("scratch", C.c_void_p),
+        ("scratch_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+        ("clear", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class TokenUnsortArgs(C.Structure):
+    _fields_ = [
+        ("elem", C.c_int32),
+        ("num_tokens", C.c_int32),
+        ("top_k", C.c_int32),
+        ("hidden", C.c_int32),
+        ("num_rows", C.c_int32),
+        ("reserved", C.c_int32),
+        ("y_stride", C.c_int64),
+        ("y", C.c_void_p),
+        ("dest", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("out", C.c_void_p),
+    ]
+
+
+class TokenUnsortGradArgs(C.Structure):
+    _fields_ = [
+        ("elem", C.c_int32),
+        ("num_tokens", C.c_int32),
+        ("top_k", C.c_int32),
+        ("hidden", C.c_int32),
+        ("num_rows", C.c_int32),
+        ("clear", C.c_int32),
+        ("y_stride", C.c_int64),
+        ("dout_stride", C.c_int64),
+        ("dout", C.c_void_p),
+        ("y", C.c_void_p),
+        ("dest", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("m_indices", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("dw", C.c_void_p),
+    ]
+
+
+class ClearRowsArgs(C.Structure):
+    _fields_ = [
+        ("elem", C.c_int32),
+        ("num_rows", C.c_int32),
+        ("hidden", C.c_int32),
+        ("reserved", C.c_int32),
+        ("rows", C.c_void_p),
+        ("m_indices", C.c_void_p),
+    ]
+
+
+class CheckpointArgs(C.Structure):
+    _fields_ = [
+        ("elem", C.c_int32),
+        ("kind", C.c_int32),
+        ("num_rows", C.c_int32),
+        ("hidden", C.c_int32),
+        ("x_stride", C.c_int64),
+        ("x", C.c_void_p),
+        ("q", C.c_void_p),
+        ("scale", C.c_void_p),
+    ]
+
+
+class ActCheckpointArgs(C.Structure):
+    _fields_ = [
+        ("elem", C.c_int32),
+        ("kind", C.c_int32),
+        ("num_rows", C.c_int32),
+        ("hidden", C.c_int32),
+        ("clear", C.c_int32),
+        ("reserved", C.c_int32),
+        ("x_stride", C.c_int64),
+        ("dact_stride", C.c_int64),
+        ("x", C.c_void_p),
+        ("dact", C.c_void_p),
+        ("q", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("act", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("m_indices", C.c_void_p),
+    ]
+
+
 def pointer_array(ptrs):
     """ctypes array of device pointers (a HOST array, as the dg_ep_* calls take)."""
     return (C.c_void_p * len(ptrs))(*[int(x) for x in ptrs])
@@ -349,6 +469,16 @@ def _load() -> C.CDLL:
     lib.dg_ep_push.restype = C.c_int
     lib.dg_ep_barrier.argtypes = [C.POINTER(EpBarrierArgs), C.c_void_p]
     lib.dg_ep_barrier.restype = C.c_int
+    lib.dg_token_sort_capacity.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    lib.dg_token_sort_capacity.restype = C.c_int64
+    lib.dg_token_sort_scratch_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32]
+    lib.dg_token_sort_scratch_bytes.restype = C.c_size_t
+    for fn, args in ((lib.dg_token_sort, TokenSortArgs), (lib.dg_token_unsort, TokenUnsortArgs),
+                     (lib.dg_token_unsort_grad, TokenUnsortGradArgs), (lib.dg_clear_padding_rows, ClearRowsArgs),
+                     (lib.dg_checkpoint_rows, CheckpointArgs), (lib.dg_restore_rows, CheckpointArgs),
+                     (lib.dg_act_checkpoint, ActCheckpointArgs), (lib.dg_act_checkpoint_grad, ActCheckpointArgs)):
+        fn.argtypes = [C.POINTER(args), C.c_void_p]
+        fn.restype = C.c_int
     lib.dg_query.argtypes = [C.c_int32]
     lib.dg_query.restype = C.c_int64
     lib.dg_strerror.argtypes = [C.c_int]

@@ -579,6 +579,148 @@ typedef struct dg_ep_barrier_args {
  * own call with the same epoch (system-scope fence, signal, bounded wait; one tiny kernel). */
 DG_API int dg_ep_barrier(const dg_ep_barrier_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * A training step of an MoE layer: tokens sorted by expert and back, activation checkpoints in
+ * 8 bits.  (The gradients of the grouped product itself are declared further down.)  The reference
+ * library is forward only; these are additions of this library.
+ * Element types (`elem`): DG_OUT_BF16, DG_OUT_F16 or DG_OUT_F32.  Rows may lie apart (`*_stride`,
+ * in elements); any row length is taken, multiples of 8 on 16-byte boundaries are fastest.
+ * "Rows that stand for no pair" are those with m_indices < 0: `clear` != 0 sets them to zero in the
+ * outputs, `clear` == 0 leaves them as they are.
+ * --------------------------------------------------------------------------------------- */
+#define DG_MAX_TOP_K 128
+
+/* Tokens sorted by expert.  Pair p = t * top_k + j goes to row
+ *   dest[p] = offsets[ids[p]] + (number of pairs before p with the same id),
+ *   offsets[e] = sum over e' < e of counts[e'] rounded up to a multiple of `align`,
+ * rows[dest[p]] = x[t], m_indices[dest[p]] = ids[p], -1 in every other entry; m_total = the end of
+ * the last expert's (padded) rows.  A negative id, or one >= num_groups (reported in `status`),
+ * gives dest = -1 and no row. */
+typedef struct dg_token_sort_args {
+  int32_t elem_bytes;   /* 2 or 4: rows are only copied */
+  int32_t ids64;        /* 0: ids are int32, else int64 */
+  int32_t num_tokens;
+  int32_t top_k;        /* 1..DG_MAX_TOP_K */
+  int32_t num_groups;   /* 1..DG_MAX_GROUPS */
+  int32_t hidden;       /* elements of a row */
+  int32_t align;        /* 1 for the compact layout, 128 or 256 for the contiguous one */
+  int32_t cap;          /* rows of `rows`, at least dg_token_sort_capacity(...) */
+  int64_t x_stride;     /* elements between the rows of x */
+  const void* x;        /* [num_tokens][hidden] */
+  const void* ids;      /* [num_tokens][top_k] */
+  void*    rows;        /* [cap][hidden] */
+  int32_t* dest;        /* [num_tokens][top_k] */
+  int32_t* m_indices;   /* [cap] */
+  int32_t* counts;      /* [num_groups] pairs of each expert */
+  int32_t* offsets;     /* [num_groups] first row of each expert */
+  int32_t* m_total;     /* [1] */
+  void*    scratch;     /* dg_token_sort_scratch_bytes(...) bytes, NULL when that is 0 */
+  size_t   scratch_bytes;
+  int32_t* status;      /* NULL, or int32[DG_STATUS_WORDS] */
+  int32_t  clear;
+  int32_t  reserved;
+} dg_token_sort_args;
+
+/* Rows that hold any routing of `pairs` pairs: every expert in use ends in a padded block; -1 on
+ * bad arguments. */
+DG_API int64_t dg_token_sort_capacity(int64_t pairs, int32_t num_groups, int32_t align);
+/* 0 when no scratch is needed (up to 65536 pairs). */
+DG_API size_t dg_token_sort_scratch_bytes(int32_t num_tokens, int32_t top_k, int32_t num_groups);
+/* One launch (three above 65536 pairs). */
+DG_API int dg_token_sort(const dg_token_sort_args* args, void* stream);
+
+/* out[t] = sum over j, in order and in fp32, of weights[t][j] * y[dest[t][j]]; pairs with dest < 0
+ * add nothing.  Without weights this is also the gradient of dg_token_sort (y = gradient of rows). */
+typedef struct dg_token_unsort_args {
+  int32_t elem;
+  int32_t num_tokens;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t num_rows;       /* rows of y */
+  int32_t reserved;
+  int64_t y_stride;
+  const void*    y;       /* [num_rows][hidden] */
+  const int32_t* dest;    /* [num_tokens][top_k] */
+  const float*   weights; /* [num_tokens][top_k], or NULL: ones */
+  void*          out;     /* [num_tokens][hidden] */
+} dg_token_unsort_args;
+DG_API int dg_token_unsort(const dg_token_unsort_args* args, void* stream);
+
+/* Its gradients: dy[dest[t][j]] = weights[t][j] * dout[t], dw[t][j] = <dout[t], y[dest[t][j]]> (fp32
+ * sums in a fixed order; 0 for a pair without a row).  Every row may be named by one pair only, as
+ * dg_token_sort gives them. */
+typedef struct dg_token_unsort_grad_args {
+  int32_t elem;
+  int32_t num_tokens;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t num_rows;
+  int32_t clear;
+  int64_t y_stride;
+  int64_t dout_stride;
+  const void*    dout;      /* [num_tokens][hidden] */
+  const void*    y;         /* [num_rows][hidden]; NULL if dw is */
+  const int32_t* dest;
+  const float*   weights;   /* NULL: ones */
+  const int32_t* m_indices; /* [num_rows]; needed with `clear` */
+  void*          dy;        /* [num_rows][hidden] */
+  float*         dw;        /* [num_tokens][top_k], or NULL */
+} dg_token_unsort_grad_args;
+DG_API int dg_token_unsort_grad(const dg_token_unsort_grad_args* args, void* stream);
+
+/* Sets the rows with m_indices < 0 to zero. */
+typedef struct dg_clear_rows_args {
+  int32_t elem;
+  int32_t num_rows;
+  int32_t hidden;
+  int32_t reserved;
+  void*          rows;      /* [num_rows][hidden] */
+  const int32_t* m_indices; /* [num_rows] */
+} dg_clear_rows_args;
+DG_API int dg_clear_padding_rows(const dg_clear_rows_args* args, void* stream);
+
+/* Rows in 8 bits: 128 columns of a row (fewer at its end) share one fp32 scale s, code q stands for
+ * q * s.  DG_KIND_E4M3: s is the smallest power of two with max|x| / s <= 448 (at least 2^-126);
+ * DG_KIND_I8: s = max|x| / 127, q in [-127, 127].  s = 1 for a block of zeros, NaN for a block that
+ * holds a NaN or an infinity. */
+typedef struct dg_checkpoint_args {
+  int32_t elem;
+  int32_t kind;       /* DG_KIND_E4M3 or DG_KIND_I8 */
+  int32_t num_rows;
+  int32_t hidden;
+  int64_t x_stride;
+  void*   x;          /* [num_rows][hidden]: read by dg_checkpoint_rows, written (row after row) by dg_restore_rows */
+  void*   q;          /* [num_rows][hidden] bytes */
+  float*  scale;      /* [num_rows][ceil(hidden / 128)] */
+} dg_checkpoint_args;
+DG_API int dg_checkpoint_rows(const dg_checkpoint_args* args, void* stream);
+DG_API int dg_restore_rows(const dg_checkpoint_args* args, void* stream);
+
+/* The experts' activation with a checkpoint of its inputs.  Rows of x are gate (hidden columns), then
+ * up.  Forward: act = bf16/fp16/fp32(gate * sigmoid(gate) * up), computed in fp32 from x and rounded
+ * once, and q / scale = the checkpoint of gate and of up, each with blocks of its own.  Backward, from
+ * the values g, u that the checkpoint stands for:
+ *   dx = ( dact * u * sig(g) * (1 + g * (1 - sig(g))) | dact * g * sig(g) ),   act = g * sig(g) * u. */
+typedef struct dg_act_checkpoint_args {
+  int32_t elem;
+  int32_t kind;              /* DG_KIND_E4M3 or DG_KIND_I8 */
+  int32_t num_rows;
+  int32_t hidden;            /* H: columns of gate, of up and of act */
+  int32_t clear;
+  int32_t reserved;
+  int64_t x_stride;          /* forward */
+  int64_t dact_stride;       /* backward */
+  const void*    x;          /* forward: [num_rows][2 H] */
+  const void*    dact;       /* backward: [num_rows][H] */
+  void*          q;          /* [num_rows][2 H] bytes; written forward, read backward */
+  float*         scale;      /* [num_rows][2 * ceil(H / 128)] */
+  void*          act;        /* [num_rows][H] written; backward: may be NULL */
+  void*          dx;         /* backward: [num_rows][2 H] written */
+  const int32_t* m_indices;  /* NULL, or rows with m_indices < 0 are skipped */
+} dg_act_checkpoint_args;
+DG_API int dg_act_checkpoint(const dg_act_checkpoint_args* args, void* stream);
+DG_API int dg_act_checkpoint_grad(const dg_act_checkpoint_args* args, void* stream);
+
 /* dg_query() selectors. */
 #define DG_QUERY_ABI_VERSION   0
 #define DG_QUERY_SM_COUNT      1 /* multiprocessors of the current device (cached per device) */
