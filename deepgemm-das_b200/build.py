@@ -31,6 +31,7 @@ GLUE_STAMP = GLUE_PATH + ".stamp"
 SOURCES = {
     "dg_api.cu": ["dg_host.h", "dg_ptx.cuh", "dg_grouped_gemm.cuh", "dg_grouped_gemm_pair.cuh", "dg_grouped_gemm_w4.cuh",
                   "dg_grouped_gemm_w4s.cuh", "dg_pack.cuh", "dg_quant_group.cuh", "dg_moe_chain.cuh", "dg_ep.cuh"],
+    "dg_wgrad_api.cu": ["dg_host.h", "dg_ptx.cuh", "dg_grouped_wgrad.cuh"],
     "dg_train_api.cu": ["dg_host.h", "dg_rows.cuh", "dg_token_sort.cuh", "dg_checkpoint.cuh"],
 }
 OBJ_DIR = os.path.join(PKG_DIR, "build")

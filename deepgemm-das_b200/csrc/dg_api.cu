@@ -202,6 +202,7 @@ struct Problem {
   const int32_t* offsets;
   int G, M, N, K, block_n, expected_m;
   int narrow;  // filled by validate_and_launch: KernelParams::narrow
+  int b_trans;   // 1: dg_grouped_input_grad (contiguous layout, bf16): N = columns of D, K = contraction = rows of a weight block
   int dense;     // 1: dg_dense_gemm (row-major weights, no masked_m, any N, out_kind honoured)
   int out_kind;  // DG_OUT_BF16 / DG_OUT_F16 / DG_OUT_F32
   void* debug_acc;
@@ -219,13 +220,22 @@ struct Problem {
   int block_m, num_blocks, num_sorted, real_topk, max_runs;
 };
 
-template <int KIND, int BN, bool kGather = false>
+// The packed weight as the kBT kernels read it: [64 columns][n rows][groups x column blocks], so
+// that a box that reaches behind the n rows of its block is filled with zeros.
+int encode_bt_map(CUtensorMap* map, const Problem& pr) {
+  const uint64_t dims[3] = {64u, (uint64_t)pr.K, (uint64_t)pr.G * (pr.N / 64)};
+  const uint64_t strides[2] = {(uint64_t)kRowBytes, (uint64_t)kRowBytes * pr.K};
+  const uint32_t box[3] = {64u, 64u, 1u};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pr.b, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int KIND, int BN, bool kGather = false, bool kBT = false>
 int launch(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int STAGES = StagesFor<KIND, BN>::value;
   using L = SmemLayout<KIND, BN, STAGES>;
   static_assert(STAGES >= 2, "ring too shallow");
   static_assert(kGatherDepth < STAGES, "the gathering warps would wait for stages they have not signalled");
-  auto kernel = grouped_gemm_kernel<KIND, BN, STAGES, kGather>;
+  auto kernel = grouped_gemm_kernel<KIND, BN, STAGES, kGather, kBT>;
 
   const int esize = (KIND == DG_KIND_BF16) ? 2 : 1;
   const int elems_per_row = kRowBytes / esize;  // A elements per 128-byte K block
@@ -328,7 +338,9 @@ int launch(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   const uint64_t b_dims[2] = {pr.dense ? (uint64_t)pr.K : (uint64_t)elems_per_row,
                               pr.dense ? (uint64_t)pr.G * pr.N : (uint64_t)pr.G * p.kblocks * pr.N};
   const uint64_t b_strides[1] = {pr.dense ? (uint64_t)pr.K * esize : (uint64_t)kRowBytes};
-  {
+  if (kBT) {
+    rc = encode_bt_map(&tm_b, pr);
+  } else {
     const uint32_t box[2] = {(uint32_t)elems_per_row, (uint32_t)BN};
     rc = encode_map(&tm_b, dt_a, 2, pr.b, b_dims, b_strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   }
@@ -375,10 +387,10 @@ int launch(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
 }
 
 // Two-CTA (cta_group::2) 256x256 tiles for compute-bound shapes; one cluster per TPC.
-template <int KIND>
+template <int KIND, bool kBT = false>
 int launch_pair(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   using L = PairSmem;
-  auto kernel = grouped_gemm_pair_kernel<KIND>;
+  auto kernel = grouped_gemm_pair_kernel<KIND, kBT>;
   const int esize = (KIND == DG_KIND_BF16) ? 2 : 1;
   const int elems_per_row = kRowBytes / esize;
   KernelParams p{};
@@ -433,7 +445,9 @@ int launch_pair(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
     rc = encode_map(&tm_a, dt_a, 2, pr.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   if (rc != DG_OK) return rc;
-  {
+  if (kBT) {
+    rc = encode_bt_map(&tm_b, pr);
+  } else {
     const uint64_t dims[2] = {pr.dense ? (uint64_t)pr.K : (uint64_t)elems_per_row,
                               pr.dense ? (uint64_t)pr.G * pr.N : (uint64_t)pr.G * p.kblocks * pr.N};
     const uint64_t strides[1] = {pr.dense ? (uint64_t)pr.K * esize : (uint64_t)kRowBytes};
@@ -668,8 +682,10 @@ int validate_and_launch(Problem& pr, cudaStream_t stream) {
   // INT8 / FP8: K % 64 (the reference's W6 block, deepgemm/m_group_gemm.py:815-818).  The kernels step K
   // in 128-byte blocks: the packed weight then carries ceil(K / 128) blocks whose tail is zero
   // (the packers pad it) and TMA fills the activation's last half block with zeros.
-  const int kq = (pr.kind == DG_KIND_W4A8) ? 256 : 64;
-  if (pr.K % kq != 0) return DG_ERR_BAD_SHAPE;
+  // Used transposed, the contraction runs over the weight's rows (16-byte rows of A) and the
+  // columns are whole 64-column blocks.
+  const int kq = pr.b_trans ? 8 : (pr.kind == DG_KIND_W4A8) ? 256 : 64;
+  if (pr.K % kq != 0 || (pr.b_trans && pr.N % 64 != 0)) return DG_ERR_BAD_SHAPE;
   const int kstep = (pr.kind == DG_KIND_BF16) ? 64 : (pr.kind == DG_KIND_W4A8 ? 256 : 128);
   if ((long long)pr.G * ((pr.K + kstep - 1) / kstep) * pr.N > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
   if (pr.M == 0) return DG_OK;
@@ -736,6 +752,11 @@ int validate_and_launch(Problem& pr, cudaStream_t stream) {
     return launch_w4(pr, *dev, stream);
   }
 
+  if (pr.b_trans) {
+    if (bn == 512) return launch_pair<DG_KIND_BF16, true>(pr, *dev, stream);
+    return bn == 256 ? launch<DG_KIND_BF16, 256, false, true>(pr, *dev, stream)
+                     : launch<DG_KIND_BF16, 128, false, true>(pr, *dev, stream);
+  }
   if (bn == 512) {  // two-CTA 256x256 tiles
     switch (pr.kind) {
       case DG_KIND_I8: return launch_pair<DG_KIND_I8>(pr, *dev, stream);
@@ -884,6 +905,28 @@ int dg_contig_gemm(const dg_contig_args* a, void* stream) {
     pr.scatter_base = a->scatter_base;
     pr.scatter_world = a->scatter_world;
   }
+  return validate_and_launch(pr, static_cast<cudaStream_t>(stream));
+}
+
+int dg_grouped_input_grad(const dg_input_grad_args* a, void* stream) {
+  if (a == nullptr) return DG_ERR_NULL_POINTER;
+  if (a->n < 16 || a->n % 16 != 0) return DG_ERR_BAD_SHAPE;
+  if (a->block_n != 0 && a->block_n != 128 && a->block_n != 256 && a->block_n != 512) return DG_ERR_BAD_ARGUMENT;
+  Problem pr{};
+  pr.kind = DG_KIND_BF16;
+  pr.scale_mode = DG_SCALE_NONE;
+  pr.mode = MODE_CONTIG;
+  pr.b_trans = 1;
+  pr.a = a->dy;
+  pr.b = a->w_packed;
+  pr.d = a->dx;
+  pr.sched = a->m_indices;
+  pr.G = a->num_groups;
+  pr.M = a->m_total;
+  pr.N = a->k;
+  pr.K = a->n;
+  pr.block_n = a->block_n;
+  pr.status = a->status;
   return validate_and_launch(pr, static_cast<cudaStream_t>(stream));
 }
 

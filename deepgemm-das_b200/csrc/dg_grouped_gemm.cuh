@@ -497,7 +497,13 @@ struct ItemDecoder {
 // tile by index (the other instantiations carry none of that code).
 constexpr int kGatherThreads = 128;
 constexpr int kGatherDepth = 2;  // K blocks a gathering thread keeps in flight behind the one it issues
-template <int KIND, int BN, int STAGES, bool kGather = false>
+// kBT: the weight is used the other way round (gradient of the rows): D[row][c] = sum_n A[row][n] *
+// W[n][c], c running along the packed weight's 64-column blocks.  packed[g][c / 64][n][c % 64] is,
+// read with n as the contraction, an operand stored along N: a box of 64 columns x 64 rows lands
+// as the tensor cores want it, so the forward weight needs no second copy.  p.N is then the row
+// length of D and p.kblocks counts 64-value blocks of n.  BF16 only.
+constexpr uint32_t kBTBlockBytes = 64 * kRowBytes;  // 64 columns x 64 values of n
+template <int KIND, int BN, int STAGES, bool kGather = false, bool kBT = false>
 __global__ void __launch_bounds__(SmemLayout<KIND, BN, STAGES>::kThreads + (kGather ? kGatherThreads : 0), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_a64,
@@ -512,8 +518,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
       (KIND == DG_KIND_E4M3) ? UMMA_F8F6F4 : (KIND == DG_KIND_BF16 ? UMMA_F16 : UMMA_I8);
   constexpr bool kIntAcc = (KIND == DG_KIND_I8);
   constexpr int kElemsPerRow = (KIND == DG_KIND_BF16) ? 64 : 128;  // A elements per 128 bytes
+  static_assert(!kBT || KIND == DG_KIND_BF16, "weights are used transposed in bf16 only");
   constexpr uint32_t kIdesc =
-      umma_idesc(kIntAcc ? 2u : 1u, (KIND == DG_KIND_E4M3) ? 0u : 1u, kBM, BN);
+      umma_idesc(kIntAcc ? 2u : 1u, (KIND == DG_KIND_E4M3) ? 0u : 1u, kBM, BN) | (kBT ? kIdescBMn : 0u);
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -831,10 +838,17 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tma_load_3d(a_dst, tm_act, bar_full(s), kb * kElemsPerRow, t.row0, t.g, pol_a);
               else
                 tma_load_2d(a_dst, tm_act, bar_full(s), kb * kElemsPerRow, t.row0, pol_a);
-              int bx, by;
-              weight_coords(p, t.g, t.n0, kb, kElemsPerRow, bx, by);
-              tma_load_2d(base + L::off_b + s * L::kBStage + j * sh.b_stride, tm_w, bar_full(s), bx,
-                          by, pol_b);
+              if constexpr (kBT) {
+#pragma unroll
+                for (int c = 0; c < BN / 64; ++c)
+                  tma_load_3d(base + L::off_b + s * L::kBStage + c * kBTBlockBytes, tm_w, bar_full(s), 0,
+                              kb * 64, t.g * (p.N / 64) + t.n0 / 64 + c, pol_b);
+              } else {
+                int bx, by;
+                weight_coords(p, t.g, t.n0, kb, kElemsPerRow, bx, by);
+                tma_load_2d(base + L::off_b + s * L::kBStage + j * sh.b_stride, tm_w, bar_full(s), bx,
+                            by, pol_b);
+              }
             }
           }
         }
@@ -887,12 +901,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
             for (int j = 0; j < nb; ++j) {
               const uint64_t a_desc = umma_desc_sw128(base + L::off_a + s * L::kAStage +
                                                       (kNarrow ? j * sh.a_stride : 0u));
-              const uint64_t b_desc = umma_desc_sw128(base + L::off_b + s * L::kBStage +
-                                                      (kNarrow ? j * sh.b_stride : 0u));
+              const uint64_t b_desc =
+                  kBT ? umma_desc_mn_sw128(base + L::off_b + s * L::kBStage, kBTBlockBytes)
+                      : umma_desc_sw128(base + L::off_b + s * L::kBStage + (kNarrow ? j * sh.b_stride : 0u));
+              constexpr uint32_t kBStep = kBT ? 2048 / 16 : 2;
 #pragma unroll
               for (int k = 0; k < kRowBytes / 32; ++k) {
                 // +2 in the start-address field = +32 bytes along K inside the swizzled row
-                umma_ss<kUmmaKind>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc,
+                umma_ss<kUmmaKind>(d_tmem, a_desc + 2u * k, b_desc + kBStep * k, idesc,
                                    (kb0 | j | k) != 0 ? 1u : 0u);
               }
             }

@@ -90,7 +90,9 @@ struct PairDecoder {
   }
 };
 
-template <int KIND>
+// kBT: the weight is used the other way round, as in the one-CTA kernel; each block then holds 128
+// of the tile's columns as two 64-column boxes.
+template <int KIND, bool kBT = false>
 __global__ void __launch_bounds__(PairSmem::kThreads, 1)
 grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_b, const KernelParams p) {
@@ -100,8 +102,9 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
       (KIND == DG_KIND_E4M3) ? UMMA_F8F6F4 : (KIND == DG_KIND_BF16 ? UMMA_F16 : UMMA_I8);
   constexpr bool kIntAcc = (KIND == DG_KIND_I8);
   constexpr int kElemsPerRow = (KIND == DG_KIND_BF16) ? 64 : 128;
+  static_assert(!kBT || KIND == DG_KIND_BF16, "weights are used transposed in bf16 only");
   constexpr uint32_t kIdesc =
-      umma_idesc(kIntAcc ? 2u : 1u, (KIND == DG_KIND_E4M3) ? 0u : 1u, 256, kPairBN);
+      umma_idesc(kIntAcc ? 2u : 1u, (KIND == DG_KIND_E4M3) ? 0u : 1u, 256, kPairBN) | (kBT ? kIdescBMn : 0u);
   constexpr uint32_t kStageBytes = kATileBytes + L::kBHalfBytes;
 
   extern __shared__ uint8_t smem_raw[];
@@ -254,9 +257,16 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
             tma_load_3d_pair(a_dst, &tm_a, full_leader, kb * kElemsPerRow, a_row, t.g, pol_a);
           else
             tma_load_2d_pair(a_dst, &tm_a, full_leader, kb * kElemsPerRow, a_row, pol_a);
-          int bx, by;
-          weight_coords(p, t.g, b_n0, kb, kElemsPerRow, bx, by);
-          tma_load_2d_pair(b_dst, &tm_b, full_leader, bx, by, pol_b);
+          if constexpr (kBT) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              tma_load_3d_pair(b_dst + c * kBTBlockBytes, &tm_b, full_leader, 0, kb * 64,
+                               t.g * (p.N / 64) + b_n0 / 64 + c, pol_b);
+          } else {
+            int bx, by;
+            weight_coords(p, t.g, b_n0, kb, kElemsPerRow, bx, by);
+            tma_load_2d_pair(b_dst, &tm_b, full_leader, bx, by, pol_b);
+          }
         }
       }
       if (rank == 0) {
@@ -318,10 +328,12 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
             tc_fence_after_sync();
           }
           const uint64_t a_desc = umma_desc_sw128(base + L::off_a + s * kATileBytes);
-          const uint64_t b_desc = umma_desc_sw128(base + L::off_b + s * L::kBHalfBytes);
+          const uint64_t b_desc = kBT ? umma_desc_mn_sw128(base + L::off_b + s * L::kBHalfBytes, kBTBlockBytes)
+                                      : umma_desc_sw128(base + L::off_b + s * L::kBHalfBytes);
+          constexpr uint32_t kBStep = kBT ? 2048 / 16 : 2;
 #pragma unroll
           for (int k = 0; k < kRowBytes / 32; ++k)
-            umma_ss_pair<kUmmaKind>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, kIdesc,
+            umma_ss_pair<kUmmaKind>(d_tmem, a_desc + 2u * k, b_desc + kBStep * k, kIdesc,
                                     (kb | k) != 0 ? 1u : 0u);
           umma_commit_pair(bar_empty(s), 3);
         }

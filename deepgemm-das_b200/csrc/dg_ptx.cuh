@@ -225,6 +225,16 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for an operand tile stored along M (or N): rows of 128 bytes hold 64 16-bit values of
+// the M/N dimension for one value of K, eight K values are 1024 bytes (a swizzle atom), the next
+// eight K values follow at SBO = 1024, the next 64 values of M/N at LBO = `mn_stride` bytes.  This
+// is what a SWIZZLE_128B TMA box of 64 values x 64 rows leaves when the rows run along K.
+// Stepping 16 values along K adds 2048 bytes to the start address.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t mn_stride) {
+  return umma_desc_sw128(smem_addr) | (static_cast<uint64_t>(mn_stride >> 4) << 16);
+}
+constexpr uint32_t kIdescAMn = 1u << 15, kIdescBMn = 1u << 16;  // the operand is stored along M / N
+
 // Instruction descriptor (upper 32 bits of the UMMA "idesc"): dense, no negate, A and B
 // both K-major.  c_fmt: 1 = f32, 2 = s32.  ab_fmt: kind::i8 1 = signed 8-bit;
 // kind::f8f6f4 0 = e4m3; kind::f16 1 = bf16.

@@ -1,0 +1,120 @@
+// C ABI of the weight gradient of the grouped GEMM: argument checks, tensor maps, launch.
+#include "dg_host.h"
+#include "dg_grouped_wgrad.cuh"
+
+namespace {
+
+using namespace dg;
+using namespace dg::host;
+
+template <int CL>
+int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& dev, cudaStream_t stream) {
+  auto kernel = grouped_wgrad_kernel<CL>;
+  constexpr int BT = 128 * CL;
+  p.n_tiles = (p.N + BT - 1) / BT;
+  p.k_tiles = (p.K + BT - 1) / BT;
+  const long long items = (long long)p.G * p.n_tiles * p.k_tiles;
+  if (items > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
+  const int smem = WgradSmem::total(p.G, p.m_blocks);
+  if (smem > dev.max_smem) return DG_ERR_TOO_LARGE;
+
+  CUtensorMap tm_dy, tm_x, tm_d;
+  const uint32_t box[2] = {64u, 64u};
+  // Without rows nothing is loaded; the maps then describe one row that is never read.
+  const uint64_t rows = p.M > 0 ? p.M : 1;
+  const void* dy = p.M > 0 ? a->dy : a->dw;
+  const void* x = p.M > 0 ? a->x : a->dw;
+  const uint64_t dy_dims[2] = {(uint64_t)p.N, rows}, x_dims[2] = {(uint64_t)p.K, rows};
+  const uint64_t dy_str[1] = {(uint64_t)p.N * 2}, x_str[1] = {(uint64_t)p.K * 2};
+  int rc = encode_map(&tm_dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, dy_dims, dy_str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == DG_OK)
+    rc = encode_map(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_dims, x_str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t es = p.f32 ? 4 : 2;
+  const uint64_t d_dims[3] = {64u, (uint64_t)p.N, (uint64_t)p.G * (p.K / 64)};
+  const uint64_t d_str[2] = {64 * es, 64 * es * p.N};
+  const uint32_t d_box[3] = {p.f32 ? 32u : 64u, 32u, 1u};
+  if (rc == DG_OK)
+    rc = encode_map(&tm_d, p.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a->dw, d_dims, d_str,
+                    d_box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != DG_OK) return rc;
+
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kWgThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+
+  // Once per device: opt in to the shared-memory size and ask how many clusters fit at once.
+  static std::mutex mu;
+  static int max_units[kMaxDevices] = {0};
+  int devid = 0;
+  cudaGetDevice(&devid);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (max_units[devid] == 0) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem);
+      if (e != cudaSuccess) return cuda_fail(e);
+      cudaLaunchConfig_t q = cfg;
+      q.gridDim = dim3(dev.sm_count / CL * CL, 1, 1);
+      q.dynamicSmemBytes = dev.max_smem;
+      int n = 0;
+      e = cudaOccupancyMaxActiveClusters(&n, kernel, &q);
+      if (e != cudaSuccess) return cuda_fail(e);
+      if (n < 1) return DG_ERR_TOO_LARGE;
+      max_units[devid] = n < dev.sm_count / CL ? n : dev.sm_count / CL;
+    }
+  }
+  const long long units = items < max_units[devid] ? items : max_units[devid];
+  cfg.gridDim = dim3(static_cast<unsigned>(CL * units), 1, 1);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm_dy, tm_x, tm_d, p);
+  if (e != cudaSuccess) return cuda_fail(e);
+  count_launches(1);
+  return DG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
+  if (a == nullptr) return DG_ERR_NULL_POINTER;
+  if (a->num_groups < 1 || a->m_total < 0 || a->n < 16 || a->n % 16 != 0 || a->k < 64 || a->k % 64 != 0) return DG_ERR_BAD_SHAPE;
+  if (a->out_kind != DG_OUT_BF16 && a->out_kind != DG_OUT_F32) return DG_ERR_BAD_ARGUMENT;
+  if (a->accumulate != 0 && a->out_kind != DG_OUT_F32) return DG_ERR_BAD_ARGUMENT;  // sums are kept in 32 bits
+  if (a->tile != 0 && a->tile != 128 && a->tile != 256) return DG_ERR_BAD_ARGUMENT;
+  if (a->num_groups > DG_MAX_GROUPS || a->m_total > DG_MAX_CONTIG_ROWS) return DG_ERR_TOO_LARGE;
+  if ((long long)a->num_groups * (a->k / 64) > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
+  if (!a->dw || (a->m_total > 0 && (!a->dy || !a->x || !a->m_indices))) return DG_ERR_NULL_POINTER;
+  if (!aligned16(a->dy) || !aligned16(a->x) || !aligned16(a->dw)) return DG_ERR_BAD_ALIGNMENT;
+  if (a->m_total == 0 && a->accumulate) return DG_OK;
+  const DeviceInfo* dev = nullptr;
+  const int rc = device_info(&dev);
+  if (rc != DG_OK) return rc;
+  WgradParams p{};
+  p.G = a->num_groups;
+  p.M = a->m_total;
+  p.N = a->n;
+  p.K = a->k;
+  p.m_blocks = (a->m_total + 127) / 128;
+  p.m_indices = a->m_indices;
+  p.status = a->status;
+  p.f32 = a->out_kind == DG_OUT_F32;
+  p.add = a->accumulate != 0;
+  int tile = a->tile;
+  if (tile == 0) {
+    // 256 x 256 tiles move half the operand bytes per product; 128 x 128 ones give four times the
+    // work items, which small problems need to reach every SM.
+    const long long items = (long long)p.G * ((p.N + 255) / 256) * ((p.K + 255) / 256);
+    tile = items >= dev->sm_count / 2 ? 256 : 128;
+  }
+  return tile == 256 ? launch_wgrad<2>(a, p, *dev, static_cast<cudaStream_t>(stream))
+                     : launch_wgrad<1>(a, p, *dev, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

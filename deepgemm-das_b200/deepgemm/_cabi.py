@@ -37,6 +37,8 @@ EXPORTED_SYMBOLS = (
     "dg_ep_plan",
     "dg_ep_push",
     "dg_ep_barrier",
+    "dg_grouped_input_grad",
+    "dg_grouped_weight_grad",
     "dg_token_sort_capacity",
     "dg_token_sort_scratch_bytes",
     "dg_token_sort",
@@ -317,6 +319,40 @@ class EpBarrierArgs(C.Structure):
 MAX_GROUPS, MAX_TOP_K = 1024, 128
 
 
+class InputGradArgs(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p),
+        ("w_packed", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("m_indices", C.c_void_p),
+        ("num_groups", C.c_int32),
+        ("m_total", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("block_n", C.c_int32),
+        ("reserved", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
+class WeightGradArgs(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p),
+        ("x", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("m_indices", C.c_void_p),
+        ("num_groups", C.c_int32),
+        ("m_total", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("out_kind", C.c_int32),
+        ("accumulate", C.c_int32),
+        ("tile", C.c_int32),
+        ("reserved", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
 class TokenSortArgs(C.Structure):
     _fields_ = [
         ("elem_bytes", C.c_int32),
@@ -473,7 +509,8 @@ def _load() -> C.CDLL:
     lib.dg_token_sort_capacity.restype = C.c_int64
     lib.dg_token_sort_scratch_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32]
     lib.dg_token_sort_scratch_bytes.restype = C.c_size_t
-    for fn, args in ((lib.dg_token_sort, TokenSortArgs), (lib.dg_token_unsort, TokenUnsortArgs),
+    for fn, args in ((lib.dg_grouped_input_grad, InputGradArgs), (lib.dg_grouped_weight_grad, WeightGradArgs),
+                     (lib.dg_token_sort, TokenSortArgs), (lib.dg_token_unsort, TokenUnsortArgs),
                      (lib.dg_token_unsort_grad, TokenUnsortGradArgs), (lib.dg_clear_padding_rows, ClearRowsArgs),
                      (lib.dg_checkpoint_rows, CheckpointArgs), (lib.dg_restore_rows, CheckpointArgs),
                      (lib.dg_act_checkpoint, ActCheckpointArgs), (lib.dg_act_checkpoint_grad, ActCheckpointArgs)):

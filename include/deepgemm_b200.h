@@ -579,9 +579,51 @@ typedef struct dg_ep_barrier_args {
  * own call with the same epoch (system-scope fence, signal, bounded wait; one tiny kernel). */
 DG_API int dg_ep_barrier(const dg_ep_barrier_args* args, void* stream);
 
+/* Gradient of the rows of the contiguous BF16 grouped GEMM (dg_contig_gemm with DG_KIND_BF16), on
+ * the weight that the forward pass uses, in the layout it has there:
+ *   dx[i][c] = bf16( sum over r of dy[i][r] * W[m_indices[i]][r][c] ),  W[g][r][c] = packed[g][c / 64][r][c % 64]
+ * m_indices names one group for every 128 rows, as there; rows with m_indices < 0 are not written. */
+typedef struct dg_input_grad_args {
+  const void*    dy;        /* [m_total][n] bf16 */
+  const void*    w_packed;  /* [num_groups][k / 64][n][64] bf16 */
+  void*          dx;        /* [m_total][k] bf16 */
+  const int32_t* m_indices; /* [m_total] */
+  int32_t num_groups;
+  int32_t m_total;
+  int32_t n;                /* rows of a group's weight, multiple of 16 */
+  int32_t k;                /* its columns, multiple of 64 */
+  int32_t block_n;          /* 0 = choose; 128 / 256 = one-CTA tile width; 512 = two-CTA 256x256 tiles */
+  int32_t reserved;
+  int32_t*       status;    /* NULL, or int32[DG_STATUS_WORDS] */
+} dg_input_grad_args;
+DG_API int dg_grouped_input_grad(const dg_input_grad_args* args, void* stream);
+
+/* Gradient of the weights of the contiguous BF16 grouped GEMM, in the packed layout of the weight:
+ *   dW[g][r][c] = sum over i with m_indices[i] = g of dy[i][r] * x[i][c],  dw[g][c / 64][r][c % 64]
+ * in fp32, rounded once (DG_OUT_BF16) or not at all (DG_OUT_F32; there `accumulate` adds to what dw
+ * holds, every value once, so the result does not depend on an order).  m_indices names one group
+ * for every 128 rows (the group of their first row); rows of them with another entry count for
+ * nothing, whatever they hold.  Groups without rows give zeros. */
+typedef struct dg_weight_grad_args {
+  const void*    dy;        /* [m_total][n] bf16 */
+  const void*    x;         /* [m_total][k] bf16 */
+  void*          dw;        /* [num_groups][k / 64][n][64] */
+  const int32_t* m_indices; /* [m_total] */
+  int32_t num_groups;
+  int32_t m_total;
+  int32_t n;                /* multiple of 16 */
+  int32_t k;                /* multiple of 64 */
+  int32_t out_kind;         /* DG_OUT_BF16 or DG_OUT_F32 */
+  int32_t accumulate;       /* DG_OUT_F32 only */
+  int32_t tile;             /* 0 = choose; 128 / 256 */
+  int32_t reserved;
+  int32_t*       status;    /* NULL, or int32[DG_STATUS_WORDS] */
+} dg_weight_grad_args;
+DG_API int dg_grouped_weight_grad(const dg_weight_grad_args* args, void* stream);
+
 /* ---------------------------------------------------------------------------------------
  * A training step of an MoE layer: tokens sorted by expert and back, activation checkpoints in
- * 8 bits.  (The gradients of the grouped product itself are declared further down.)  The reference
+ * 8 bits.  (The gradients of the grouped product itself are declared above.)  The reference
  * library is forward only; these are additions of this library.
  * Element types (`elem`): DG_OUT_BF16, DG_OUT_F16 or DG_OUT_F32.  Rows may lie apart (`*_stride`,
  * in elements); any row length is taken, multiples of 8 on 16-byte boundaries are fastest.

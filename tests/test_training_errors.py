@@ -11,7 +11,8 @@ import deepgemm
 from deepgemm import _cabi
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-STRUCTS = {"dg_token_sort_args": _cabi.TokenSortArgs, "dg_token_unsort_args": _cabi.TokenUnsortArgs,
+STRUCTS = {"dg_input_grad_args": _cabi.InputGradArgs, "dg_weight_grad_args": _cabi.WeightGradArgs,
+           "dg_token_sort_args": _cabi.TokenSortArgs, "dg_token_unsort_args": _cabi.TokenUnsortArgs,
            "dg_token_unsort_grad_args": _cabi.TokenUnsortGradArgs, "dg_clear_rows_args": _cabi.ClearRowsArgs,
            "dg_checkpoint_args": _cabi.CheckpointArgs, "dg_act_checkpoint_args": _cabi.ActCheckpointArgs}
 
@@ -52,7 +53,7 @@ def test_sort_refuses(over, code):
 
 
 def test_null_arguments():
-    for name in ("dg_token_sort", "dg_token_unsort", "dg_token_unsort_grad", "dg_clear_padding_rows", "dg_checkpoint_rows",
+    for name in ("dg_grouped_input_grad", "dg_grouped_weight_grad", "dg_token_sort", "dg_token_unsort", "dg_token_unsort_grad", "dg_clear_padding_rows", "dg_checkpoint_rows",
                  "dg_restore_rows", "dg_act_checkpoint", "dg_act_checkpoint_grad"):
         assert call(name, None) == -1
 
@@ -90,6 +91,21 @@ def test_checkpoints_refuse():
             assert call(entry, _cabi.ActCheckpointArgs(**{**a, **over})) == code, (entry, over)
 
 
+def test_gradients_of_the_product_refuse():
+    i = dict(dy=4096, w_packed=4096, dx=4096, m_indices=4096, num_groups=2, m_total=128, n=64, k=128)
+    for over, code in ((dict(n=8), -3), (dict(n=72), -3), (dict(k=96), -3), (dict(k=0), -3), (dict(num_groups=0), -3), (dict(m_total=-1), -3),
+                       (dict(num_groups=1025), -8), (dict(m_total=4096 * 128 + 1), -8), (dict(block_n=64), -9), (dict(dy=None), -1),
+                       (dict(w_packed=None), -1), (dict(dx=None), -1), (dict(m_indices=None), -1), (dict(dy=4104), -4), (dict(dx=4098), -4)):
+        assert call("dg_grouped_input_grad", _cabi.InputGradArgs(**{**i, **over})) == code, over
+    assert call("dg_grouped_input_grad", _cabi.InputGradArgs(**{**i, "m_total": 0})) == 0
+    w = dict(dy=4096, x=4096, dw=4096, m_indices=4096, num_groups=2, m_total=128, n=64, k=128)
+    for over, code in ((dict(n=8), -3), (dict(n=72), -3), (dict(k=96), -3), (dict(num_groups=0), -3), (dict(num_groups=1025), -8),
+                       (dict(m_total=4096 * 128 + 1), -8), (dict(tile=64), -9), (dict(out_kind=1), -9), (dict(accumulate=1), -9),
+                       (dict(dy=None), -1), (dict(x=None), -1), (dict(dw=None), -1), (dict(m_indices=None), -1), (dict(x=4104), -4)):
+        assert call("dg_grouped_weight_grad", _cabi.WeightGradArgs(**{**w, **over})) == code, over
+    assert call("dg_grouped_weight_grad", _cabi.WeightGradArgs(**{**w, "m_total": 0, "out_kind": 2, "accumulate": 1})) == 0
+
+
 def test_capacity():
     for pairs, experts, align in ((0, 4, 128), (1, 4, 128), (8, 256, 1), (8, 256, 128), (1000, 3, 16), (7, 7, 5)):
         got = deepgemm.sort_capacity(pairs, experts, align)
@@ -108,7 +124,9 @@ def test_python_functions_refuse_cpu_tensors():
     ids = torch.zeros(4, 2, dtype=torch.int32)
     plan = deepgemm.TokenPlan(ids, torch.zeros(8, dtype=torch.int32), None, None, None)
     c = deepgemm.Checkpoint(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4, 1), torch.bfloat16)
-    for f in (lambda: deepgemm.sort_tokens(x, ids, 4), lambda: deepgemm.unsort_tokens(x, plan), lambda: deepgemm.sort_tokens_grad(x, plan),
+    w = torch.zeros(1, 1, 64, 64, dtype=torch.bfloat16)
+    for f in (lambda: deepgemm.grouped_bf16_input_grad(x, w, ids[:, 0]), lambda: deepgemm.grouped_bf16_weight_grad(x, x, ids[:, 0], 1),
+              lambda: deepgemm.sort_tokens(x, ids, 4), lambda: deepgemm.unsort_tokens(x, plan), lambda: deepgemm.sort_tokens_grad(x, plan),
               lambda: deepgemm.unsort_tokens_grad(x, x, plan), lambda: deepgemm.clear_padding_rows(x, ids[:, 0]),
               lambda: deepgemm.checkpoint_rows(x), lambda: deepgemm.restore_rows(c), lambda: deepgemm.silu_mul_checkpoint(x),
               lambda: deepgemm.silu_mul_checkpoint_grad(c, x), lambda: deepgemm.silu_mul(x)):
