@@ -14,15 +14,21 @@
 // for problems with few tiles.  Either way a ring stage holds 64 rows of 128 columns of each
 // operand (32 KB), six stages.  A work item is (group, tile); its contraction walks the 128-row
 // blocks of the group in ascending order, 64 rows (a chunk) at a time.
-//   warp 0      TMA producer (each block its own copies, completing on its own stage-full barrier)
+//   warp 0      TMA producer (each block its own copies)
 //   warp 1      UMMA issuer (leader)
 //   warps 2..5  epilogue: accumulator -> bf16 or fp32 -> 32-row strip in shared memory -> TMA store
 //               (or TMA reduce-add, when the gradient is added to what is there)
-//   warp 6      row filter: looks at the m_indices of each chunk before the tensor cores do.  Rows
-//               that stand for nothing (padding, rows behind the last group) are set to zero in
-//               shared memory, in both operands, so that whatever they held (NaN, infinities) does
-//               not reach a sum; of a chunk's four 16-row steps only those that end in a row of the
-//               group are issued.  It passes the stage on through a second barrier.
+//   warp 6      row filter.  Rows that stand for nothing (padding, rows behind the last group) are
+//               set to zero in shared memory, in both operands, so that whatever they held (NaN,
+//               infinities) does not reach a sum; of a chunk's four 16-row steps only those up to
+//               its last row are issued, and a block's second chunk is left out when it is empty.
+// A chunk whose 64 rows all count, i.e. nearly every one, goes straight to the tensor cores: the
+// copies of both blocks complete on the leader's `ready` barrier.  Only the others complete on their
+// own block's `full` barrier, for the filter, which then arrives on `ready` in the producers' place.
+// (With the filter between every chunk and its products, each stage paid a remote arrival with
+// cluster-wide release and an acquire to match: 1.0 us a chunk, whatever the tensor cores did.)
+// Which rows count is known beforehand: every block of the grid reads all of m_indices once (from
+// L2) and keeps a byte for each 128 rows.
 // Groups without rows give zeros (or, added, nothing) and cost no products.
 //
 // Every mbarrier wait is bounded, as in the other kernels.
@@ -39,6 +45,8 @@ constexpr int kWgThreads = 224;
 constexpr uint32_t kWgBoxBytes = 64 * 128;         // 64 columns x 64 rows
 constexpr uint32_t kWgOperand = 2 * kWgBoxBytes;   // 128 columns x 64 rows
 constexpr uint32_t kWgStageBytes = 2 * kWgOperand;
+
+constexpr int kWgIrregular = 255;  // rows that count lie between others: looked up where they are used
 
 enum : int { WG_SITE_EMPTY = 21, WG_SITE_FILTER = 22, WG_SITE_READY = 23, WG_SITE_ACC_EMPTY = 24, WG_SITE_ACC_FULL = 25 };
 
@@ -61,42 +69,20 @@ struct WgradSmem {
   static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort
   static constexpr int off_steps = off_misc + 16;          // per stage: 16-row steps to issue
   static constexpr int off_table = off_steps + kWgStages * 4;
-  // table: first[G + 1] (int32) and the group's 128-row blocks in order (uint16)
+  // table: first[G + 1] (int32), the groups' 128-row blocks in order (uint16), rows that count (uint8)
   __host__ __device__ static constexpr int total(int groups, int blocks) {
-    return off_table + (groups + 1) * 4 + ((blocks * 2 + 15) & ~15) + 1024;
+    return off_table + (groups + 1) * 4 + blocks * 3 + 16 + 1024;
   }
   // The table is built from m_indices[128 b] of every block b, held as int16 in the (still empty) ring.
   static_assert(kWgStages * static_cast<int>(kWgStageBytes) >= DG_MAX_CONTIG_ROWS / 128 * 2, "");
 };
 
-__device__ __forceinline__ bool wg_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
-  auto look = [&]() {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-  };
-#pragma unroll 1
-  for (int i = 0; i < 128; ++i)
-    if (look()) return true;
-  const uint64_t t0 = global_timer_ns();
-#pragma unroll 1
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (look()) return true;
-    if (*abort_flag) return false;
-    if (global_timer_ns() - t0 > 1500000000ull) {
-      *abort_flag = site;
-      return false;
-    }
-  }
+// An arrival on another block's mbarrier that orders nothing (the copies it announces are ordered by
+// the barrier's byte count).
+__device__ __forceinline__ void wg_arrive_remote_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+__device__ __forceinline__ void wg_fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 __device__ __forceinline__ void wg_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
@@ -142,12 +128,13 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   volatile int* steps_s = reinterpret_cast<volatile int*>(smem + L::off_steps);
   int32_t* first = reinterpret_cast<int32_t*>(smem + L::off_table);
   uint16_t* blocks = reinterpret_cast<uint16_t*>(first + p.G + 1);
+  uint8_t* valid = reinterpret_cast<uint8_t*>(blocks + p.m_blocks);  // of each 128-row block
 
   if (tid == 0) {
     *abort_flag = 0;
     for (int s = 0; s < S; ++s) {
       mbar_init(bar_full(s), 1);
-      mbar_init(bar_ready(s), CL);  // the filter warp of each block
+      mbar_init(bar_ready(s), CL);  // the producer of each block, or its filter
       mbar_init(bar_empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -167,12 +154,33 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     for (int g = tid; g <= p.G; g += kWgThreads) first[g] = 0;
     __syncthreads();
     bool bad = false;
-    for (int b = tid; b < p.m_blocks; b += kWgThreads) {
-      const int e = p.m_indices[(size_t)b * 128];
-      bad |= e >= p.G;
-      const bool in = e >= 0 && e < p.G;
-      of_block[b] = static_cast<int16_t>(in ? e : -1);
-      if (in) atomicAdd(&first[e], 1);
+#pragma unroll 4
+    for (int b = warp; b < p.m_blocks; b += kWgThreads / 32) {
+      int m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = b * 128 + 32 * i + lane;
+        m[i] = row < p.M ? __ldg(p.m_indices + row) : -1;
+      }
+      const int e = __shfl_sync(0xffffffffu, m[0], 0);
+      uint32_t in_group[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) in_group[i] = __ballot_sync(0xffffffffu, m[i] == e);
+      if (lane == 0) {
+        const bool in = e >= 0 && e < p.G;
+        bad |= e >= p.G;
+        // rows 0 .. n - 1 and no others?
+        const int n = __popc(in_group[0]) + __popc(in_group[1]) + __popc(in_group[2]) + __popc(in_group[3]);
+        bool prefix = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int here = max(0, min(32, n - 32 * i));
+          prefix &= in_group[i] == (here == 32 ? 0xffffffffu : (1u << here) - 1u);
+        }
+        of_block[b] = static_cast<int16_t>(in ? e : -1);
+        valid[b] = static_cast<uint8_t>(prefix ? n : kWgIrregular);
+        if (in) atomicAdd(&first[e], 1);
+      }
     }
     if (bad && blockIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, DG_DEV_OK, DG_DEV_BAD_GROUP_INDEX);
     __syncthreads();
@@ -242,6 +250,10 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     return it;
   };
 
+  // Rows that count in half c & 1 of a block with the table's entry n: 0 (left out), 1..63, 64, or
+  // kWgIrregular.
+  auto rows_of = [&](int n, int c) { return n == kWgIrregular ? n : max(0, min(64, n - 64 * (c & 1))); };
+
   if (warp == 0) {
     if (lane == 0) {
       // ---- TMA producer
@@ -250,20 +262,40 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
         const Item w = item_of(item);
-        for (int c = 0; c < w.chunks; ++c, ++it) {
+        for (int c = 0; c < w.chunks; ++c) {
+          const int b = blocks[w.b0 + (c >> 1)];
+          const int rows = rows_of(valid[b], c);
+          if (rows == 0) continue;
           const int s = it % S;
           if (!mbar_wait_bounded(bar_empty(s), ((it / S) & 1u) ^ 1u, abort_flag, WG_SITE_EMPTY)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(bar_full(s), kWgStageBytes);
-          const int row = blocks[w.b0 + (c >> 1)] * 128 + (c & 1) * 64;
+          ++it;
+          const int row = b * 128 + (c & 1) * 64;
           const uint32_t dst = base + L::off_stage + s * kWgStageBytes;
           const int n = w.n0 + static_cast<int>(rank) * 128, k = w.k0 + static_cast<int>(rank) * 128;
+          if (rows == 64) {
+            uint32_t bar = bar_ready(s);
+            if constexpr (CL == 2) {
+              bar = mapa_shared(bar, 0);
+              if (rank == 0) mbar_arrive_expect_tx(bar_ready(s), 2 * kWgStageBytes); else wg_arrive_remote_relaxed(bar);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(dst + i * kWgBoxBytes, &tm_dy, bar, n + 64 * i, row, pol);
+                tma_load_2d_pair(dst + kWgOperand + i * kWgBoxBytes, &tm_x, bar, k + 64 * i, row, pol);
+              }
+              continue;
+            }
+            mbar_arrive_expect_tx(bar, kWgStageBytes);
+          } else {
+            mbar_arrive_expect_tx(bar_full(s), kWgStageBytes);
+          }
+          const uint32_t bar = rows == 64 ? bar_ready(s) : bar_full(s);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            tma_load_2d(dst + i * kWgBoxBytes, &tm_dy, bar_full(s), n + 64 * i, row, pol);
-            tma_load_2d(dst + kWgOperand + i * kWgBoxBytes, &tm_x, bar_full(s), k + 64 * i, row, pol);
+            tma_load_2d(dst + i * kWgBoxBytes, &tm_dy, bar, n + 64 * i, row, pol);
+            tma_load_2d(dst + kWgOperand + i * kWgBoxBytes, &tm_x, bar, k + 64 * i, row, pol);
           }
         }
       }
@@ -277,22 +309,26 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
         const Item w = item_of(item);
         if (w.chunks == 0) continue;
         const uint32_t buf = tile & 1u;
-        if (!wg_wait_cluster(bar_acc_empty(buf), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
+        if (!mbar_wait_bounded(bar_acc_empty(buf), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * BT;
-        for (int c = 0; c < w.chunks; ++c, ++it) {
+        for (int c = 0; c < w.chunks; ++c) {
+          const int rows = rows_of(valid[blocks[w.b0 + (c >> 1)]], c);
+          if (rows == 0) continue;
           const int s = it % S;
-          if (!wg_wait_cluster(bar_ready(s), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
+          if (!mbar_wait_bounded(bar_ready(s), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
             ok = false;
             break;
           }
+          ++it;
+          if (rows != 64) wg_fence_cluster();  // both filters' writes
           tc_fence_after_sync();
-          const int steps = steps_s[s];
+          const int steps = rows == kWgIrregular ? steps_s[s] : (rows + 15) / 16;
           const uint32_t at = base + L::off_stage + s * kWgStageBytes;
           const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
           const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
           for (int k = 0; k < steps; ++k) {  // 16 rows each: 2048 bytes on in every box
-            const uint32_t acc = (c | k) != 0 ? 1u : 0u;
+            const uint32_t acc = (c | k) != 0 ? 1u : 0u;  // (a block's first chunk always has rows)
             if constexpr (CL == 2)
               umma_ss_pair<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
             else
@@ -313,37 +349,39 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     }
   } else if (warp == 6) {
     // ---- row filter
-    uint32_t it = 0;
+    uint32_t it = 0, phase = 0;  // bit s: parity of the next use of stage s's full barrier
     bool ok = true;
     for (int item = unit; ok && item < n_items; item += units) {
       const Item w = item_of(item);
-      int e0 = -1, e1 = -1;
-      auto fetch = [&](int c) {  // the m_indices of a chunk, a chunk ahead of their use
-        e0 = e1 = -1;
-        if (c < w.chunks) {
-          const int row = blocks[w.b0 + (c >> 1)] * 128 + (c & 1) * 64;
-          if (row + lane < p.M) e0 = __ldg(p.m_indices + row + lane);
-          if (row + 32 + lane < p.M) e1 = __ldg(p.m_indices + row + 32 + lane);
-        }
-      };
-      fetch(0);
-      for (int c = 0; c < w.chunks; ++c, ++it) {
+      for (int c = 0; c < w.chunks; ++c) {
+        const int b = blocks[w.b0 + (c >> 1)];
+        int rows = rows_of(valid[b], c);
+        if (rows == 0) continue;
         const int s = it % S;
-        const uint32_t lo = __ballot_sync(0xffffffffu, e0 == w.g), hi = __ballot_sync(0xffffffffu, e1 == w.g);
-        fetch(c + 1);
-        // steps of 16 rows, up to the last row of the group; at least one, so that every stage has
-        // an instruction for its commit to follow
-        const int rows = hi ? 64 - __clz(hi) : 32 - __clz(lo);
+        ++it;
+        if (rows == 64) continue;
+        uint32_t lo, hi;  // rows of the chunk that count
+        if (rows == kWgIrregular) {
+          const int row = b * 128 + (c & 1) * 64 + lane;
+          lo = __ballot_sync(0xffffffffu, (row < p.M ? __ldg(p.m_indices + row) : -1) == w.g);
+          hi = __ballot_sync(0xffffffffu, (row + 32 < p.M ? __ldg(p.m_indices + row + 32) : -1) == w.g);
+          rows = hi ? 64 - __clz(hi) : 32 - __clz(lo);
+        } else {
+          lo = rows >= 32 ? 0xffffffffu : (1u << rows) - 1u;
+          hi = rows > 32 ? (1u << (rows - 32)) - 1u : 0u;
+        }
+        // steps of 16 rows; at least one, so that every stage has an instruction for its commit to follow
         const int steps = max(1, (rows + 15) / 16);
-        if (!mbar_wait_warp(bar_full(s), (it / S) & 1u, abort_flag, WG_SITE_FILTER)) {
+        if (!mbar_wait_warp(bar_full(s), (phase >> s) & 1u, abort_flag, WG_SITE_FILTER)) {
           ok = false;
           break;
         }
+        phase ^= 1u << s;
         uint32_t zlo = ~lo, zhi = ~hi;  // rows to clear, of those that are issued
         if (steps < 2) zlo &= 0xffffu;
         if (steps < 3) zhi = 0;
         else if (steps < 4) zhi &= 0xffffu;
-        if (zlo | zhi) {
+        {
           // a row is 128 bytes in each of the four boxes: one 16-byte store of every lane
           uint8_t* at = smem + L::off_stage + s * kWgStageBytes + (lane >> 3) * kWgBoxBytes + (lane & 7) * 16;
           while (zlo) {
