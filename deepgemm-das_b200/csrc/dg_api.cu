@@ -222,10 +222,10 @@ struct Problem {
 
 // The packed weight as the kBT kernels read it: [64 columns][n rows][groups x column blocks], so
 // that a box that reaches behind the n rows of its block is filled with zeros.
-int encode_bt_map(CUtensorMap* map, const Problem& pr) {
+int encode_bt_map(CUtensorMap* map, const Problem& pr, int columns) {
   const uint64_t dims[3] = {64u, (uint64_t)pr.K, (uint64_t)pr.G * (pr.N / 64)};
   const uint64_t strides[2] = {(uint64_t)kRowBytes, (uint64_t)kRowBytes * pr.K};
-  const uint32_t box[3] = {64u, 64u, 1u};
+  const uint32_t box[3] = {64u, 64u, (uint32_t)columns / 64};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pr.b, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -339,7 +339,7 @@ int launch(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
                               pr.dense ? (uint64_t)pr.G * pr.N : (uint64_t)pr.G * p.kblocks * pr.N};
   const uint64_t b_strides[1] = {pr.dense ? (uint64_t)pr.K * esize : (uint64_t)kRowBytes};
   if (kBT) {
-    rc = encode_bt_map(&tm_b, pr);
+    rc = encode_bt_map(&tm_b, pr, BN);
   } else {
     const uint32_t box[2] = {(uint32_t)elems_per_row, (uint32_t)BN};
     rc = encode_map(&tm_b, dt_a, 2, pr.b, b_dims, b_strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -446,7 +446,7 @@ int launch_pair(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   }
   if (rc != DG_OK) return rc;
   if (kBT) {
-    rc = encode_bt_map(&tm_b, pr);
+    rc = encode_bt_map(&tm_b, pr, 128);
   } else {
     const uint64_t dims[2] = {pr.dense ? (uint64_t)pr.K : (uint64_t)elems_per_row,
                               pr.dense ? (uint64_t)pr.G * pr.N : (uint64_t)pr.G * p.kblocks * pr.N};

@@ -838,11 +838,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tma_load_3d(a_dst, tm_act, bar_full(s), kb * kElemsPerRow, t.row0, t.g, pol_a);
               else
                 tma_load_2d(a_dst, tm_act, bar_full(s), kb * kElemsPerRow, t.row0, pol_a);
-              if constexpr (kBT) {
-#pragma unroll
-                for (int c = 0; c < BN / 64; ++c)
-                  tma_load_3d(base + L::off_b + s * L::kBStage + c * kBTBlockBytes, tm_w, bar_full(s), 0,
-                              kb * 64, t.g * (p.N / 64) + t.n0 / 64 + c, pol_b);
+              if constexpr (kBT) {  // BN / 64 column blocks in one box
+                tma_load_3d(base + L::off_b + s * L::kBStage, tm_w, bar_full(s), 0, kb * 64,
+                            t.g * (p.N / 64) + t.n0 / 64, pol_b);
               } else {
                 int bx, by;
                 weight_coords(p, t.g, t.n0, kb, kElemsPerRow, bx, by);

@@ -91,7 +91,7 @@ struct PairDecoder {
 };
 
 // kBT: the weight is used the other way round, as in the one-CTA kernel; each block then holds 128
-// of the tile's columns as two 64-column boxes.
+// of the tile's columns as two 64-column blocks.
 template <int KIND, bool kBT = false>
 __global__ void __launch_bounds__(PairSmem::kThreads, 1)
 grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
@@ -257,11 +257,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
             tma_load_3d_pair(a_dst, &tm_a, full_leader, kb * kElemsPerRow, a_row, t.g, pol_a);
           else
             tma_load_2d_pair(a_dst, &tm_a, full_leader, kb * kElemsPerRow, a_row, pol_a);
-          if constexpr (kBT) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              tma_load_3d_pair(b_dst + c * kBTBlockBytes, &tm_b, full_leader, 0, kb * 64,
-                               t.g * (p.N / 64) + b_n0 / 64 + c, pol_b);
+          if constexpr (kBT) {  // two column blocks in one box
+            tma_load_3d_pair(b_dst, &tm_b, full_leader, 0, kb * 64, t.g * (p.N / 64) + b_n0 / 64, pol_b);
           } else {
             int bx, by;
             weight_coords(p, t.g, b_n0, kb, kElemsPerRow, bx, by);

@@ -22,6 +22,9 @@
 //               set to zero in shared memory, in both operands, so that whatever they held (NaN,
 //               infinities) does not reach a sum; of a chunk's four 16-row steps only those up to
 //               its last row are issued, and a block's second chunk is left out when it is empty.
+//   warp 7      watcher (leader): waits on the barriers in the UMMA issuer's place and posts counts in
+//               plain shared-memory words.  The issuer has 512 cycles for a chunk (four instructions
+//               of 256 x 256 x 16); a first look at a barrier alone takes 200 of them.
 // A chunk whose 64 rows all count, i.e. nearly every one, goes straight to the tensor cores: the
 // copies of both blocks complete on the leader's `ready` barrier.  Only the others complete on their
 // own block's `full` barrier, for the filter, which then arrives on `ready` in the producers' place.
@@ -41,7 +44,7 @@
 namespace dg {
 
 constexpr int kWgStages = 6;
-constexpr int kWgThreads = 224;
+constexpr int kWgThreads = 256;
 constexpr uint32_t kWgBoxBytes = 64 * 128;         // 64 columns x 64 rows
 constexpr uint32_t kWgOperand = 2 * kWgBoxBytes;   // 128 columns x 64 rows
 constexpr uint32_t kWgStageBytes = 2 * kWgOperand;
@@ -58,6 +61,7 @@ struct WgradParams {
   int32_t* status;
   int f32;                   // output type: fp32 (else bf16)
   int add;                   // fp32 only: add to what the output holds
+  int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
 };
 
 struct WgradSmem {
@@ -66,7 +70,7 @@ struct WgradSmem {
   // full[S], ready[S], empty[S], acc_full[2], acc_empty[2], drain
   static constexpr int kNumBars = 3 * kWgStages + 5;
   static constexpr int off_bar = off_strip + 4 * 4096;
-  static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort
+  static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort, stages ready, items ready
   static constexpr int off_steps = off_misc + 16;          // per stage: 16-row steps to issue
   static constexpr int off_table = off_steps + kWgStages * 4;
   // table: first[G + 1] (int32), the groups' 128-row blocks in order (uint16), rows that count (uint8)
@@ -125,6 +129,8 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   const uint32_t bar_drain = base + L::off_bar + 8u * (3 * S + 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::off_misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 4);
+  const uint32_t stages_addr = base + L::off_misc + 8;  // stages whose operands are ready
+  const uint32_t items_addr = base + L::off_misc + 12;  // work items whose accumulator is free
   volatile int* steps_s = reinterpret_cast<volatile int*>(smem + L::off_steps);
   int32_t* first = reinterpret_cast<int32_t*>(smem + L::off_table);
   uint16_t* blocks = reinterpret_cast<uint16_t*>(first + p.G + 1);
@@ -132,6 +138,8 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
 
   if (tid == 0) {
     *abort_flag = 0;
+    *reinterpret_cast<volatile uint32_t*>(smem + L::off_misc + 8) = 0;
+    *reinterpret_cast<volatile uint32_t*>(smem + L::off_misc + 12) = 0;
     for (int s = 0; s < S; ++s) {
       mbar_init(bar_full(s), 1);
       mbar_init(bar_ready(s), CL);  // the producer of each block, or its filter
@@ -275,66 +283,100 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
           const int row = b * 128 + (c & 1) * 64;
           const uint32_t dst = base + L::off_stage + s * kWgStageBytes;
           const int n = w.n0 + static_cast<int>(rank) * 128, k = w.k0 + static_cast<int>(rank) * 128;
-          if (rows == 64) {
-            uint32_t bar = bar_ready(s);
-            if constexpr (CL == 2) {
-              bar = mapa_shared(bar, 0);
-              if (rank == 0) mbar_arrive_expect_tx(bar_ready(s), 2 * kWgStageBytes); else wg_arrive_remote_relaxed(bar);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                tma_load_2d_pair(dst + i * kWgBoxBytes, &tm_dy, bar, n + 64 * i, row, pol);
-                tma_load_2d_pair(dst + kWgOperand + i * kWgBoxBytes, &tm_x, bar, k + 64 * i, row, pol);
-              }
-              continue;
+          // 64 rows x 128 columns of an operand are one box (two blocks of 64 columns): with a box for
+          // each block the copies alone took 1.27 ms instead of 1.06 (32 groups of 1024 rows, 4096 x
+          // 7168), the whole kernel 1.50 instead of 1.42.
+          if (CL == 2 && rows == 64) {
+            const uint32_t bar = mapa_shared(bar_ready(s), 0);
+            if (rank == 0) mbar_arrive_expect_tx(bar_ready(s), 2 * kWgStageBytes); else wg_arrive_remote_relaxed(bar);
+            if (p.dy_blocks) {
+              tma_load_3d_pair(dst, &tm_dy, bar, 0, row, n / 64, pol);
+            } else {
+              tma_load_2d_pair(dst, &tm_dy, bar, n, row, pol);
+              tma_load_2d_pair(dst + kWgBoxBytes, &tm_dy, bar, n + 64, row, pol);
             }
-            mbar_arrive_expect_tx(bar, kWgStageBytes);
+            tma_load_3d_pair(dst + kWgOperand, &tm_x, bar, 0, row, k / 64, pol);
           } else {
-            mbar_arrive_expect_tx(bar_full(s), kWgStageBytes);
-          }
-          const uint32_t bar = rows == 64 ? bar_ready(s) : bar_full(s);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            tma_load_2d(dst + i * kWgBoxBytes, &tm_dy, bar, n + 64 * i, row, pol);
-            tma_load_2d(dst + kWgOperand + i * kWgBoxBytes, &tm_x, bar, k + 64 * i, row, pol);
+            const uint32_t bar = rows == 64 ? bar_ready(s) : bar_full(s);
+            mbar_arrive_expect_tx(bar, kWgStageBytes);
+            if (p.dy_blocks) {
+              tma_load_3d(dst, &tm_dy, bar, 0, row, n / 64, pol);
+            } else {
+              tma_load_2d(dst, &tm_dy, bar, n, row, pol);
+              tma_load_2d(dst + kWgBoxBytes, &tm_dy, bar, n + 64, row, pol);
+            }
+            tma_load_3d(dst + kWgOperand, &tm_x, bar, 0, row, k / 64, pol);
           }
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      // ---- UMMA issuer
-      uint32_t it = 0, tile = 0;
+      // ---- UMMA issuer.  It touches no barrier and looks a block of rows ahead in the table.
+      auto poll_above = [&](uint32_t addr, uint32_t have, int site) -> uint32_t {
+        uint32_t v;
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+          if (v > have) return v;
+        }
+        const uint64_t t0 = global_timer_ns();
+        uint32_t spins = 0;
+        while (true) {
+          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+          if (v > have) return v;
+          if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
+            if (!*abort_flag) *abort_flag = site;
+            return 0;
+          }
+        }
+      };
+      uint32_t it = 0, tile = 0, stages_known = 0, items_known = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
         const Item w = item_of(item);
         if (w.chunks == 0) continue;
         const uint32_t buf = tile & 1u;
-        if (!mbar_wait_bounded(bar_acc_empty(buf), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
+        int n_next = valid[blocks[w.b0]];
+        if (items_known <= tile && (items_known = poll_above(items_addr, tile, WG_SITE_ACC_EMPTY)) == 0) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * BT;
-        for (int c = 0; c < w.chunks; ++c) {
-          const int rows = rows_of(valid[blocks[w.b0 + (c >> 1)]], c);
-          if (rows == 0) continue;
-          const int s = it % S;
-          if (!mbar_wait_bounded(bar_ready(s), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
-            ok = false;
-            break;
+        uint32_t acc = 0;
+        for (int i = 0; ok && 2 * i < w.chunks; ++i) {
+          const int n = n_next;
+          if (2 * (i + 1) < w.chunks) n_next = valid[blocks[w.b0 + i + 1]];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int rows = rows_of(n, half);
+            if (rows == 0) continue;
+            const int s = it % S;
+            if (stages_known <= it) {
+              if ((stages_known = poll_above(stages_addr, it, WG_SITE_READY)) == 0) {
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+            }
+            ++it;
+            const uint32_t at = base + L::off_stage + s * kWgStageBytes;
+            const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
+            const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
+            auto step = [&](int k) {  // 16 rows: 2048 bytes on in every box
+              if constexpr (CL == 2)
+                umma_ss_pair<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
+              else
+                umma_ss<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
+              acc = 1;
+            };
+            if (rows == 64) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) step(k);
+            } else {
+              const int steps = rows == kWgIrregular ? steps_s[s] : (rows + 15) / 16;
+              for (int k = 0; k < steps; ++k) step(k);
+            }
+            if constexpr (CL == 2) umma_commit_pair(bar_empty(s), 3); else umma_commit(bar_empty(s));
           }
-          ++it;
-          if (rows != 64) wg_fence_cluster();  // both filters' writes
-          tc_fence_after_sync();
-          const int steps = rows == kWgIrregular ? steps_s[s] : (rows + 15) / 16;
-          const uint32_t at = base + L::off_stage + s * kWgStageBytes;
-          const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
-          const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
-          for (int k = 0; k < steps; ++k) {  // 16 rows each: 2048 bytes on in every box
-            const uint32_t acc = (c | k) != 0 ? 1u : 0u;  // (a block's first chunk always has rows)
-            if constexpr (CL == 2)
-              umma_ss_pair<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
-            else
-              umma_ss<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
-          }
-          if constexpr (CL == 2) umma_commit_pair(bar_empty(s), 3); else umma_commit(bar_empty(s));
         }
         if (ok) {
           if constexpr (CL == 2) umma_commit_pair(bar_acc_full(buf), 3); else umma_commit(bar_acc_full(buf));
@@ -345,6 +387,30 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
         int local_abort = 0;
         if constexpr (CL == 2) umma_commit_pair(bar_drain, 1); else umma_commit(bar_drain);
         mbar_wait_bounded(bar_drain, 0, &local_abort, 0);
+      }
+    }
+  } else if (warp == 7) {
+    if (lane == 0 && rank == 0) {
+      // ---- watcher
+      uint32_t it = 0, tile = 0;
+      bool ok = true;
+      for (int item = unit; ok && item < n_items; item += units) {
+        const Item w = item_of(item);
+        if (w.chunks == 0) continue;
+        if (!mbar_wait_bounded(bar_acc_empty(tile & 1u), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
+        ++tile;
+        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(items_addr), "r"(tile) : "memory");
+        for (int c = 0; c < w.chunks; ++c) {
+          const int rows = rows_of(valid[blocks[w.b0 + (c >> 1)]], c);
+          if (rows == 0) continue;
+          if (!mbar_wait_bounded(bar_ready(it % S), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
+            ok = false;
+            break;
+          }
+          ++it;
+          if (rows != 64) wg_fence_cluster();  // both filters' writes
+          asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(stages_addr), "r"(it) : "memory");
+        }
       }
     }
   } else if (warp == 6) {

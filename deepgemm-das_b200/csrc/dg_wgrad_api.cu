@@ -19,16 +19,20 @@ int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& 
   if (smem > dev.max_smem) return DG_ERR_TOO_LARGE;
 
   CUtensorMap tm_dy, tm_x, tm_d;
-  const uint32_t box[2] = {64u, 64u};
   // Without rows nothing is loaded; the maps then describe one row that is never read.
   const uint64_t rows = p.M > 0 ? p.M : 1;
-  const void* dy = p.M > 0 ? a->dy : a->dw;
-  const void* x = p.M > 0 ? a->x : a->dw;
-  const uint64_t dy_dims[2] = {(uint64_t)p.N, rows}, x_dims[2] = {(uint64_t)p.K, rows};
-  const uint64_t dy_str[1] = {(uint64_t)p.N * 2}, x_str[1] = {(uint64_t)p.K * 2};
-  int rc = encode_map(&tm_dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, dy_dims, dy_str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == DG_OK)
-    rc = encode_map(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_dims, x_str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  // [64-column blocks][rows][64 columns]; when N is no multiple of 64 the last block of a row would
+  // reach into the next one, and behind the last row, so dy is then [rows][columns].
+  p.dy_blocks = p.N % 64 == 0;
+  auto operand = [&](CUtensorMap* map, const void* base, int cols, bool blocks) {
+    const uint64_t dims[3] = {blocks ? 64u : (uint64_t)cols, rows, (uint64_t)cols / 64};
+    const uint64_t strides[2] = {(uint64_t)cols * 2, 128};
+    const uint32_t box[3] = {64u, 64u, 2u};
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, blocks ? 3 : 2, p.M > 0 ? base : a->dw, dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  int rc = operand(&tm_dy, a->dy, p.N, p.dy_blocks);
+  if (rc == DG_OK) rc = operand(&tm_x, a->x, p.K, true);
   const uint64_t es = p.f32 ? 4 : 2;
   const uint64_t d_dims[3] = {64u, (uint64_t)p.N, (uint64_t)p.G * (p.K / 64)};
   const uint64_t d_str[2] = {64 * es, 64 * es * p.N};
