@@ -18,20 +18,20 @@
 //   warp 1      UMMA issuer (leader)
 //   warps 2..5  epilogue: accumulator -> bf16 or fp32 -> 32-row strip in shared memory -> TMA store
 //               (or TMA reduce-add, when the gradient is added to what is there)
-//   warp 6      row filter.  Rows that stand for nothing (padding, rows behind the last group) are
-//               set to zero in shared memory, in both operands, so that whatever they held (NaN,
-//               infinities) does not reach a sum; of a chunk's four 16-row steps only those up to
-//               its last row are issued, and a block's second chunk is left out when it is empty.
+//   warp 6      ragged steps.  The products run in steps of 16 rows.  Rows that stand for nothing
+//               (padding, rows behind the last group) must not reach a sum, whatever they hold (NaN,
+//               infinities): a step that has some beside rows that count is copied by this warp,
+//               with zeros in their place in both operands, into a buffer of its own, ahead of its
+//               use (a group usually ends in one).  Steps whose 16 rows all count, nearly every one,
+//               come from the ring.
 //   warp 7      watcher (leader): waits on the barriers in the UMMA issuer's place and posts counts in
 //               plain shared-memory words.  The issuer has 512 cycles for a chunk (four instructions
 //               of 256 x 256 x 16); a first look at a barrier alone takes 200 of them.
-// A chunk whose 64 rows all count, i.e. nearly every one, goes straight to the tensor cores: the
-// copies of both blocks complete on the leader's `ready` barrier.  Only the others complete on their
-// own block's `full` barrier, for the filter, which then arrives on `ready` in the producers' place.
-// (With the filter between every chunk and its products, each stage paid a remote arrival with
-// cluster-wide release and an acquire to match: 1.0 us a chunk, whatever the tensor cores did.)
 // Which rows count is known beforehand: every block of the grid reads all of m_indices once (from
-// L2) and keeps a byte for each 128 rows.
+// L2) and keeps a byte for each 128 rows.  Two earlier forms cleared the rows in the ring, in
+// front of the tensor cores: for every chunk that cost 1.0 us a chunk (a remote arrival with
+// cluster-wide release and an acquire to match, on the path of every stage), for ragged chunks
+// alone still 0.5 us a work item (32 groups of 300 to 3000 rows, 4096 x 7168: 1.65 ms instead of 1.55).
 // Groups without rows give zeros (or, added, nothing) and cost no products.
 //
 // Every mbarrier wait is bounded, as in the other kernels.
@@ -43,43 +43,51 @@
 
 namespace dg {
 
-constexpr int kWgStages = 6;
+constexpr int kWgStages = 6;                       // five where the table below needs the room
 constexpr int kWgThreads = 256;
 constexpr uint32_t kWgBoxBytes = 64 * 128;         // 64 columns x 64 rows
 constexpr uint32_t kWgOperand = 2 * kWgBoxBytes;   // 128 columns x 64 rows
 constexpr uint32_t kWgStageBytes = 2 * kWgOperand;
+constexpr uint32_t kWgTailBox = 64 * 2 * 16;       // 64 columns x 16 rows
+constexpr uint32_t kWgTailBytes = 4 * kWgTailBox;  // 128 columns of both operands
 
 constexpr int kWgIrregular = 255;  // rows that count lie between others: looked up where they are used
 
-enum : int { WG_SITE_EMPTY = 21, WG_SITE_FILTER = 22, WG_SITE_READY = 23, WG_SITE_ACC_EMPTY = 24, WG_SITE_ACC_FULL = 25 };
+enum : int { WG_SITE_EMPTY = 21, WG_SITE_TAIL_EMPTY = 22, WG_SITE_READY = 23, WG_SITE_ACC_EMPTY = 24, WG_SITE_ACC_FULL = 25,
+             WG_SITE_TAIL_READY = 26 };
 
 struct WgradParams {
   int G, M, N, K;
   int n_tiles, k_tiles;      // tiles of a group
   int m_blocks;              // ceil(M / 128)
   const int32_t* m_indices;
+  const __nv_bfloat16* dy;
+  const __nv_bfloat16* x;
   int32_t* status;
   int f32;                   // output type: fp32 (else bf16)
   int add;                   // fp32 only: add to what the output holds
   int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
 };
 
+template <int S>
 struct WgradSmem {
   static constexpr int off_stage = 0;
-  static constexpr int off_strip = off_stage + kWgStages * kWgStageBytes;  // 4 KB for each epilogue warp
-  // full[S], ready[S], empty[S], acc_full[2], acc_empty[2], drain
-  static constexpr int kNumBars = 3 * kWgStages + 5;
+  static constexpr int off_tail = off_stage + S * kWgStageBytes;
+  static constexpr int off_strip = off_tail + kWgTailBytes;  // 4 KB for each epilogue warp
+  // ready[S], empty[S], tail_ready, tail_empty, acc_full[2], acc_empty[2], drain
+  static constexpr int kNumBars = 2 * S + 7;
   static constexpr int off_bar = off_strip + 4 * 4096;
-  static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort, stages ready, items ready
-  static constexpr int off_steps = off_misc + 16;          // per stage: 16-row steps to issue
-  static constexpr int off_table = off_steps + kWgStages * 4;
+  static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort, stages ready, items ready, tails ready
+  static constexpr int off_table = off_misc + 24;
   // table: first[G + 1] (int32), the groups' 128-row blocks in order (uint16), rows that count (uint8)
   __host__ __device__ static constexpr int total(int groups, int blocks) {
     return off_table + (groups + 1) * 4 + blocks * 3 + 16 + 1024;
   }
   // The table is built from m_indices[128 b] of every block b, held as int16 in the (still empty) ring.
-  static_assert(kWgStages * static_cast<int>(kWgStageBytes) >= DG_MAX_CONTIG_ROWS / 128 * 2, "");
+  static_assert(S * static_cast<int>(kWgStageBytes) >= DG_MAX_CONTIG_ROWS / 128 * 2, "");
+  static_assert(off_table % 4 == 0 && off_strip % 1024 == 0 && off_tail % 1024 == 0, "");
 };
+static_assert(WgradSmem<kWgStages - 1>::total(DG_MAX_GROUPS, DG_MAX_CONTIG_ROWS / 128) <= 232448, "");
 
 // An arrival on another block's mbarrier that orders nothing (the copies it announces are ordered by
 // the barrier's byte count).
@@ -102,12 +110,11 @@ __device__ __forceinline__ void wg_store_commit() { asm volatile("cp.async.bulk.
 __device__ __forceinline__ void wg_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void wg_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-template <int CL>
+template <int CL, int S>
 __global__ void __launch_bounds__(kWgThreads, 1)
 grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_d, const WgradParams p) {
-  using L = WgradSmem;
-  constexpr int S = kWgStages;
+  using L = WgradSmem<S>;
   constexpr int BT = 128 * CL;  // tile edge
   constexpr uint32_t kIdesc = umma_idesc(1u, 1u, BT, BT) | kIdescAMn | kIdescBMn;
   constexpr int kTmemCols = 2 * BT;
@@ -121,17 +128,18 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   const uint32_t rank = CL == 2 ? cluster_ctarank() : 0u;
   const int unit = blockIdx.x / CL, units = gridDim.x / CL;
 
-  auto bar_full = [&](int s) { return base + L::off_bar + 8u * s; };
-  auto bar_ready = [&](int s) { return base + L::off_bar + 8u * (S + s); };
-  auto bar_empty = [&](int s) { return base + L::off_bar + 8u * (2 * S + s); };
-  auto bar_acc_full = [&](int b) { return base + L::off_bar + 8u * (3 * S + b); };
-  auto bar_acc_empty = [&](int b) { return base + L::off_bar + 8u * (3 * S + 2 + b); };
-  const uint32_t bar_drain = base + L::off_bar + 8u * (3 * S + 4);
+  auto bar_ready = [&](int s) { return base + L::off_bar + 8u * s; };
+  auto bar_empty = [&](int s) { return base + L::off_bar + 8u * (S + s); };
+  const uint32_t bar_tail_ready = base + L::off_bar + 8u * (2 * S);
+  const uint32_t bar_tail_empty = base + L::off_bar + 8u * (2 * S + 1);
+  auto bar_acc_full = [&](int b) { return base + L::off_bar + 8u * (2 * S + 2 + b); };
+  auto bar_acc_empty = [&](int b) { return base + L::off_bar + 8u * (2 * S + 4 + b); };
+  const uint32_t bar_drain = base + L::off_bar + 8u * (2 * S + 6);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::off_misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 4);
   const uint32_t stages_addr = base + L::off_misc + 8;  // stages whose operands are ready
   const uint32_t items_addr = base + L::off_misc + 12;  // work items whose accumulator is free
-  volatile int* steps_s = reinterpret_cast<volatile int*>(smem + L::off_steps);
+  const uint32_t tails_addr = base + L::off_misc + 16;  // ragged steps whose operands are ready
   int32_t* first = reinterpret_cast<int32_t*>(smem + L::off_table);
   uint16_t* blocks = reinterpret_cast<uint16_t*>(first + p.G + 1);
   uint8_t* valid = reinterpret_cast<uint8_t*>(blocks + p.m_blocks);  // of each 128-row block
@@ -140,11 +148,13 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     *abort_flag = 0;
     *reinterpret_cast<volatile uint32_t*>(smem + L::off_misc + 8) = 0;
     *reinterpret_cast<volatile uint32_t*>(smem + L::off_misc + 12) = 0;
+    *reinterpret_cast<volatile uint32_t*>(smem + L::off_misc + 16) = 0;
     for (int s = 0; s < S; ++s) {
-      mbar_init(bar_full(s), 1);
-      mbar_init(bar_ready(s), CL);  // the producer of each block, or its filter
+      mbar_init(bar_ready(s), CL);  // the producer of each block
       mbar_init(bar_empty(s), 1);
     }
+    mbar_init(bar_tail_ready, CL);  // warp 6 of each block
+    mbar_init(bar_tail_empty, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_acc_full(b), 1);
       mbar_init(bar_acc_empty(b), 4 * CL);
@@ -244,7 +254,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   const int tiles = p.n_tiles * p.k_tiles;
   const int n_items = p.G * tiles;
   struct Item {
-    int g, n0, k0, b0, chunks;
+    int g, n0, k0, b0, blocks;  // blocks[b0 .. b0 + blocks) are the group's
   };
   auto item_of = [&](int item) {
     Item it;
@@ -254,13 +264,14 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     it.n0 = nt * BT;
     it.k0 = (t - nt * p.k_tiles) * BT;
     it.b0 = it.g > 0 ? first[it.g - 1] : 0;
-    it.chunks = 2 * (first[it.g] - it.b0);
+    it.blocks = first[it.g] - it.b0;
     return it;
   };
 
-  // Rows that count in half c & 1 of a block with the table's entry n: 0 (left out), 1..63, 64, or
-  // kWgIrregular.
-  auto rows_of = [&](int n, int c) { return n == kWgIrregular ? n : max(0, min(64, n - 64 * (c & 1))); };
+  // A block whose table entry is n: steps of 16 rows of its first and second 64 rows that come from
+  // the ring, and ragged steps behind them (all eight steps of an irregular block).
+  auto ring_steps = [&](int n, int half) { return n == kWgIrregular ? 0 : max(0, min(4, n / 16 - 4 * half)); };
+  auto ragged_steps = [&](int n) { return n == kWgIrregular ? 8 : (n % 16 != 0 ? 1 : 0); };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -270,42 +281,44 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
         const Item w = item_of(item);
-        for (int c = 0; c < w.chunks; ++c) {
-          const int b = blocks[w.b0 + (c >> 1)];
-          const int rows = rows_of(valid[b], c);
-          if (rows == 0) continue;
-          const int s = it % S;
-          if (!mbar_wait_bounded(bar_empty(s), ((it / S) & 1u) ^ 1u, abort_flag, WG_SITE_EMPTY)) {
-            ok = false;
-            break;
-          }
-          ++it;
-          const int row = b * 128 + (c & 1) * 64;
-          const uint32_t dst = base + L::off_stage + s * kWgStageBytes;
-          const int n = w.n0 + static_cast<int>(rank) * 128, k = w.k0 + static_cast<int>(rank) * 128;
-          // 64 rows x 128 columns of an operand are one box (two blocks of 64 columns): with a box for
-          // each block the copies alone took 1.27 ms instead of 1.06 (32 groups of 1024 rows, 4096 x
-          // 7168), the whole kernel 1.50 instead of 1.42.
-          if (CL == 2 && rows == 64) {
-            const uint32_t bar = mapa_shared(bar_ready(s), 0);
-            if (rank == 0) mbar_arrive_expect_tx(bar_ready(s), 2 * kWgStageBytes); else wg_arrive_remote_relaxed(bar);
-            if (p.dy_blocks) {
-              tma_load_3d_pair(dst, &tm_dy, bar, 0, row, n / 64, pol);
-            } else {
-              tma_load_2d_pair(dst, &tm_dy, bar, n, row, pol);
-              tma_load_2d_pair(dst + kWgBoxBytes, &tm_dy, bar, n + 64, row, pol);
+        const int n = w.n0 + static_cast<int>(rank) * 128, k = w.k0 + static_cast<int>(rank) * 128;
+        for (int i = 0; ok && i < w.blocks; ++i) {
+          const int b = blocks[w.b0 + i];
+          const int count = valid[b];
+          for (int half = 0; half < 2; ++half) {
+            if (ring_steps(count, half) == 0) break;
+            const int s = it % S;
+            if (!mbar_wait_bounded(bar_empty(s), ((it / S) & 1u) ^ 1u, abort_flag, WG_SITE_EMPTY)) {
+              ok = false;
+              break;
             }
-            tma_load_3d_pair(dst + kWgOperand, &tm_x, bar, 0, row, k / 64, pol);
-          } else {
-            const uint32_t bar = rows == 64 ? bar_ready(s) : bar_full(s);
-            mbar_arrive_expect_tx(bar, kWgStageBytes);
-            if (p.dy_blocks) {
-              tma_load_3d(dst, &tm_dy, bar, 0, row, n / 64, pol);
+            ++it;
+            const int row = b * 128 + half * 64;
+            const uint32_t dst = base + L::off_stage + s * kWgStageBytes;
+            // 64 rows x 128 columns of an operand are one box (two blocks of 64 columns): with a box
+            // for each block the copies alone took 1.27 ms instead of 1.06 (32 groups of 1024 rows,
+            // 4096 x 7168), the whole kernel 1.50 instead of 1.42.
+            if constexpr (CL == 2) {
+              // the copies of both blocks complete on the leader's barrier
+              const uint32_t bar = mapa_shared(bar_ready(s), 0);
+              if (rank == 0) mbar_arrive_expect_tx(bar_ready(s), 2 * kWgStageBytes); else wg_arrive_remote_relaxed(bar);
+              if (p.dy_blocks) {
+                tma_load_3d_pair(dst, &tm_dy, bar, 0, row, n / 64, pol);
+              } else {
+                tma_load_2d_pair(dst, &tm_dy, bar, n, row, pol);
+                tma_load_2d_pair(dst + kWgBoxBytes, &tm_dy, bar, n + 64, row, pol);
+              }
+              tma_load_3d_pair(dst + kWgOperand, &tm_x, bar, 0, row, k / 64, pol);
             } else {
-              tma_load_2d(dst, &tm_dy, bar, n, row, pol);
-              tma_load_2d(dst + kWgBoxBytes, &tm_dy, bar, n + 64, row, pol);
+              mbar_arrive_expect_tx(bar_ready(s), kWgStageBytes);
+              if (p.dy_blocks) {
+                tma_load_3d(dst, &tm_dy, bar_ready(s), 0, row, n / 64, pol);
+              } else {
+                tma_load_2d(dst, &tm_dy, bar_ready(s), n, row, pol);
+                tma_load_2d(dst + kWgBoxBytes, &tm_dy, bar_ready(s), n + 64, row, pol);
+              }
+              tma_load_3d(dst + kWgOperand, &tm_x, bar_ready(s), 0, row, k / 64, pol);
             }
-            tma_load_3d(dst + kWgOperand, &tm_x, bar, 0, row, k / 64, pol);
           }
         }
       }
@@ -331,24 +344,34 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
           }
         }
       };
-      uint32_t it = 0, tile = 0, stages_known = 0, items_known = 0;
+      uint32_t it = 0, tile = 0, tail = 0, stages_known = 0, items_known = 0, tails_known = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
         const Item w = item_of(item);
-        if (w.chunks == 0) continue;
+        if (w.blocks == 0) continue;
         const uint32_t buf = tile & 1u;
         int n_next = valid[blocks[w.b0]];
         if (items_known <= tile && (items_known = poll_above(items_addr, tile, WG_SITE_ACC_EMPTY)) == 0) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * BT;
-        uint32_t acc = 0;
-        for (int i = 0; ok && 2 * i < w.chunks; ++i) {
+        uint32_t acc = 0;  // the first product of an item overwrites
+        auto step = [&](uint64_t a_desc, uint64_t b_desc) {
+          if constexpr (CL == 2)
+            umma_ss_pair<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
+          else
+            umma_ss<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
+          acc = 1;
+        };
+        auto commit = [&](uint32_t bar) {
+          if constexpr (CL == 2) umma_commit_pair(bar, 3); else umma_commit(bar);
+        };
+        for (int i = 0; ok && i < w.blocks; ++i) {
           const int n = n_next;
-          if (2 * (i + 1) < w.chunks) n_next = valid[blocks[w.b0 + i + 1]];
+          if (i + 1 < w.blocks) n_next = valid[blocks[w.b0 + i + 1]];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int rows = rows_of(n, half);
-            if (rows == 0) continue;
+            const int steps = ring_steps(n, half);
+            if (steps == 0) break;
             const int s = it % S;
             if (stages_known <= it) {
               if ((stages_known = poll_above(stages_addr, it, WG_SITE_READY)) == 0) {
@@ -361,26 +384,29 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
             const uint32_t at = base + L::off_stage + s * kWgStageBytes;
             const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
             const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
-            auto step = [&](int k) {  // 16 rows: 2048 bytes on in every box
-              if constexpr (CL == 2)
-                umma_ss_pair<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
-              else
-                umma_ss<UMMA_F16>(d_tmem, a_desc + 128u * k, b_desc + 128u * k, kIdesc, acc);
-              acc = 1;
-            };
-            if (rows == 64) {
+            if (steps == 4) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) step(k);
+              for (int k = 0; k < 4; ++k) step(a_desc + 128u * k, b_desc + 128u * k);  // 2048 bytes on in every box
             } else {
-              const int steps = rows == kWgIrregular ? steps_s[s] : (rows + 15) / 16;
-              for (int k = 0; k < steps; ++k) step(k);
+              for (int k = 0; k < steps; ++k) step(a_desc + 128u * k, b_desc + 128u * k);
             }
-            if constexpr (CL == 2) umma_commit_pair(bar_empty(s), 3); else umma_commit(bar_empty(s));
+            commit(bar_empty(s));
+          }
+          for (int r = ragged_steps(n); ok && r > 0; --r) {
+            if (tails_known <= tail) {
+              if ((tails_known = poll_above(tails_addr, tail, WG_SITE_TAIL_READY)) == 0) {
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+            }
+            ++tail;
+            const uint32_t at = base + L::off_tail;
+            step(umma_desc_mn_sw128(at, kWgTailBox), umma_desc_mn_sw128(at + 2 * kWgTailBox, kWgTailBox));
+            commit(bar_tail_empty);
           }
         }
-        if (ok) {
-          if constexpr (CL == 2) umma_commit_pair(bar_acc_full(buf), 3); else umma_commit(bar_acc_full(buf));
-        }
+        if (ok) commit(bar_acc_full(buf));
         ++tile;
       }
       if (*abort_flag) {
@@ -392,83 +418,86 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   } else if (warp == 7) {
     if (lane == 0 && rank == 0) {
       // ---- watcher
-      uint32_t it = 0, tile = 0;
+      auto post = [&](uint32_t addr, uint32_t v) {
+        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+      };
+      uint32_t it = 0, tile = 0, tail = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
         const Item w = item_of(item);
-        if (w.chunks == 0) continue;
+        if (w.blocks == 0) continue;
         if (!mbar_wait_bounded(bar_acc_empty(tile & 1u), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
-        ++tile;
-        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(items_addr), "r"(tile) : "memory");
-        for (int c = 0; c < w.chunks; ++c) {
-          const int rows = rows_of(valid[blocks[w.b0 + (c >> 1)]], c);
-          if (rows == 0) continue;
-          if (!mbar_wait_bounded(bar_ready(it % S), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
-            ok = false;
-            break;
+        post(items_addr, ++tile);
+        for (int i = 0; ok && i < w.blocks; ++i) {
+          const int n = valid[blocks[w.b0 + i]];
+          for (int half = 0; half < 2; ++half) {
+            if (ring_steps(n, half) == 0) break;
+            if (!mbar_wait_bounded(bar_ready(it % S), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
+              ok = false;
+              break;
+            }
+            post(stages_addr, ++it);
           }
-          ++it;
-          if (rows != 64) wg_fence_cluster();  // both filters' writes
-          asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(stages_addr), "r"(it) : "memory");
+          for (int r = ragged_steps(n); ok && r > 0; --r) {
+            if (!mbar_wait_bounded(bar_tail_ready, tail & 1u, abort_flag, WG_SITE_TAIL_READY)) {
+              ok = false;
+              break;
+            }
+            if constexpr (CL == 2) wg_fence_cluster();  // the other block's stores
+            post(tails_addr, ++tail);
+          }
         }
       }
     }
   } else if (warp == 6) {
-    // ---- row filter
-    uint32_t it = 0, phase = 0;  // bit s: parity of the next use of stage s's full barrier
+    // ---- ragged steps: 16 rows x 128 columns of both operands through registers, fetched before the
+    // buffer is free.  Lane l takes the 16-byte piece l % 16 (64-column block (l % 16) / 8) of rows
+    // l / 16, l / 16 + 2, ...
+    const int piece = lane & 15, rsub = lane >> 4;
+    uint32_t tail = 0;
     bool ok = true;
     for (int item = unit; ok && item < n_items; item += units) {
       const Item w = item_of(item);
-      for (int c = 0; c < w.chunks; ++c) {
-        const int b = blocks[w.b0 + (c >> 1)];
-        int rows = rows_of(valid[b], c);
-        if (rows == 0) continue;
-        const int s = it % S;
-        ++it;
-        if (rows == 64) continue;
-        uint32_t lo, hi;  // rows of the chunk that count
-        if (rows == kWgIrregular) {
-          const int row = b * 128 + (c & 1) * 64 + lane;
-          lo = __ballot_sync(0xffffffffu, (row < p.M ? __ldg(p.m_indices + row) : -1) == w.g);
-          hi = __ballot_sync(0xffffffffu, (row + 32 < p.M ? __ldg(p.m_indices + row + 32) : -1) == w.g);
-          rows = hi ? 64 - __clz(hi) : 32 - __clz(lo);
-        } else {
-          lo = rows >= 32 ? 0xffffffffu : (1u << rows) - 1u;
-          hi = rows > 32 ? (1u << (rows - 32)) - 1u : 0u;
-        }
-        // steps of 16 rows; at least one, so that every stage has an instruction for its commit to follow
-        const int steps = max(1, (rows + 15) / 16);
-        if (!mbar_wait_warp(bar_full(s), (phase >> s) & 1u, abort_flag, WG_SITE_FILTER)) {
-          ok = false;
-          break;
-        }
-        phase ^= 1u << s;
-        uint32_t zlo = ~lo, zhi = ~hi;  // rows to clear, of those that are issued
-        if (steps < 2) zlo &= 0xffffu;
-        if (steps < 3) zhi = 0;
-        else if (steps < 4) zhi &= 0xffffu;
-        {
-          // a row is 128 bytes in each of the four boxes: one 16-byte store of every lane
-          uint8_t* at = smem + L::off_stage + s * kWgStageBytes + (lane >> 3) * kWgBoxBytes + (lane & 7) * 16;
-          while (zlo) {
-            const int r = __ffs(zlo) - 1;
-            zlo &= zlo - 1;
-            *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0u, 0u, 0u, 0u);
+      const int cn = w.n0 + static_cast<int>(rank) * 128 + piece * 8;
+      const int ck = w.k0 + static_cast<int>(rank) * 128 + piece * 8;
+      for (int i = 0; ok && i < w.blocks; ++i) {
+        const int b = blocks[w.b0 + i];
+        const int n = valid[b];
+        const int count = ragged_steps(n);
+        for (int r = 0; ok && r < count; ++r, ++tail) {
+          const int row0 = b * 128 + 16 * (n == kWgIrregular ? r : n / 16);
+          uint32_t rows = (1u << (n & 15)) - 1u;  // rows of the step that count
+          if (n == kWgIrregular) {
+            const int row = row0 + lane;
+            rows = __ballot_sync(0xffffffffu, lane < 16 && row < p.M && __ldg(p.m_indices + row) == w.g);
           }
-          while (zhi) {
-            const int r = __ffs(zhi) - 1;
-            zhi &= zhi - 1;
-            *reinterpret_cast<uint4*>(at + (32 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
+          uint4 dy[8], x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int rr = rsub + 2 * j;
+            const size_t row = static_cast<size_t>(row0 + rr);
+            const bool in = (rows >> rr) & 1u;
+            dy[j] = x[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (in && cn < p.N) dy[j] = __ldg(reinterpret_cast<const uint4*>(p.dy + row * p.N + cn));
+            if (in && ck < p.K) x[j] = __ldg(reinterpret_cast<const uint4*>(p.x + row * p.K + ck));
+          }
+          if (!mbar_wait_warp(bar_tail_empty, (tail & 1u) ^ 1u, abort_flag, WG_SITE_TAIL_EMPTY)) {
+            ok = false;
+            break;
+          }
+          uint8_t* at = smem + L::off_tail + (piece >> 3) * kWgTailBox;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int rr = rsub + 2 * j;
+            const int off = rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
+            *reinterpret_cast<uint4*>(at + off) = dy[j];
+            *reinterpret_cast<uint4*>(at + 2 * kWgTailBox + off) = x[j];
           }
           fence_proxy_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) {
-          if (rank == 0) steps_s[s] = steps;
-          if constexpr (CL == 2)
-            mbar_arrive_remote(mapa_shared(bar_ready(s), 0));
-          else
-            mbar_arrive(bar_ready(s));
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CL == 2) mbar_arrive_remote(mapa_shared(bar_tail_ready, 0)); else mbar_arrive(bar_tail_ready);
+          }
         }
       }
     }
@@ -502,7 +531,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       const int n = w.n0 + static_cast<int>(rank) * 128 + q * 32;
       const int kb0 = w.k0 / 64;
       const int kbs = n < p.N ? min(BT / 64, kb_all - kb0) : 0;  // 64-column blocks to store
-      if (w.chunks == 0) {
+      if (w.blocks == 0) {
         if (!p.add && kbs > 0) {
           before();
 #pragma unroll

@@ -7,15 +7,15 @@ namespace {
 using namespace dg;
 using namespace dg::host;
 
-template <int CL>
+template <int CL, int S>
 int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& dev, cudaStream_t stream) {
-  auto kernel = grouped_wgrad_kernel<CL>;
+  auto kernel = grouped_wgrad_kernel<CL, S>;
   constexpr int BT = 128 * CL;
   p.n_tiles = (p.N + BT - 1) / BT;
   p.k_tiles = (p.K + BT - 1) / BT;
   const long long items = (long long)p.G * p.n_tiles * p.k_tiles;
   if (items > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
-  const int smem = WgradSmem::total(p.G, p.m_blocks);
+  const int smem = WgradSmem<S>::total(p.G, p.m_blocks);
   if (smem > dev.max_smem) return DG_ERR_TOO_LARGE;
 
   CUtensorMap tm_dy, tm_x, tm_d;
@@ -107,6 +107,8 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   p.K = a->k;
   p.m_blocks = (a->m_total + 127) / 128;
   p.m_indices = a->m_indices;
+  p.dy = static_cast<const __nv_bfloat16*>(a->dy);
+  p.x = static_cast<const __nv_bfloat16*>(a->x);
   p.status = a->status;
   p.f32 = a->out_kind == DG_OUT_F32;
   p.add = a->accumulate != 0;
@@ -117,8 +119,11 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
     const long long items = (long long)p.G * ((p.N + 255) / 256) * ((p.K + 255) / 256);
     tile = items >= dev->sm_count / 2 ? 256 : 128;
   }
-  return tile == 256 ? launch_wgrad<2>(a, p, *dev, static_cast<cudaStream_t>(stream))
-                     : launch_wgrad<1>(a, p, *dev, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // the table of very many rows takes the room of a ring stage
+  if (WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem)
+    return tile == 256 ? launch_wgrad<2, kWgStages>(a, p, *dev, st) : launch_wgrad<1, kWgStages>(a, p, *dev, st);
+  return tile == 256 ? launch_wgrad<2, kWgStages - 1>(a, p, *dev, st) : launch_wgrad<1, kWgStages - 1>(a, p, *dev, st);
 }
 
 }  // extern "C"

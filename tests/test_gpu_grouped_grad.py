@@ -249,3 +249,20 @@ def test_refusals():
     for kind, call in bad:
         with pytest.raises(kind):
             call()
+
+
+@pytest.mark.parametrize("tile", [128, 256])
+def test_the_most_rows_and_groups(tile):
+    """4096 blocks of 128 rows, 1024 groups in a scattered order: the largest table."""
+    m, g, n, k = 4096 * 128, 1024, 16, 64
+    gen = torch.Generator().manual_seed(8)
+    of_block = torch.randint(0, g, (4096,), generator=gen)
+    count = torch.randint(1, 129, (4096,), generator=gen)
+    mi = torch.where(torch.arange(128)[None] < count[:, None], of_block[:, None], -1).reshape(-1).int()
+    dy, x = whole(gen, m, n, lim=1), whole(gen, m, k, lim=1)
+    out = grouped_bf16_weight_grad(dy.to(DEV), x.to(DEV), mi.to(DEV), g, dtype=torch.float32, tile=tile)
+    deepgemm.check_device_status()
+    d, xx, key = dy.float().to(DEV), x.float().to(DEV), mi.to(DEV)
+    pairs = (d[:, :, None] * xx[:, None, :4]).view(m, -1)    # whole numbers: any order of the sums is exact
+    want = torch.zeros(g + 1, pairs.shape[1], device=DEV).index_add_(0, torch.where(key < 0, g, key).long(), pairs)[:g].view(g, n, 4)
+    assert torch.equal(out[:, 0, :, :4], want)
