@@ -4,8 +4,7 @@
 //   e4m3:  s = the smallest power of two with max|x| / s <= 448.  A power of two costs a
 //          floating-point format no precision (only its range ends a factor of up to two earlier),
 //          x / s is exact, and q * s is exact in bf16: taking the rows out again adds no rounding.
-//   int8:  s = max|x| / 127, q = rint(x * (1 / s)) (within 1.6e-5 steps of the nearest: two
-//          roundings of 2^-24 on at most 127 steps).
+//   int8:  s = max|x| / 127, q = rint(x / s).
 // s = 1 for a block of zeros and never less than 2^-126; a block that holds a NaN or an infinity
 // gets s = NaN, so that it comes back as NaN and an overflow is not lost in the checkpoint.  Values
 // come back at most as large as the largest finite one of their type.
@@ -21,6 +20,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "dg_rows.cuh"
 
 namespace dg {
@@ -29,12 +30,54 @@ constexpr int kCkBlock = 128;    // columns of one scale
 constexpr int kCkThreads = 256;
 constexpr int kCkLanes = 16;     // lanes of one block of columns
 
-// Bits of the largest magnitude (NaN and infinities order above everything finite), over the 16
-// lanes of a block of columns.
-__device__ __forceinline__ uint32_t ck_max_bits(uint32_t m) {
+// The largest magnitude of 128 columns, over the 16 lanes that hold them, as the bits of an fp32
+// value.  Magnitudes order like their bits, NaN and infinities above everything finite.  16-bit
+// types compare two at a time, and two blocks of columns (gate and up) share the exchanges between
+// the lanes.
+__device__ __forceinline__ uint32_t ck_max2(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+template <class T>
+__device__ __forceinline__ uint32_t ck_bits16(uint32_t b) {  // bits of a 16-bit value -> bits of it in fp32
+  if constexpr (sizeof(T) == 4) return b;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return b << 16;
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(b))));
+}
+template <class T, bool VEC>
+__device__ __forceinline__ uint32_t ck_lane_max16(const Eight<T, VEC, kCkLanes>& v) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(v.raw);
+  const uint32_t m = ck_max2(ck_max2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), ck_max2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+  return max(m >> 16, m & 0xffffu);
+}
+template <class T, bool VEC>
+__device__ __forceinline__ uint32_t ck_lane_max32(const Eight<T, VEC, kCkLanes>& v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v.get(i)) & 0x7fffffffu);
+  return m;
+}
+template <class T, bool VEC>
+__device__ __forceinline__ uint32_t ck_top(const Eight<T, VEC, kCkLanes>& v) {
+  uint32_t m = sizeof(T) == 2 ? ck_lane_max16(v) : ck_lane_max32(v);
 #pragma unroll
   for (int o = kCkLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+  return ck_bits16<T>(m);
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void ck_top_of_two(const Eight<T, VEC, kCkLanes>& v0, const Eight<T, VEC, kCkLanes>& v1, uint32_t& t0,
+                                              uint32_t& t1) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = (ck_lane_max16(v0) << 16) | ck_lane_max16(v1);
+#pragma unroll
+    for (int o = kCkLanes / 2; o > 0; o >>= 1) m = ck_max2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    t0 = ck_bits16<T>(m >> 16);
+    t1 = ck_bits16<T>(m & 0xffffu);
+  } else {
+    t0 = ck_top(v0);
+    t1 = ck_top(v1);
+  }
 }
 
 // Scale and its reciprocal for a block whose largest magnitude has the bits `top`.
@@ -60,27 +103,58 @@ __device__ __forceinline__ void ck_scale(uint32_t top, float& s, float& inv) {
   }
 }
 
-template <int KIND>
-__device__ __forceinline__ uint8_t ck_code(float x, float inv) {
-  const float v = x * inv;
-  if constexpr (KIND == DG_KIND_E4M3)
-    return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-  else
-    return static_cast<uint8_t>(max(-127, min(127, __float2int_rn(v))));
+// x / s, correctly rounded, from inv = 1 / s correctly rounded (Markstein, "Computation of elementary
+// functions on the IBM RISC System/6000 processor", 1990: q + (x - q s) inv with fused operations).
+// Near a tie of rint the product x * inv alone picks the further of two steps.
+__device__ __forceinline__ float ck_quotient(float x, float s, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, s, x), inv, q);
 }
-// The value that a code stands for, at most `most` in magnitude (NaN stays NaN): a value just below
-// the largest of its type may have been rounded up to a code beyond it (255 to 256 of 2^120, say)
-// and still comes back finite.
-template <int KIND>
-__device__ __forceinline__ float ck_value(uint8_t q, float s, float most) {
-  float v;
-  if constexpr (KIND == DG_KIND_E4M3)
-    v = __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3))) * s;
-  else
-    v = static_cast<float>(static_cast<int8_t>(q)) * s;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(most));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(-most));
-  return v;
+
+// Codes of eight values.
+template <int KIND, bool VEC, class Values>
+__device__ __forceinline__ EightBytes<VEC, kCkLanes> ck_codes(const Values& x, float s, float inv) {
+  EightBytes<VEC, kCkLanes> q;
+  if constexpr (KIND == DG_KIND_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q.half[i] = __nv_cvt_float2_to_fp8x2(make_float2(x.get(2 * i) * inv, x.get(2 * i + 1) * inv), __NV_SATFINITE, __NV_E4M3);
+  } else {
+    // Adding 1.5 * 2^23 rounds to a whole number (nearest, ties to even) and leaves it in the low bits;
+    // |x| <= 127 s up to a rounding, so nothing lies beyond 127.
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = __float_as_uint(ck_quotient(x.get(i), s, inv) + 12582912.0f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      q.word[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
+  }
+  return q;
+}
+
+// The values that eight codes stand for, at most `most` in magnitude (NaN stays NaN): a value just
+// below the largest of its type may have been rounded up to a code beyond it (255 to 256 of 2^120,
+// say) and still comes back finite.
+template <int KIND, bool VEC>
+__device__ __forceinline__ void ck_values(const EightBytes<VEC, kCkLanes>& q, float s, float most, float (&v)[8]) {
+  if constexpr (KIND == DG_KIND_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(q.half[i], __NV_E4M3)));
+      v[2 * i] = f.x * s;
+      v[2 * i + 1] = f.y * s;
+    }
+  } else {
+    // byte + 128 under the exponent of 2^23: 8388608 + byte + 128
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = (__uint_as_float(__byte_perm(q.word[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)) - 8388736.0f) * s;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(most));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(-most));
+  }
 }
 constexpr float kCkMaxF32 = 3.402823466e+38f;
 template <class T>
@@ -91,14 +165,6 @@ template <>
 __device__ __forceinline__ float ck_most<__half>() { return 65504.0f; }
 template <>
 __device__ __forceinline__ float ck_most<__nv_bfloat16>() { return 3.3895313892515355e+38f; }
-
-template <class T, bool VEC>
-__device__ __forceinline__ uint32_t ck_lane_max(const Eight<T, VEC, kCkLanes>& v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v.get(i)) & 0x7fffffffu);
-  return m;
-}
 
 // 1 / (1 + exp(-g)).  16-bit results take the hardware's exp and reciprocal (relative error below
 // 2^-21 where the sigmoid is not negligible), 32-bit ones the exact forms.
@@ -122,28 +188,50 @@ struct CheckpointParams {
   long long x_stride;
 };
 
-// Rows into a checkpoint.  A unit is 128 columns of one row.
+// A unit is 128 columns of one row, the work of 16 lanes; a block takes kCkUnits of them for each
+// group of 16 lanes, all of whose loads are under way before the first is used.
+constexpr int kCkUnits = 4;
+constexpr int kCkGroups = kCkThreads / kCkLanes;
+struct CkUnit {
+  long long u, r;  // u: the unit; r: its row, -1 behind the last unit
+  int b;           // its block of columns
+};
+template <int UNITS = kCkUnits>
+__device__ __forceinline__ CkUnit ck_unit(int k, int rows, int blocks) {
+  CkUnit w;
+  w.u = ((long long)blockIdx.x * UNITS + k) * kCkGroups + threadIdx.x / kCkLanes;
+  const long long all = (long long)rows * blocks;
+  if (all <= 0xffffffffLL) {
+    const uint32_t r = static_cast<uint32_t>(w.u) / static_cast<uint32_t>(blocks);
+    w.r = r;
+    w.b = static_cast<int>(static_cast<uint32_t>(w.u) - r * static_cast<uint32_t>(blocks));
+  } else {
+    w.r = w.u / blocks;
+    w.b = static_cast<int>(w.u - w.r * blocks);
+  }
+  if (w.u >= all) w.r = -1;
+  return w;
+}
+
+// Rows into a checkpoint.
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) checkpoint_rows_kernel(const CheckpointParams p) {
   const int lane = threadIdx.x & (kCkLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  const long long units = (long long)p.rows * blocks;
-  const long long step = (long long)gridDim.x * (kCkThreads / kCkLanes);
-  const long long first = (long long)blockIdx.x * (kCkThreads / kCkLanes) + threadIdx.x / kCkLanes;
-  for (long long base = first; base - first < units; base += step) {  // the same number of rounds for a whole warp
-    const long long u = min(base, units - 1);
-    const long long r = u / blocks;
-    const int b = static_cast<int>(u - r * blocks);
-    Eight<T, VEC, kCkLanes> v;
-    v.load(static_cast<const T*>(p.x) + (size_t)r * p.x_stride, b * kCkBlock, lane, p.H);
-    float s, inv;
-    ck_scale<KIND>(ck_max_bits(ck_lane_max(v)), s, inv);
-    if (base >= units) continue;
-    EightBytes<VEC, kCkLanes> q;
+  CkUnit w[kCkUnits];
+  Eight<T, VEC, kCkLanes> v[kCkUnits];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q.val[i] = ck_code<KIND>(v.get(i), inv);
-    q.store(p.q + (size_t)r * p.H, b * kCkBlock, lane, p.H);
-    if (lane == 0) p.scale[u] = s;
+  for (int k = 0; k < kCkUnits; ++k) {
+    w[k] = ck_unit(k, p.rows, blocks);
+    v[k].load(static_cast<const T*>(p.x) + (size_t)max(w[k].r, 0LL) * p.x_stride, w[k].b * kCkBlock, lane, p.H, w[k].r >= 0);
+  }
+#pragma unroll
+  for (int k = 0; k < kCkUnits; ++k) {
+    float s, inv;
+    ck_scale<KIND>(ck_top(v[k]), s, inv);  // every lane takes part
+    if (w[k].r < 0) continue;
+    ck_codes<KIND, VEC>(v[k], s, inv).store(p.q + (size_t)w[k].r * p.H, w[k].b * kCkBlock, lane, p.H);
+    if (lane == 0) p.scale[w[k].u] = s;
   }
 }
 
@@ -152,18 +240,24 @@ template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) restore_rows_kernel(const CheckpointParams p) {
   const int lane = threadIdx.x & (kCkLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  const long long units = (long long)p.rows * blocks;
-  const long long step = (long long)gridDim.x * (kCkThreads / kCkLanes);
-  for (long long u = (long long)blockIdx.x * (kCkThreads / kCkLanes) + threadIdx.x / kCkLanes; u < units; u += step) {
-    const long long r = u / blocks;
-    const int b = static_cast<int>(u - r * blocks);
-    const float s = p.scale[u];
-    EightBytes<VEC, kCkLanes> q;
-    q.load(p.q + (size_t)r * p.H, b * kCkBlock, lane, p.H);
+  CkUnit w[kCkUnits];
+  EightBytes<VEC, kCkLanes> q[kCkUnits];
+  float s[kCkUnits];
+#pragma unroll
+  for (int k = 0; k < kCkUnits; ++k) {
+    w[k] = ck_unit(k, p.rows, blocks);
+    q[k].load(p.q + (size_t)max(w[k].r, 0LL) * p.H, w[k].b * kCkBlock, lane, p.H, w[k].r >= 0);
+    s[k] = w[k].r >= 0 ? p.scale[w[k].u] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < kCkUnits; ++k) {
+    if (w[k].r < 0) continue;
+    float f[8];
+    ck_values<KIND, VEC>(q[k], s[k], ck_most<T>(), f);
     Eight<T, VEC, kCkLanes> v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v.set(i, ck_value<KIND>(q.val[i], s, ck_most<T>()));
-    v.store(static_cast<T*>(p.out) + (size_t)r * p.H, b * kCkBlock, lane, p.H);
+    for (int i = 0; i < 8; ++i) v.set(i, f[i]);
+    v.store(static_cast<T*>(p.out) + (size_t)w[k].r * p.H, w[k].b * kCkBlock, lane, p.H);
   }
 }
 
@@ -179,45 +273,46 @@ struct ActCheckpointParams {
   long long x_stride, dact_stride;
 };
 
+constexpr int kCkActUnits = 2;
+
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) act_checkpoint_kernel(const ActCheckpointParams p) {
   const int lane = threadIdx.x & (kCkLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  const long long units = (long long)p.rows * blocks;
-  const long long step = (long long)gridDim.x * (kCkThreads / kCkLanes);
-  const long long first = (long long)blockIdx.x * (kCkThreads / kCkLanes) + threadIdx.x / kCkLanes;
-  for (long long base = first; base - first < units; base += step) {
-    const long long u = min(base, units - 1);
-    const long long r = u / blocks;
-    const int b = static_cast<int>(u - r * blocks), c0 = b * kCkBlock;
-    const bool skip = p.m_indices != nullptr && p.m_indices[r] < 0;
-    Eight<T, VEC, kCkLanes> g, up;
-    if (!skip) {
-      const T* x = static_cast<const T*>(p.x) + (size_t)r * p.x_stride;
-      g.load(x, c0, lane, p.H);
-      up.load(x + p.H, c0, lane, p.H);
-    }
+  CkUnit w[kCkActUnits];
+  bool skip[kCkActUnits];
+  Eight<T, VEC, kCkLanes> g[kCkActUnits], up[kCkActUnits];
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
+    w[k] = ck_unit<kCkActUnits>(k, p.rows, blocks);
+    skip[k] = w[k].r < 0 || (p.m_indices != nullptr && p.m_indices[w[k].r] < 0);
+  }
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
+    const T* x = static_cast<const T*>(p.x) + (size_t)max(w[k].r, 0LL) * p.x_stride;
+    g[k].load(x, w[k].b * kCkBlock, lane, p.H, !skip[k]);
+    up[k].load(x + p.H, w[k].b * kCkBlock, lane, p.H, !skip[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
     float sg, ig, su, iu;
-    ck_scale<KIND>(ck_max_bits(ck_lane_max(g)), sg, ig);
-    ck_scale<KIND>(ck_max_bits(ck_lane_max(up)), su, iu);
-    if (base >= units || (skip && !p.clear)) continue;
-    EightBytes<VEC, kCkLanes> qg, qu;
+    uint32_t tg, tu;
+    ck_top_of_two(g[k], up[k], tg, tu);  // every lane takes part
+    ck_scale<KIND>(tg, sg, ig);
+    ck_scale<KIND>(tu, su, iu);
+    if (w[k].r < 0 || (skip[k] && !p.clear)) continue;
+    const int c0 = w[k].b * kCkBlock;
     Eight<T, VEC, kCkLanes> a;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gv = g.get(i), uv = up.get(i);
-      qg.val[i] = ck_code<KIND>(gv, ig);
-      qu.val[i] = ck_code<KIND>(uv, iu);
-      a.set(i, ck_silu<T>(gv) * uv);
-    }
-    a.store(static_cast<T*>(p.act) + (size_t)r * p.H, c0, lane, p.H);
-    uint8_t* q = p.q + (size_t)r * 2 * p.H;
-    qg.store(q, c0, lane, p.H);
-    qu.store(q + p.H, c0, lane, p.H);
+    for (int i = 0; i < 8; ++i) a.set(i, ck_silu<T>(g[k].get(i)) * up[k].get(i));
+    a.store(static_cast<T*>(p.act) + (size_t)w[k].r * p.H, c0, lane, p.H);
+    uint8_t* q = p.q + (size_t)w[k].r * 2 * p.H;
+    ck_codes<KIND, VEC>(g[k], sg, ig).store(q, c0, lane, p.H);
+    ck_codes<KIND, VEC>(up[k], su, iu).store(q + p.H, c0, lane, p.H);
     if (lane == 0) {
-      float* s = p.scale + (size_t)r * 2 * blocks;
-      s[b] = sg;
-      s[blocks + b] = su;
+      float* s = p.scale + (size_t)w[k].r * 2 * blocks;
+      s[w[k].b] = sg;
+      s[blocks + w[k].b] = su;
     }
   }
 }
@@ -226,37 +321,51 @@ template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) act_checkpoint_grad_kernel(const ActCheckpointParams p) {
   const int lane = threadIdx.x & (kCkLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  const long long units = (long long)p.rows * blocks;
-  const long long step = (long long)gridDim.x * (kCkThreads / kCkLanes);
-  for (long long u = (long long)blockIdx.x * (kCkThreads / kCkLanes) + threadIdx.x / kCkLanes; u < units; u += step) {
-    const long long r = u / blocks;
-    const int b = static_cast<int>(u - r * blocks), c0 = b * kCkBlock;
-    const bool skip = p.m_indices != nullptr && p.m_indices[r] < 0;
-    if (skip && !p.clear) continue;
+  CkUnit w[kCkActUnits];
+  bool skip[kCkActUnits];
+  EightBytes<VEC, kCkLanes> qg[kCkActUnits], qu[kCkActUnits];
+  Eight<T, VEC, kCkLanes> d[kCkActUnits];
+  float sg[kCkActUnits], su[kCkActUnits];
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
+    w[k] = ck_unit<kCkActUnits>(k, p.rows, blocks);
+    skip[k] = w[k].r < 0 || (p.m_indices != nullptr && p.m_indices[w[k].r] < 0);
+  }
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
+    const size_t r = static_cast<size_t>(max(w[k].r, 0LL));
+    const float* s = p.scale + r * 2 * blocks;
+    const uint8_t* q = p.q + r * 2 * p.H;
+    const int c0 = w[k].b * kCkBlock;
+    qg[k].load(q, c0, lane, p.H, !skip[k]);
+    qu[k].load(q + p.H, c0, lane, p.H, !skip[k]);
+    d[k].load(static_cast<const T*>(p.dact) + r * p.dact_stride, c0, lane, p.H, !skip[k]);
+    sg[k] = skip[k] ? 0.0f : s[w[k].b];
+    su[k] = skip[k] ? 0.0f : s[blocks + w[k].b];
+  }
+#pragma unroll
+  for (int k = 0; k < kCkActUnits; ++k) {
+    if (w[k].r < 0 || (skip[k] && !p.clear)) continue;
     Eight<T, VEC, kCkLanes> dg, du, a;
-    if (!skip) {
-      const float* s = p.scale + (size_t)r * 2 * blocks;
-      const float sg = s[b], su = s[blocks + b];
-      const uint8_t* q = p.q + (size_t)r * 2 * p.H;
-      EightBytes<VEC, kCkLanes> qg, qu;
-      Eight<T, VEC, kCkLanes> d;
-      qg.load(q, c0, lane, p.H);
-      qu.load(q + p.H, c0, lane, p.H);
-      d.load(static_cast<const T*>(p.dact) + (size_t)r * p.dact_stride, c0, lane, p.H);
+    if (!skip[k]) {
+      float gv[8], uv[8];
+      ck_values<KIND, VEC>(qg[k], sg[k], kCkMaxF32, gv);
+      ck_values<KIND, VEC>(qu[k], su[k], kCkMaxF32, uv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float gv = ck_value<KIND>(qg.val[i], sg, kCkMaxF32), uv = ck_value<KIND>(qu.val[i], su, kCkMaxF32), dv = d.get(i);
-        const float sig = ck_sigmoid<T>(gv);
-        const float silu = gv * sig;
-        dg.set(i, dv * uv * sig * fmaf(gv, 1.0f - sig, 1.0f));
+        const float dv = d[k].get(i);
+        const float sig = ck_sigmoid<T>(gv[i]);
+        const float silu = gv[i] * sig;
+        dg.set(i, dv * uv[i] * sig * fmaf(gv[i], 1.0f - sig, 1.0f));
         du.set(i, dv * silu);
-        a.set(i, silu * uv);
+        a.set(i, silu * uv[i]);
       }
     }
-    T* dx = static_cast<T*>(p.dx) + (size_t)r * 2 * p.H;
+    const int c0 = w[k].b * kCkBlock;
+    T* dx = static_cast<T*>(p.dx) + (size_t)w[k].r * 2 * p.H;
     dg.store(dx, c0, lane, p.H);
     du.store(dx + p.H, c0, lane, p.H);
-    if (p.act != nullptr) a.store(static_cast<T*>(p.act) + (size_t)r * p.H, c0, lane, p.H);
+    if (p.act != nullptr) a.store(static_cast<T*>(p.act) + (size_t)w[k].r * p.H, c0, lane, p.H);
   }
 }
 

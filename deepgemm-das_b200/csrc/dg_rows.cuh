@@ -14,6 +14,31 @@ namespace dg {
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// 16 (8) bytes that are read once, or zeros where `on` is false (nothing is read).  One predicated
+// instruction and volatile: several of these in a row stay together in front of their first use.
+// Written as a branch around a plain load, the compiler moved each load and what uses it into the
+// branch, which put eight memory latencies behind one another in the gradient of the way back
+// (380 us instead of 180).
+__device__ __forceinline__ uint4 load_once(const void* p, bool on) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %5, 0;\n\t"
+      "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@on ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(on)));
+  return v;
+}
+__device__ __forceinline__ uint2 load_once8(const void* p, bool on) {
+  uint2 v;
+  asm volatile(
+      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+      "@on ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y)
+      : "l"(p), "r"(static_cast<uint32_t>(on)));
+  return v;
+}
+
 template <class T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -39,19 +64,18 @@ struct Eight {
   static __device__ __forceinline__ int col(int c0, int lane, int i) {
     return VEC ? c0 + 8 * lane + i : c0 + lane + LANES * i;
   }
-  // columns at or beyond `cols` are left at zero
-  __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols) {
+  // columns at or beyond `cols` are zero, and all of them where `on` is false
+  __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols, bool on = true) {
     if constexpr (VEC) {
       const int c = c0 + 8 * lane;
-      if (c < cols) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
-      }
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        raw[i] = load_once(reinterpret_cast<const uint4*>(row + c) + i, on && c < cols);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = c0 + lane + LANES * i;
-        if (c < cols) val[i] = row[c];
+        val[i] = on && c < cols ? row[c] : T();
       }
     }
   }
@@ -79,18 +103,20 @@ template <bool VEC, int LANES>
 struct EightBytes {
   union {
     uint2 raw;
+    uint32_t word[2];
+    uint16_t half[4];
     uint8_t val[8];
   };
   __device__ __forceinline__ EightBytes() { raw = make_uint2(0u, 0u); }
-  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols) {
+  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on = true) {
     if constexpr (VEC) {
       const int c = c0 + 8 * lane;
-      if (c < cols) raw = __ldg(reinterpret_cast<const uint2*>(row + c));
+      raw = load_once8(row + c, on && c < cols);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = c0 + lane + LANES * i;
-        if (c < cols) val[i] = row[c];
+        val[i] = on && c < cols ? row[c] : uint8_t(0);
       }
     }
   }

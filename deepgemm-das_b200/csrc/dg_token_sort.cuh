@@ -40,7 +40,10 @@ struct TokenSortParams {
   int rep;              // copies of the shared-memory histogram (fewer lanes meet at one address)
 };
 
-constexpr int kSortThreads = 512;
+#ifndef SORT_T
+#define SORT_T 1024
+#endif
+constexpr int kSortThreads = SORT_T;
 constexpr int kSortMaxChunk = 2048;  // pairs of one block
 
 __device__ __forceinline__ int sort_id(const TokenSortParams& p, long long i) {
@@ -239,33 +242,39 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
     }
   }
 
-  // m_indices, and zeros in the rows that stand for no pair
-  const int per = (p.cap + gridDim.x - 1) / gridDim.x;
-  const long long r1 = min((long long)(blockIdx.x + 1) * per, (long long)p.cap);
-  for (long long rb = (long long)blockIdx.x * per; rb < r1; rb += kSortThreads) {
-    if (tid == 0) list_n = 0;
-    __syncthreads();
-    const long long r = rb + tid;
-    if (r < r1) {
-      int lo = 0, hi = p.G;  // the last expert that begins at or before r (empty ones begin where the next does)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (offset[mid] <= r) lo = mid; else hi = mid;
-      }
-      const bool used = r < (long long)offset[lo] + count[lo];
-      if (first) p.m_indices[r] = used ? lo : -1;
-      if (!used && p.clear) list[atomicAdd(&list_n, 1)] = static_cast<int>(r);
+  // m_indices: a stretch of rows for each block
+  auto expert_of = [&](long long r) {  // -1: the row stands for no pair
+    int lo = 0, hi = p.G;  // the last expert that begins at or before r (empty ones begin where the next does)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (offset[mid] <= r) lo = mid; else hi = mid;
     }
-    __syncthreads();
-    const int n = list_n;
-    for (int u = warp; u < n * segs; u += kSortThreads / 32) {
-      const int i = u / segs, v0 = (seg0 + u - i * segs) * kSeg + lane;
-      V* dst = reinterpret_cast<V*>(rows + (size_t)list[i] * p.row_bytes);
+    return r < (long long)offset[lo] + count[lo] ? lo : -1;
+  };
+  if (first) {
+    const int per = (p.cap + gridDim.x - 1) / gridDim.x;
+    const long long r1 = min((long long)(blockIdx.x + 1) * per, (long long)p.cap);
+    for (long long r = (long long)blockIdx.x * per + tid; r < r1; r += kSortThreads) p.m_indices[r] = expert_of(r);
+  }
+  // zeros in the rows that stand for no pair; most of them lie together, so the blocks take every
+  // gridDim.x-th row
+  if (p.clear) {
+    for (long long rb = 0; rb < p.cap; rb += (long long)gridDim.x * kSortThreads) {
+      if (tid == 0) list_n = 0;
+      __syncthreads();
+      const long long r = rb + (long long)tid * gridDim.x + blockIdx.x;
+      if (r < p.cap && expert_of(r) < 0) list[atomicAdd(&list_n, 1)] = static_cast<int>(r);
+      __syncthreads();
+      const int n = list_n;
+      for (int u = warp; u < n * segs; u += kSortThreads / 32) {
+        const int i = u / segs, v0 = (seg0 + u - i * segs) * kSeg + lane;
+        V* dst = reinterpret_cast<V*>(rows + (size_t)list[i] * p.row_bytes);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (v0 + 32 * k < nv) dst[v0 + 32 * k] = V{};
+        for (int k = 0; k < 4; ++k)
+          if (v0 + 32 * k < nv) dst[v0 + 32 * k] = V{};
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -284,42 +293,41 @@ constexpr int kUnsortThreads = 256;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kUnsortThreads) token_unsort_kernel(const TokenUnsortParams p) {
   const int lane = threadIdx.x & 31;
-  const int segs = (p.H + 255) / 256;
-  const long long units = (long long)p.T * segs;
-  const long long step = (long long)gridDim.x * (kUnsortThreads / 32);
-  for (long long u = (long long)blockIdx.x * (kUnsortThreads / 32) + (threadIdx.x >> 5); u < units; u += step) {
-    const long long t = u / segs;
-    const int c0 = static_cast<int>(u - t * segs) * 256;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < p.top_k; j0 += 8) {
-      int d = -1;
-      float w = 1.0f;
-      if (lane < 8 && j0 + lane < p.top_k) {
-        d = p.dest[t * p.top_k + j0 + lane];
-        if (d >= p.rows) d = -1;
-        if (p.weights) w = p.weights[t * p.top_k + j0 + lane];
-      }
-      Eight<T, VEC, 32> v[8];
-      int dj[8];
+  const unsigned segs = (p.H + 255u) / 256u;
+  const unsigned u = blockIdx.x * (kUnsortThreads / 32u) + (threadIdx.x >> 5);  // the host keeps units below 2^32
+  const unsigned t = u / segs;
+  if (t >= static_cast<unsigned>(p.T)) return;
+  const int c0 = static_cast<int>(u - t * segs) * 256;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+    int d = -1;
+    float w = 1.0f;
+    if (lane < 8 && j0 + lane < p.top_k) {
+      const size_t i = (size_t)t * p.top_k + j0 + lane;
+      d = p.dest[i];
+      if (d >= p.rows) d = -1;
+      if (p.weights) w = p.weights[i];
+    }
+    Eight<T, VEC, 32> v[8];
+    int dj[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dj[j] = __shfl_sync(0xffffffffu, d, j);
-        if (dj[j] >= 0) v[j].load(static_cast<const T*>(p.y) + (size_t)dj[j] * p.y_stride, c0, lane, p.H);
-      }
+    for (int j = 0; j < 8; ++j) {
+      dj[j] = __shfl_sync(0xffffffffu, d, j);
+      v[j].load(static_cast<const T*>(p.y) + (size_t)max(dj[j], 0) * p.y_stride, c0, lane, p.H, dj[j] >= 0);
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float wj = __shfl_sync(0xffffffffu, w, j);
-        if (dj[j] >= 0) {  // a pair without a row adds nothing, whatever its weight is
+    for (int j = 0; j < 8; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      if (dj[j] >= 0) {  // a pair without a row adds nothing, whatever its weight is
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = fmaf(wj, v[j].get(i), acc[i]);
-        }
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(wj, v[j].get(i), acc[i]);
       }
     }
-    Eight<T, VEC, 32> o;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o.set(i, acc[i]);
-    o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0, lane, p.H);
   }
+  Eight<T, VEC, 32> o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.set(i, acc[i]);
+  o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0, lane, p.H);
 }
 
 struct TokenUnsortGradParams {
@@ -336,94 +344,95 @@ struct TokenUnsortGradParams {
   int clear_blocks;          // blocks behind those of the tokens that clear rows
 };
 
-// Sets rows with m_indices < 0 to zero: block `b` of `nb`.
-template <class T, bool VEC, int THREADS>
+// Sets rows with m_indices < 0 to zero: block `b` of `nb`.  Most of them lie together, so the warps
+// take every so-many-th row; lane l looks at the warp's l-th.
+template <class T, bool VEC>
 __device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indices, int rows, int H, int b, int nb) {
   const int lane = threadIdx.x & 31;
-  const int per = (rows + nb - 1) / nb;
-  const long long r1 = min((long long)(b + 1) * per, (long long)rows);
-  // a warp looks at 32 rows at a time and clears the ones that stand for nothing together
-  for (long long rb = (long long)b * per + (threadIdx.x >> 5) * 32; rb < r1; rb += THREADS) {
-    const bool free_row = rb + lane < r1 && m_indices[rb + lane] < 0;
-    unsigned mask = __ballot_sync(0xffffffffu, free_row);
+  const int warps = nb * (blockDim.x >> 5);
+  const int first = b * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  for (long long rb = 0; rb < rows; rb += 32LL * warps) {
+    const long long mine = rb + (long long)lane * warps + first;
+    unsigned mask = __ballot_sync(0xffffffffu, mine < rows && m_indices[mine] < 0);
     while (mask) {
       const int i = __ffs(mask) - 1;
       mask &= mask - 1;
-      T* row = out + (size_t)(rb + i) * H;
+      T* row = out + (size_t)(rb + (long long)i * warps + first) * H;
       const Eight<T, VEC, 32> zero;
       for (int c0 = 0; c0 < H; c0 += 256) zero.store(row, c0, lane, H);
     }
   }
 }
 
-// One block takes `per` pairs of one token: dout[t] stays in registers (2048 columns at a time)
-// while the rows of y go by; each row's product with dout is summed over the block in a fixed
+// One block takes `per` pairs of one token, a warp 256 columns at a time: its piece of dout[t]
+// stays in registers while the rows of eight pairs go by, all of them on their way before the first
+// is used.  A pair's product is summed over a lane's columns, the lanes and the warps in that fixed
 // order.
-constexpr int kUnsortGradThreads = 128;
+constexpr int kUnsortGradWarps = 8;
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kUnsortGradThreads) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
-  constexpr int kWarps = kUnsortGradThreads / 32;
-  __shared__ float part[kWarps][32];
-  const int splits = (p.top_k + p.per - 1) / p.per;
-  const long long token_blocks = (long long)p.T * splits;
-  if ((long long)blockIdx.x >= token_blocks) {
-    clear_rows_block<T, VEC, kUnsortGradThreads>(static_cast<T*>(p.dy), p.m_indices, p.rows, p.H,
-                                                 static_cast<int>(blockIdx.x - token_blocks), p.clear_blocks);
+__global__ void __launch_bounds__(32 * kUnsortGradWarps) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
+  __shared__ float part[kUnsortGradWarps][8];
+  const int warps = blockDim.x >> 5;
+  const unsigned splits = (p.top_k + p.per - 1) / p.per;
+  const unsigned token_blocks = static_cast<unsigned>(p.T) * splits;
+  if (blockIdx.x >= token_blocks) {
+    clear_rows_block<T, VEC>(static_cast<T*>(p.dy), p.m_indices, p.rows, p.H, static_cast<int>(blockIdx.x - token_blocks), p.clear_blocks);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long t = blockIdx.x / splits;
+  const unsigned t = blockIdx.x / splits;
   const int j_begin = static_cast<int>(blockIdx.x - t * splits) * p.per;
   const int j_end = min(j_begin + p.per, p.top_k);
   const T* dout = static_cast<const T*>(p.dout) + (size_t)t * p.dout_stride;
-  for (int j0 = j_begin; j0 < j_end; j0 += 32) {
-    const int nj = min(32, j_end - j0);
-    float dot = 0.0f;  // lane j: this warp's part of pair j0 + j
-    constexpr int kPass = 2;
-    for (int base = 0; base < p.H; base += kPass * kWarps * 256) {
-      Eight<T, VEC, 32> g[kPass];
+  for (int j0 = j_begin; j0 < j_end; j0 += 8) {
+    int d_lane = -1;
+    float w_lane = 1.0f;
+    if (lane < 8 && j0 + lane < j_end) {
+      const size_t i = (size_t)t * p.top_k + j0 + lane;
+      d_lane = p.dest[i];
+      if (d_lane >= p.rows) d_lane = -1;
+      if (p.weights) w_lane = p.weights[i];
+    }
+    float dot[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int c0 = warp * 256; c0 < p.H; c0 += warps * 256) {
+      Eight<T, VEC, 32> g;
+      g.load(dout, c0, lane, p.H);
+      if (p.dw != nullptr) {
+        Eight<T, VEC, 32> v[8];
 #pragma unroll
-      for (int k = 0; k < kPass; ++k) g[k].load(dout, base + (k * kWarps + warp) * 256, lane, p.H);
-#pragma unroll 2
-      for (int j = 0; j < nj; ++j) {
-        const int d = p.dest[t * p.top_k + j0 + j];
-        if (d < 0 || d >= p.rows) continue;
-        const float w = p.weights ? p.weights[t * p.top_k + j0 + j] : 1.0f;
-        const T* yr = static_cast<const T*>(p.y) + (size_t)d * p.y_stride;
-        T* dr = static_cast<T*>(p.dy) + (size_t)d * p.H;
-        float s = 0.0f;
-        if (p.dw != nullptr) {
-          Eight<T, VEC, 32> v[kPass];
-#pragma unroll
-          for (int k = 0; k < kPass; ++k) v[k].load(yr, base + (k * kWarps + warp) * 256, lane, p.H);
-#pragma unroll
-          for (int k = 0; k < kPass; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              s = fmaf(g[k].get(i), v[k].get(i), s);  // columns behind the row's end hold zeros
+        for (int j = 0; j < 8; ++j) {
+          const int d = __shfl_sync(0xffffffffu, d_lane, j);
+          v[j].load(static_cast<const T*>(p.y) + (size_t)max(d, 0) * p.y_stride, c0, lane, p.H, d >= 0);
         }
 #pragma unroll
-        for (int k = 0; k < kPass; ++k) {
-          Eight<T, VEC, 32> o;
+        for (int j = 0; j < 8; ++j)  // columns behind the row's end and rows of no pair hold zeros
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o.set(i, w * g[k].get(i));
-          o.store(dr, base + (k * kWarps + warp) * 256, lane, p.H);
-        }
-        if (p.dw != nullptr) {
+          for (int i = 0; i < 8; ++i) dot[j] = fmaf(g.get(i), v[j].get(i), dot[j]);
+      }
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (lane == j) dot += s;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int d = __shfl_sync(0xffffffffu, d_lane, j);
+        const float w = __shfl_sync(0xffffffffu, w_lane, j);
+        if (d < 0) continue;
+        Eight<T, VEC, 32> o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.set(i, w * g.get(i));
+        o.store(static_cast<T*>(p.dy) + (size_t)d * p.H, c0, lane, p.H);
       }
     }
     if (p.dw != nullptr) {
-      part[warp][lane] = dot;
-      __syncthreads();
-      if (threadIdx.x < nj) {
-        float s = part[0][lane];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) s += part[w][lane];
-        p.dw[t * p.top_k + j0 + lane] = s;  // zero for a pair without a row
+      for (int j = 0; j < 8; ++j) {
+        const int d = __shfl_sync(0xffffffffu, d_lane, j);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+        if (lane == 0) part[warp][j] = d < 0 ? 0.0f : dot[j];  // (0 * dout is NaN where dout is infinite)
+      }
+      __syncthreads();
+      if (threadIdx.x < 8 && j0 + static_cast<int>(threadIdx.x) < j_end) {
+        float s = part[0][threadIdx.x];
+        for (int w = 1; w < warps; ++w) s += part[w][threadIdx.x];
+        p.dw[(size_t)t * p.top_k + j0 + threadIdx.x] = s;
       }
       __syncthreads();
     }
@@ -433,7 +442,7 @@ __global__ void __launch_bounds__(kUnsortGradThreads) token_unsort_grad_kernel(c
 constexpr int kClearThreads = 128;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kClearThreads) clear_rows_kernel(T* out, const int32_t* m_indices, int rows, int H) {
-  clear_rows_block<T, VEC, kClearThreads>(out, m_indices, rows, H, blockIdx.x, gridDim.x);
+  clear_rows_block<T, VEC>(out, m_indices, rows, H, blockIdx.x, gridDim.x);
 }
 
 }  // namespace dg

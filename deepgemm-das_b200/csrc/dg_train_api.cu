@@ -52,8 +52,11 @@ int blocks_for(long long units, int per_block, const DeviceInfo& dev, int per_sm
 // The pairs above which a block does not count all of them itself.
 constexpr long long kSortSelfCount = 65536;
 
+#ifndef SORT_PER_SM
+#define SORT_PER_SM 1
+#endif
 int sort_tokens_per_block(int tokens, int top_k, int sms) {
-  long long per = (tokens + 4LL * sms - 1) / (4LL * sms);
+  long long per = (tokens + SORT_PER_SM * (long long)sms - 1) / (SORT_PER_SM * (long long)sms);
   const long long most = kSortMaxChunk / top_k;
   if (per > most) per = most;
   return static_cast<int>(per < 1 ? 1 : per);
@@ -174,7 +177,9 @@ int dg_token_unsort(const dg_token_unsort_args* a, void* stream) {
   p.rows = a->num_rows;
   p.y_stride = a->y_stride;
   const bool vec = vec_rows(p.y, p.y_stride, p.H, a->elem) && aligned16(p.out);
-  const int grid = blocks_for((long long)p.T * ((p.H + 255) / 256), kUnsortThreads / 32, *dev, 8);
+  const long long units = (long long)p.T * ((p.H + 255) / 256);
+  if (units > 0xffffff00LL) return DG_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>((units + kUnsortThreads / 32 - 1) / (kUnsortThreads / 32));
   by_type(a->elem, vec, [&](auto t, auto v) {
     token_unsort_kernel<decltype(t), decltype(v)::value><<<grid, kUnsortThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   });
@@ -212,6 +217,9 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
   p.dout_stride = a->dout_stride;
   // few tokens: a block for every pair, so that more SMs take part
   p.per = (long long)p.T >= 4LL * dev->sm_count ? p.top_k : 1;
+  // as many warps as divide the row's 256-column pieces evenly
+  const int pieces = (p.H + 255) / 256, turns = (pieces + kUnsortGradWarps - 1) / kUnsortGradWarps;
+  const int warps = (pieces + turns - 1) / turns;
   p.clear_blocks = a->clear && p.rows > 0 ? blocks_for(p.rows, 16, *dev, 2) : 0;
   const long long grid = (long long)p.T * ((p.top_k + p.per - 1) / p.per) + p.clear_blocks;
   if (grid == 0) return DG_OK;
@@ -219,7 +227,7 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
                    (!p.dw || vec_rows(p.y, p.y_stride, p.H, a->elem));
   by_type(a->elem, vec, [&](auto t, auto v) {
     token_unsort_grad_kernel<decltype(t), decltype(v)::value>
-        <<<static_cast<unsigned>(grid), kUnsortGradThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        <<<static_cast<unsigned>(grid), 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(p);
   });
   return launched(1);
 }
@@ -263,7 +271,9 @@ static int checkpoint_common(bool restore, const dg_checkpoint_args* a, void* st
   p.x_stride = a->x_stride;
   const bool vec = vec_rows(p.x, p.x_stride, p.H, a->elem) && aligned_to(p.q, 8);
   const long long units = (long long)p.rows * ((p.H + kCkBlock - 1) / kCkBlock);
-  const int grid = blocks_for(units, kCkThreads / kCkLanes, *dev, 8);
+  const long long want = (units + kCkUnits * kCkGroups - 1) / (kCkUnits * kCkGroups);
+  if (want > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>(want);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_type(a->elem, vec, [&](auto t, auto v) {
     using T = decltype(t);
@@ -321,7 +331,9 @@ static int act_checkpoint_common(bool grad, const dg_act_checkpoint_args* a, voi
                    (grad ? aligned16(p.dx) && vec_rows(p.dact, p.dact_stride, p.H, a->elem)
                          : vec_rows(p.x, p.x_stride, p.H, a->elem));
   const long long units = (long long)p.rows * ((p.H + kCkBlock - 1) / kCkBlock);
-  const int grid = blocks_for(units, kCkThreads / kCkLanes, *dev, 8);
+  const long long want = (units + kCkActUnits * kCkGroups - 1) / (kCkActUnits * kCkGroups);
+  if (want > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>(want);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_type(a->elem, vec, [&](auto t, auto v) {
     using T = decltype(t);
