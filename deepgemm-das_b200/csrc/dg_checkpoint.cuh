@@ -14,11 +14,17 @@
 // all in fp32, rounded once.  The backward kernel also hands out act again, which the gradient
 // of the weights behind it needs, so that the forward pass need not keep it.
 //
-// Bound by HBM: 8 bytes per activation forward (4 read, 2 + 2 written), 10 backward (2 + 2 read,
-// 4 + 2 written).  16 lanes hold the 128 columns of one scale, eight each.
+// HBM moves 8 bytes per activation forward (4 read, 2 + 2 written) and 10 backward (2 + 2 read, 4 + 2
+// written); with that little work per byte the instructions count as much as the bytes.  So 8 lanes
+// hold the 128 columns of one scale, sixteen each (what a block of columns costs once, its
+// address, exchanges between lanes and scale, is spread over twice the columns that 16 lanes give;
+// see the figures at the kernels), 16-bit magnitudes are compared two at a time and codes are made
+// and read two (e4m3) or four (int8) at a time.
 #pragma once
 
 #include <cuda_fp8.h>
+
+#include <string.h>
 
 #include <type_traits>
 
@@ -28,9 +34,88 @@ namespace dg {
 
 constexpr int kCkBlock = 128;    // columns of one scale
 constexpr int kCkThreads = 256;
-constexpr int kCkLanes = 16;     // lanes of one block of columns
 
-// The largest magnitude of 128 columns, over the 16 lanes that hold them, as the bits of an fp32
+// What a lane holds of a block's 128 columns.  VEC: 8 lanes, each eight of the first 64 columns and
+// eight of the others.  Otherwise (rows that begin anywhere) 32 lanes, columns lane, lane + 32, ...,
+// so that a warp's accesses of single values lie side by side.
+template <class T, bool VEC>
+struct CkValues {
+  static constexpr int kLanes = 8, N = 16;
+  Eight<T, true, 8> h[2];
+  __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols, bool on) {
+    h[0].load(row, c0, lane, cols, on);
+    h[1].load(row, c0 + 64, lane, cols, on);
+  }
+  __device__ __forceinline__ void store(T* row, int c0, int lane, int cols) const {
+    h[0].store(row, c0, lane, cols);
+    h[1].store(row, c0 + 64, lane, cols);
+  }
+  __device__ __forceinline__ float get(int i) const { return h[i / 8].get(i % 8); }
+  __device__ __forceinline__ void set2(int i, float a, float b) { h[i / 8].set2(i % 8, a, b); }
+  __device__ __forceinline__ uint32_t pair(int i) const { return reinterpret_cast<const uint32_t*>(h[i / 4].raw)[i % 4]; }
+};
+template <class T>
+struct CkValues<T, false> {
+  static constexpr int kLanes = 32, N = 4;
+  T val[4] = {T(), T(), T(), T()};
+  __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols, bool on) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) val[i] = on && c0 + lane + 32 * i < cols ? row[c0 + lane + 32 * i] : T();
+  }
+  __device__ __forceinline__ void store(T* row, int c0, int lane, int cols) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + lane + 32 * i < cols) row[c0 + lane + 32 * i] = val[i];
+  }
+  __device__ __forceinline__ float get(int i) const { return to_f32(val[i]); }
+  __device__ __forceinline__ void set2(int i, float a, float b) {
+    val[i] = from_f32<T>(a);
+    val[i + 1] = from_f32<T>(b);
+  }
+  __device__ __forceinline__ uint32_t pair(int i) const {
+    const T two[2] = {val[2 * i], val[2 * i + 1]};
+    uint32_t v;
+    memcpy(&v, two, 4);
+    return v;
+  }
+};
+template <bool VEC>
+struct CkCodes {
+  EightBytes<true, 8> h[2];
+  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on) {
+    h[0].load(row, c0, lane, cols, on);
+    h[1].load(row, c0 + 64, lane, cols, on);
+  }
+  __device__ __forceinline__ void store(uint8_t* row, int c0, int lane, int cols) const {
+    h[0].store(row, c0, lane, cols);
+    h[1].store(row, c0 + 64, lane, cols);
+  }
+  __device__ __forceinline__ uint16_t& two(int i) { return h[i / 4].half[i % 4]; }
+  __device__ __forceinline__ uint16_t two(int i) const { return h[i / 4].half[i % 4]; }
+  __device__ __forceinline__ uint32_t& four(int i) { return h[i / 2].word[i % 2]; }
+  __device__ __forceinline__ uint32_t four(int i) const { return h[i / 2].word[i % 2]; }
+};
+template <>
+struct CkCodes<false> {
+  uint32_t word = 0;
+  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (on && c0 + lane + 32 * i < cols) word |= static_cast<uint32_t>(row[c0 + lane + 32 * i]) << (8 * i);
+  }
+  __device__ __forceinline__ void store(uint8_t* row, int c0, int lane, int cols) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + lane + 32 * i < cols) row[c0 + lane + 32 * i] = static_cast<uint8_t>(word >> (8 * i));
+  }
+  __device__ __forceinline__ uint16_t& two(int i) { return reinterpret_cast<uint16_t*>(&word)[i]; }
+  __device__ __forceinline__ uint16_t two(int i) const { return static_cast<uint16_t>(word >> (16 * i)); }
+  __device__ __forceinline__ uint32_t& four(int) { return word; }
+  __device__ __forceinline__ uint32_t four(int) const { return word; }
+};
+
+// The largest magnitude of 128 columns, over the lanes that hold them, as the bits of an fp32
 // value.  Magnitudes order like their bits, NaN and infinities above everything finite.  16-bit
 // types compare two at a time, and two blocks of columns (gate and up) share the exchanges between
 // the lanes.
@@ -46,32 +131,32 @@ __device__ __forceinline__ uint32_t ck_bits16(uint32_t b) {  // bits of a 16-bit
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(b))));
 }
 template <class T, bool VEC>
-__device__ __forceinline__ uint32_t ck_lane_max16(const Eight<T, VEC, kCkLanes>& v) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(v.raw);
-  const uint32_t m = ck_max2(ck_max2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), ck_max2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-  return max(m >> 16, m & 0xffffu);
+__device__ __forceinline__ uint32_t ck_lane_max(const CkValues<T, VEC>& v) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < v.N / 2; ++i) m = ck_max2(m, v.pair(i) & 0x7fff7fffu);
+    return max(m >> 16, m & 0xffffu);
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < v.N; ++i) m = max(m, __float_as_uint(v.get(i)) & 0x7fffffffu);
+    return m;
+  }
 }
 template <class T, bool VEC>
-__device__ __forceinline__ uint32_t ck_lane_max32(const Eight<T, VEC, kCkLanes>& v) {
-  uint32_t m = 0;
+__device__ __forceinline__ uint32_t ck_top(const CkValues<T, VEC>& v) {
+  uint32_t m = ck_lane_max(v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v.get(i)) & 0x7fffffffu);
-  return m;
-}
-template <class T, bool VEC>
-__device__ __forceinline__ uint32_t ck_top(const Eight<T, VEC, kCkLanes>& v) {
-  uint32_t m = sizeof(T) == 2 ? ck_lane_max16(v) : ck_lane_max32(v);
-#pragma unroll
-  for (int o = kCkLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = v.kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   return ck_bits16<T>(m);
 }
 template <class T, bool VEC>
-__device__ __forceinline__ void ck_top_of_two(const Eight<T, VEC, kCkLanes>& v0, const Eight<T, VEC, kCkLanes>& v1, uint32_t& t0,
-                                              uint32_t& t1) {
+__device__ __forceinline__ void ck_top_of_two(const CkValues<T, VEC>& v0, const CkValues<T, VEC>& v1, uint32_t& t0, uint32_t& t1) {
   if constexpr (sizeof(T) == 2) {
-    uint32_t m = (ck_lane_max16(v0) << 16) | ck_lane_max16(v1);
+    uint32_t m = (ck_lane_max(v0) << 16) | ck_lane_max(v1);
 #pragma unroll
-    for (int o = kCkLanes / 2; o > 0; o >>= 1) m = ck_max2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = v0.kLanes / 2; o > 0; o >>= 1) m = ck_max2(m, __shfl_xor_sync(0xffffffffu, m, o));
     t0 = ck_bits16<T>(m >> 16);
     t1 = ck_bits16<T>(m & 0xffffu);
   } else {
@@ -111,49 +196,49 @@ __device__ __forceinline__ float ck_quotient(float x, float s, float inv) {
   return fmaf(fmaf(-q, s, x), inv, q);
 }
 
-// Codes of eight values.
-template <int KIND, bool VEC, class Values>
-__device__ __forceinline__ EightBytes<VEC, kCkLanes> ck_codes(const Values& x, float s, float inv) {
-  EightBytes<VEC, kCkLanes> q;
+// Codes of a lane's values.
+template <int KIND, class T, bool VEC>
+__device__ __forceinline__ CkCodes<VEC> ck_codes(const CkValues<T, VEC>& x, float s, float inv) {
+  CkCodes<VEC> q;
   if constexpr (KIND == DG_KIND_E4M3) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      q.half[i] = __nv_cvt_float2_to_fp8x2(make_float2(x.get(2 * i) * inv, x.get(2 * i + 1) * inv), __NV_SATFINITE, __NV_E4M3);
+    for (int i = 0; i < x.N / 2; ++i)
+      q.two(i) = __nv_cvt_float2_to_fp8x2(make_float2(x.get(2 * i) * inv, x.get(2 * i + 1) * inv), __NV_SATFINITE, __NV_E4M3);
   } else {
     // Adding 1.5 * 2^23 rounds to a whole number (nearest, ties to even) and leaves it in the low bits;
     // |x| <= 127 s up to a rounding, so nothing lies beyond 127.
-    uint32_t n[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = __float_as_uint(ck_quotient(x.get(i), s, inv) + 12582912.0f);
+    for (int i = 0; i < x.N / 4; ++i) {
+      uint32_t n[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      q.word[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
+      for (int k = 0; k < 4; ++k) n[k] = __float_as_uint(ck_quotient(x.get(4 * i + k), s, inv) + 12582912.0f);
+      q.four(i) = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+    }
   }
   return q;
 }
 
-// The values that eight codes stand for, at most `most` in magnitude (NaN stays NaN): a value just
+// The values that a lane's codes stand for, at most `most` in magnitude (NaN stays NaN): a value just
 // below the largest of its type may have been rounded up to a code beyond it (255 to 256 of 2^120,
 // say) and still comes back finite.
-template <int KIND, bool VEC>
-__device__ __forceinline__ void ck_values(const EightBytes<VEC, kCkLanes>& q, float s, float most, float (&v)[8]) {
+template <int KIND, bool VEC, int N>
+__device__ __forceinline__ void ck_values(const CkCodes<VEC>& q, float s, float most, float (&v)[N]) {
   if constexpr (KIND == DG_KIND_E4M3) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(q.half[i], __NV_E4M3)));
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(q.two(i), __NV_E4M3)));
       v[2 * i] = f.x * s;
       v[2 * i + 1] = f.y * s;
     }
   } else {
     // byte + 128 under the exponent of 2^23: 8388608 + byte + 128
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = (__uint_as_float(__byte_perm(q.word[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)) - 8388736.0f) * s;
+    for (int i = 0; i < N; ++i)
+      v[i] = (__uint_as_float(__byte_perm(q.four(i / 4) ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)) - 8388736.0f) * s;
   }
+  if (448.0f * s > most) {  // (no code stands for more than 448 s; not so for NaN, which stays)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(most));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(-most));
+    for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
   }
 }
 constexpr float kCkMaxF32 = 3.402823466e+38f;
@@ -166,17 +251,21 @@ __device__ __forceinline__ float ck_most<__half>() { return 65504.0f; }
 template <>
 __device__ __forceinline__ float ck_most<__nv_bfloat16>() { return 3.3895313892515355e+38f; }
 
-// 1 / (1 + exp(-g)).  16-bit results take the hardware's exp and reciprocal (relative error below
-// 2^-21 where the sigmoid is not negligible), 32-bit ones the exact forms.
+// 1 / (1 + exp(-g)).  16-bit results take the hardware's 2^x and reciprocal without their handling
+// of subnormal numbers (exp(-g) below 2^-126 disappears beside the 1, a sigmoid below 2^-126 is 0),
+// 32-bit ones the exact forms.
 template <class T>
 __device__ __forceinline__ float ck_sigmoid(float g) {
   if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
-  return __fdividef(1.0f, 1.0f + __expf(-g));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
 }
 template <class T>
 __device__ __forceinline__ float ck_silu(float g) {
   if constexpr (sizeof(T) == 4) return g / (1.0f + expf(-g));
-  return __fdividef(g, 1.0f + __expf(-g));
+  return g * ck_sigmoid<T>(g);
 }
 
 struct CheckpointParams {
@@ -188,18 +277,18 @@ struct CheckpointParams {
   long long x_stride;
 };
 
-// A unit is 128 columns of one row, the work of 16 lanes; a block takes kCkUnits of them for each
-// group of 16 lanes, all of whose loads are under way before the first is used.
-constexpr int kCkUnits = 4;
-constexpr int kCkGroups = kCkThreads / kCkLanes;
+// A unit is 128 columns of one row, the work of 8 lanes; a block takes kCkUnits of them for each
+// group of 8 lanes, all of whose loads are under way before the first is used.
+template <bool VEC>
+constexpr int kCkUnits = VEC ? 1 : 2;
 struct CkUnit {
   long long u, r;  // u: the unit; r: its row, -1 behind the last unit
   int b;           // its block of columns
 };
-template <int UNITS = kCkUnits>
+template <int LANES, int UNITS>
 __device__ __forceinline__ CkUnit ck_unit(int k, int rows, int blocks) {
   CkUnit w;
-  w.u = ((long long)blockIdx.x * UNITS + k) * kCkGroups + threadIdx.x / kCkLanes;
+  w.u = ((long long)blockIdx.x * UNITS + k) * (kCkThreads / LANES) + threadIdx.x / LANES;
   const long long all = (long long)rows * blocks;
   if (all <= 0xffffffffLL) {
     const uint32_t r = static_cast<uint32_t>(w.u) / static_cast<uint32_t>(blocks);
@@ -216,21 +305,22 @@ __device__ __forceinline__ CkUnit ck_unit(int k, int rows, int blocks) {
 // Rows into a checkpoint.
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) checkpoint_rows_kernel(const CheckpointParams p) {
-  const int lane = threadIdx.x & (kCkLanes - 1);
+  constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkUnits<VEC>;
+  const int lane = threadIdx.x & (kLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  CkUnit w[kCkUnits];
-  Eight<T, VEC, kCkLanes> v[kCkUnits];
+  CkUnit w[U];
+  CkValues<T, VEC> v[U];
 #pragma unroll
-  for (int k = 0; k < kCkUnits; ++k) {
-    w[k] = ck_unit(k, p.rows, blocks);
+  for (int k = 0; k < U; ++k) {
+    w[k] = ck_unit<kLanes, U>(k, p.rows, blocks);
     v[k].load(static_cast<const T*>(p.x) + (size_t)max(w[k].r, 0LL) * p.x_stride, w[k].b * kCkBlock, lane, p.H, w[k].r >= 0);
   }
 #pragma unroll
-  for (int k = 0; k < kCkUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     float s, inv;
     ck_scale<KIND>(ck_top(v[k]), s, inv);  // every lane takes part
     if (w[k].r < 0) continue;
-    ck_codes<KIND, VEC>(v[k], s, inv).store(p.q + (size_t)w[k].r * p.H, w[k].b * kCkBlock, lane, p.H);
+    ck_codes<KIND>(v[k], s, inv).store(p.q + (size_t)w[k].r * p.H, w[k].b * kCkBlock, lane, p.H);
     if (lane == 0) p.scale[w[k].u] = s;
   }
 }
@@ -238,25 +328,26 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_rows_kernel(const Check
 // And out of it.
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) restore_rows_kernel(const CheckpointParams p) {
-  const int lane = threadIdx.x & (kCkLanes - 1);
+  constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkUnits<VEC>;
+  const int lane = threadIdx.x & (kLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  CkUnit w[kCkUnits];
-  EightBytes<VEC, kCkLanes> q[kCkUnits];
-  float s[kCkUnits];
+  CkUnit w[U];
+  CkCodes<VEC> q[U];
+  float s[U];
 #pragma unroll
-  for (int k = 0; k < kCkUnits; ++k) {
-    w[k] = ck_unit(k, p.rows, blocks);
+  for (int k = 0; k < U; ++k) {
+    w[k] = ck_unit<kLanes, U>(k, p.rows, blocks);
     q[k].load(p.q + (size_t)max(w[k].r, 0LL) * p.H, w[k].b * kCkBlock, lane, p.H, w[k].r >= 0);
     s[k] = w[k].r >= 0 ? p.scale[w[k].u] : 0.0f;
   }
 #pragma unroll
-  for (int k = 0; k < kCkUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     if (w[k].r < 0) continue;
-    float f[8];
+    float f[N];
     ck_values<KIND, VEC>(q[k], s[k], ck_most<T>(), f);
-    Eight<T, VEC, kCkLanes> v;
+    CkValues<T, VEC> v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v.set(i, f[i]);
+    for (int i = 0; i < N; i += 2) v.set2(i, f[i], f[i + 1]);
     v.store(static_cast<T*>(p.out) + (size_t)w[k].r * p.H, w[k].b * kCkBlock, lane, p.H);
   }
 }
@@ -277,24 +368,25 @@ constexpr int kCkActUnits = 2;
 
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) act_checkpoint_kernel(const ActCheckpointParams p) {
-  const int lane = threadIdx.x & (kCkLanes - 1);
+  constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkActUnits;
+  const int lane = threadIdx.x & (kLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  CkUnit w[kCkActUnits];
-  bool skip[kCkActUnits];
-  Eight<T, VEC, kCkLanes> g[kCkActUnits], up[kCkActUnits];
+  CkUnit w[U];
+  bool skip[U];
+  CkValues<T, VEC> g[U], up[U];
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
-    w[k] = ck_unit<kCkActUnits>(k, p.rows, blocks);
+  for (int k = 0; k < U; ++k) {
+    w[k] = ck_unit<kLanes, U>(k, p.rows, blocks);
     skip[k] = w[k].r < 0 || (p.m_indices != nullptr && p.m_indices[w[k].r] < 0);
   }
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     const T* x = static_cast<const T*>(p.x) + (size_t)max(w[k].r, 0LL) * p.x_stride;
     g[k].load(x, w[k].b * kCkBlock, lane, p.H, !skip[k]);
     up[k].load(x + p.H, w[k].b * kCkBlock, lane, p.H, !skip[k]);
   }
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     float sg, ig, su, iu;
     uint32_t tg, tu;
     ck_top_of_two(g[k], up[k], tg, tu);  // every lane takes part
@@ -302,13 +394,14 @@ __global__ void __launch_bounds__(kCkThreads) act_checkpoint_kernel(const ActChe
     ck_scale<KIND>(tu, su, iu);
     if (w[k].r < 0 || (skip[k] && !p.clear)) continue;
     const int c0 = w[k].b * kCkBlock;
-    Eight<T, VEC, kCkLanes> a;
+    CkValues<T, VEC> a;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a.set(i, ck_silu<T>(g[k].get(i)) * up[k].get(i));
+    for (int i = 0; i < N; i += 2)
+      a.set2(i, ck_silu<T>(g[k].get(i)) * up[k].get(i), ck_silu<T>(g[k].get(i + 1)) * up[k].get(i + 1));
     a.store(static_cast<T*>(p.act) + (size_t)w[k].r * p.H, c0, lane, p.H);
     uint8_t* q = p.q + (size_t)w[k].r * 2 * p.H;
-    ck_codes<KIND, VEC>(g[k], sg, ig).store(q, c0, lane, p.H);
-    ck_codes<KIND, VEC>(up[k], su, iu).store(q + p.H, c0, lane, p.H);
+    ck_codes<KIND>(g[k], sg, ig).store(q, c0, lane, p.H);
+    ck_codes<KIND>(up[k], su, iu).store(q + p.H, c0, lane, p.H);
     if (lane == 0) {
       float* s = p.scale + (size_t)w[k].r * 2 * blocks;
       s[w[k].b] = sg;
@@ -319,20 +412,21 @@ __global__ void __launch_bounds__(kCkThreads) act_checkpoint_kernel(const ActChe
 
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) act_checkpoint_grad_kernel(const ActCheckpointParams p) {
-  const int lane = threadIdx.x & (kCkLanes - 1);
+  constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkActUnits;
+  const int lane = threadIdx.x & (kLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
-  CkUnit w[kCkActUnits];
-  bool skip[kCkActUnits];
-  EightBytes<VEC, kCkLanes> qg[kCkActUnits], qu[kCkActUnits];
-  Eight<T, VEC, kCkLanes> d[kCkActUnits];
-  float sg[kCkActUnits], su[kCkActUnits];
+  CkUnit w[U];
+  bool skip[U];
+  CkCodes<VEC> qg[U], qu[U];
+  CkValues<T, VEC> d[U];
+  float sg[U], su[U];
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
-    w[k] = ck_unit<kCkActUnits>(k, p.rows, blocks);
+  for (int k = 0; k < U; ++k) {
+    w[k] = ck_unit<kLanes, U>(k, p.rows, blocks);
     skip[k] = w[k].r < 0 || (p.m_indices != nullptr && p.m_indices[w[k].r] < 0);
   }
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     const size_t r = static_cast<size_t>(max(w[k].r, 0LL));
     const float* s = p.scale + r * 2 * blocks;
     const uint8_t* q = p.q + r * 2 * p.H;
@@ -344,21 +438,28 @@ __global__ void __launch_bounds__(kCkThreads) act_checkpoint_grad_kernel(const A
     su[k] = skip[k] ? 0.0f : s[blocks + w[k].b];
   }
 #pragma unroll
-  for (int k = 0; k < kCkActUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     if (w[k].r < 0 || (skip[k] && !p.clear)) continue;
-    Eight<T, VEC, kCkLanes> dg, du, a;
+    CkValues<T, VEC> dg, du, a;
     if (!skip[k]) {
-      float gv[8], uv[8];
+      float gv[N], uv[N];
       ck_values<KIND, VEC>(qg[k], sg[k], kCkMaxF32, gv);
       ck_values<KIND, VEC>(qu[k], su[k], kCkMaxF32, uv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float dv = d[k].get(i);
-        const float sig = ck_sigmoid<T>(gv[i]);
-        const float silu = gv[i] * sig;
-        dg.set(i, dv * uv[i] * sig * fmaf(gv[i], 1.0f - sig, 1.0f));
-        du.set(i, dv * silu);
-        a.set(i, silu * uv[i]);
+      for (int i = 0; i < N; i += 2) {
+        float fg[2], fu[2], fa[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float dv = d[k].get(i + j), gj = gv[i + j], uj = uv[i + j];
+          const float sig = ck_sigmoid<T>(gj);
+          const float silu = gj * sig;
+          fg[j] = dv * uj * sig * fmaf(gj, 1.0f - sig, 1.0f);
+          fu[j] = dv * silu;
+          fa[j] = silu * uj;
+        }
+        dg.set2(i, fg[0], fg[1]);
+        du.set2(i, fu[0], fu[1]);
+        a.set2(i, fa[0], fa[1]);
       }
     }
     const int c0 = w[k].b * kCkBlock;

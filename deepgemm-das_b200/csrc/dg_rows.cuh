@@ -96,6 +96,22 @@ struct Eight {
   }
   __device__ __forceinline__ float get(int i) const { return to_f32(val[i]); }
   __device__ __forceinline__ void set(int i, float v) { val[i] = from_f32<T>(v); }  // round to nearest even
+  __device__ __forceinline__ void set2(int i, float a, float b) {                   // i and i + 1 (i even)
+    if constexpr (sizeof(T) == 4) {
+      set(i, a);
+      set(i + 1, b);
+    } else {
+      reinterpret_cast<uint32_t*>(raw)[i / 2] = pack2(a, b, T());
+    }
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 
 // The same for 8-bit codes: one 8-byte access, or byte by byte.

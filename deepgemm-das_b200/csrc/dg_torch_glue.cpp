@@ -5,8 +5,8 @@
 // deepgemm/_core.py does the same checks with tensor attribute reads, about 7 us a call; for a
 // sparse decode step that is half of what the kernel takes.  This module does them natively.
 //
-// It is deliberately only the accepting half: each function returns true when the arguments
-// passed every check and the launch was enqueued, false when anything at all is unusual (a
+// It is deliberately only the accepting half: each function returns true (or its results) when the
+// arguments passed every check and the launch was enqueued, false (or None) when anything at all is unusual (a
 // check failed, a layout this file does not know, a device that is not current, a launch error).
 // On false nothing was enqueued and the caller runs the Python marshalling, which either raises
 // the error with its full message or handles the unusual case.  No message text lives here.
@@ -195,6 +195,308 @@ bool contiguous(int64_t kind, int64_t scale_mode, const Tensor& a, const Tensor&
   return count(contiguous_impl(kind, scale_mode, a, b, d, a_scale, b_scale, m_indices, block_n, status));
 }
 
+// ------------------------------------------------------------------ operators of a training step
+// These allocate their results as the Python functions do (deepgemm/token_sort.py,
+// activation_checkpoint.py, grouped_grad.py) and return them, or None with nothing enqueued.
+namespace py = pybind11;
+
+inline int elem_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return DG_OUT_BF16;
+    case at::kHalf: return DG_OUT_F16;
+    case at::kFloat: return DG_OUT_F32;
+    default: return -1;
+  }
+}
+inline int code_kind(at::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? DG_KIND_E4M3 : (t == at::kChar ? DG_KIND_I8 : -1);
+}
+inline int current(const Tensor& t) {  // the tensor's device if it is the current one, else -1
+  if (!t.is_cuda()) return -1;
+  const int dev = static_cast<int>(t.get_device());
+  return dev >= 0 && dev < kMaxDevices && dev == c10::cuda::current_device() ? dev : -1;
+}
+// [rows, H] of a known type on `dev`, rows whole and apart
+inline bool rows_ok(const Tensor& t, int dev) {
+  return t.is_cuda() && t.get_device() == dev && t.dim() == 2 && elem_of(t) >= 0 && t.size(1) >= 1 && t.size(0) <= INT32_MAX &&
+         t.size(1) <= INT32_MAX / 8 && (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) < 2 || t.stride(0) >= t.size(1));
+}
+inline int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+inline bool ints_ok(const Tensor& t, int dev, int64_t n) { return on(t, dev) && t.scalar_type() == at::kInt && t.numel() == n; }
+inline void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
+inline Tensor make(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
+  return at::empty(size, at::TensorOptions().dtype(type).device(like.device()));
+}
+inline py::object count_obj(py::object o) {
+  count(!o.is_none());
+  return o;
+}
+
+py::object sort_impl(const Tensor& x, const Tensor& ids, int64_t experts, int64_t align, const OptTensor& out) {
+  const int dev = current(x);
+  if (dev < 0 || !rows_ok(x, dev) || !on(ids, dev) || ids.dim() != 2 || ids.size(0) != x.size(0)) return py::none();
+  if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) return py::none();
+  const int64_t t = ids.size(0), k = ids.size(1), h = x.size(1);
+  if (k < 1 || k > DG_MAX_TOP_K || experts < 1 || experts > DG_MAX_GROUPS || align < 1 || align > INT32_MAX) return py::none();
+  int32_t* status = status_ptr(c10::nullopt, dev);
+  const int64_t cap = dg_token_sort_capacity(t * k, static_cast<int32_t>(experts), static_cast<int32_t>(align));
+  if (status == nullptr || cap < 0 || cap > INT32_MAX) return py::none();
+  if (out.has_value() && (!on(*out, dev) || out->scalar_type() != x.scalar_type() || out->dim() != 2 || out->size(0) != cap || out->size(1) != h))
+    return py::none();
+  Tensor rows = out.has_value() ? *out : make({cap, h}, x.scalar_type(), x);
+  Tensor dest = make({t, k}, at::kInt, x), m_indices = make({cap}, at::kInt, x), counts = make({experts}, at::kInt, x),
+         offsets = make({experts}, at::kInt, x), m_total = make({1}, at::kInt, x), scratch;
+  dg_token_sort_args a{};
+  a.elem_bytes = static_cast<int32_t>(x.element_size());
+  a.ids64 = ids.scalar_type() == at::kLong;
+  a.num_tokens = static_cast<int32_t>(t);
+  a.top_k = static_cast<int32_t>(k);
+  a.num_groups = static_cast<int32_t>(experts);
+  a.hidden = static_cast<int32_t>(h);
+  a.align = static_cast<int32_t>(align);
+  a.cap = static_cast<int32_t>(cap);
+  a.x_stride = row_stride(x);
+  a.x = x.data_ptr();
+  a.ids = ids.data_ptr();
+  a.rows = rows.data_ptr();
+  a.dest = dest.data_ptr<int32_t>();
+  a.m_indices = m_indices.data_ptr<int32_t>();
+  a.counts = counts.data_ptr<int32_t>();
+  a.offsets = offsets.data_ptr<int32_t>();
+  a.m_total = m_total.data_ptr<int32_t>();
+  a.scratch_bytes = dg_token_sort_scratch_bytes(a.num_tokens, a.top_k, a.num_groups);
+  if (a.scratch_bytes > 0) {
+    scratch = make({static_cast<int64_t>(a.scratch_bytes)}, at::kByte, x);
+    a.scratch = scratch.data_ptr();
+  }
+  a.status = status;
+  a.clear = !out.has_value();
+  if (dg_token_sort(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::make_tuple(rows, dest, m_indices, counts, offsets, m_total);
+}
+
+py::object unsort_impl(const Tensor& y, const Tensor& dest, const Tensor& m_indices, const OptTensor& weights, const OptTensor& out) {
+  const int dev = current(y);
+  if (dev < 0 || !rows_ok(y, dev) || !on(dest, dev) || dest.scalar_type() != at::kInt || dest.dim() != 2 ||
+      !ints_ok(m_indices, dev, y.size(0)))
+    return py::none();
+  const int64_t t = dest.size(0), k = dest.size(1), h = y.size(1);
+  if (weights.has_value() && (!on(*weights, dev) || weights->scalar_type() != at::kFloat || weights->sizes() != dest.sizes())) return py::none();
+  if (out.has_value() && (!on(*out, dev) || out->scalar_type() != y.scalar_type() || out->dim() != 2 || out->size(0) != t || out->size(1) != h))
+    return py::none();
+  Tensor o = out.has_value() ? *out : make({t, h}, y.scalar_type(), y);
+  dg_token_unsort_args a{};
+  a.elem = elem_of(y);
+  a.num_tokens = static_cast<int32_t>(t);
+  a.top_k = static_cast<int32_t>(k);
+  a.hidden = static_cast<int32_t>(h);
+  a.num_rows = static_cast<int32_t>(y.size(0));
+  a.y_stride = row_stride(y);
+  a.y = y.data_ptr();
+  a.dest = dest.data_ptr<int32_t>();
+  a.weights = weights.has_value() ? weights->data_ptr<float>() : nullptr;
+  a.out = o.data_ptr();
+  if (dg_token_unsort(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::cast(o);
+}
+
+py::object unsort_grad_impl(const Tensor& dout, const Tensor& y, const Tensor& dest, const Tensor& m_indices, const OptTensor& weights,
+                            bool need_dweights) {
+  const int dev = current(y);
+  if (dev < 0 || !rows_ok(y, dev) || !rows_ok(dout, dev) || !on(dest, dev) || dest.scalar_type() != at::kInt || dest.dim() != 2 ||
+      !ints_ok(m_indices, dev, y.size(0)))
+    return py::none();
+  const int64_t t = dest.size(0), k = dest.size(1), h = y.size(1);
+  if (dout.scalar_type() != y.scalar_type() || dout.size(0) != t || dout.size(1) != h) return py::none();
+  if (weights.has_value() && (!on(*weights, dev) || weights->scalar_type() != at::kFloat || weights->sizes() != dest.sizes())) return py::none();
+  Tensor dy = make({y.size(0), h}, y.scalar_type(), y), dw;
+  if (weights.has_value() && need_dweights) dw = make({t, k}, at::kFloat, y);
+  dg_token_unsort_grad_args a{};
+  a.elem = elem_of(y);
+  a.num_tokens = static_cast<int32_t>(t);
+  a.top_k = static_cast<int32_t>(k);
+  a.hidden = static_cast<int32_t>(h);
+  a.num_rows = static_cast<int32_t>(y.size(0));
+  a.clear = 1;
+  a.y_stride = row_stride(y);
+  a.dout_stride = row_stride(dout);
+  a.dout = dout.data_ptr();
+  a.y = y.data_ptr();
+  a.dest = dest.data_ptr<int32_t>();
+  a.weights = weights.has_value() ? weights->data_ptr<float>() : nullptr;
+  a.m_indices = m_indices.data_ptr<int32_t>();
+  a.dy = dy.data_ptr();
+  a.dw = dw.defined() ? dw.data_ptr<float>() : nullptr;
+  if (dg_token_unsort_grad(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::make_tuple(dy, dw.defined() ? py::cast(dw) : py::none());
+}
+
+inline int64_t scale_blocks(int64_t h) { return (h + 127) / 128; }
+
+py::object checkpoint_impl(const Tensor& x, int64_t kind) {
+  const int dev = current(x);
+  if (dev < 0 || !rows_ok(x, dev)) return py::none();
+  Tensor q = make(x.sizes(), kind == DG_KIND_E4M3 ? at::kFloat8_e4m3fn : at::kChar, x);
+  Tensor scale = make({x.size(0), scale_blocks(x.size(1))}, at::kFloat, x);
+  dg_checkpoint_args a{};
+  a.elem = elem_of(x);
+  a.kind = static_cast<int32_t>(kind);
+  a.num_rows = static_cast<int32_t>(x.size(0));
+  a.hidden = static_cast<int32_t>(x.size(1));
+  a.x_stride = row_stride(x);
+  a.x = x.data_ptr();
+  a.q = q.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  if (dg_checkpoint_rows(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::make_tuple(q, scale);
+}
+
+// the checkpoint of rows that consist of `halves` parts with blocks of their own
+inline bool kept_ok(const Tensor& q, const Tensor& scale, int dev, int64_t halves) {
+  return on(q, dev) && on(scale, dev) && q.dim() == 2 && code_kind(q.scalar_type()) >= 0 && q.size(1) >= halves && q.size(1) % halves == 0 &&
+         q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX / 8 && scale.scalar_type() == at::kFloat && scale.dim() == 2 &&
+         scale.size(0) == q.size(0) && scale.size(1) == halves * scale_blocks(q.size(1) / halves);
+}
+
+py::object restore_impl(const Tensor& q, const Tensor& scale, int64_t elem) {
+  const int dev = current(q);
+  const at::ScalarType type = elem == DG_OUT_F32 ? at::kFloat : (elem == DG_OUT_F16 ? at::kHalf : at::kBFloat16);
+  if (dev < 0 || !kept_ok(q, scale, dev, 1)) return py::none();
+  Tensor x = make(q.sizes(), type, q);
+  dg_checkpoint_args a{};
+  a.elem = elem_of(x);
+  a.kind = code_kind(q.scalar_type());
+  a.num_rows = static_cast<int32_t>(q.size(0));
+  a.hidden = static_cast<int32_t>(q.size(1));
+  a.x_stride = q.size(1);
+  a.x = x.data_ptr();
+  a.q = q.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  if (dg_restore_rows(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::cast(x);
+}
+
+py::object act_impl(const Tensor& x, int64_t kind, const OptTensor& m_indices) {
+  const int dev = current(x);
+  if (dev < 0 || !rows_ok(x, dev) || x.size(1) % 2 != 0 || (m_indices.has_value() && !ints_ok(*m_indices, dev, x.size(0)))) return py::none();
+  const int64_t m = x.size(0), h = x.size(1) / 2;
+  Tensor act = make({m, h}, x.scalar_type(), x), q = make(x.sizes(), kind == DG_KIND_E4M3 ? at::kFloat8_e4m3fn : at::kChar, x),
+         scale = make({m, 2 * scale_blocks(h)}, at::kFloat, x);
+  dg_act_checkpoint_args a{};
+  a.elem = elem_of(x);
+  a.kind = static_cast<int32_t>(kind);
+  a.num_rows = static_cast<int32_t>(m);
+  a.hidden = static_cast<int32_t>(h);
+  a.clear = 1;
+  a.x_stride = row_stride(x);
+  a.x = x.data_ptr();
+  a.q = q.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  a.act = act.data_ptr();
+  a.m_indices = m_indices.has_value() ? m_indices->data_ptr<int32_t>() : nullptr;
+  if (dg_act_checkpoint(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::make_tuple(act, q, scale);
+}
+
+py::object act_grad_impl(const Tensor& q, const Tensor& scale, const Tensor& dact, const OptTensor& m_indices, bool need_act) {
+  const int dev = current(q);
+  if (dev < 0 || !kept_ok(q, scale, dev, 2) || !rows_ok(dact, dev) || dact.size(0) != q.size(0) || 2 * dact.size(1) != q.size(1) ||
+      (m_indices.has_value() && !ints_ok(*m_indices, dev, q.size(0))))
+    return py::none();
+  const int64_t m = dact.size(0), h = dact.size(1);
+  Tensor dx = make({m, 2 * h}, dact.scalar_type(), q), act;
+  if (need_act) act = make({m, h}, dact.scalar_type(), q);
+  dg_act_checkpoint_args a{};
+  a.elem = elem_of(dact);
+  a.kind = code_kind(q.scalar_type());
+  a.num_rows = static_cast<int32_t>(m);
+  a.hidden = static_cast<int32_t>(h);
+  a.clear = 1;
+  a.dact_stride = row_stride(dact);
+  a.dact = dact.data_ptr();
+  a.q = q.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  a.act = act.defined() ? act.data_ptr() : nullptr;
+  a.dx = dx.data_ptr();
+  a.m_indices = m_indices.has_value() ? m_indices->data_ptr<int32_t>() : nullptr;
+  if (dg_act_checkpoint_grad(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::make_tuple(dx, act.defined() ? py::cast(act) : py::none());
+}
+
+// a contiguous bf16 [rows, columns] operand of the grouped products
+inline bool operand_ok(const Tensor& t, int dev) {
+  return on(t, dev) && t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX;
+}
+
+py::object input_grad_impl(const Tensor& dy, const Tensor& w, const Tensor& m_indices, const OptTensor& out, int64_t block_n) {
+  const int dev = current(dy);
+  int64_t g, n, k;
+  if (dev < 0 || !operand_ok(dy, dev) || !on(w, dev) || w.scalar_type() != at::kBFloat16 || !weight_dims(w, DG_KIND_BF16, &g, &n, &k) ||
+      dy.size(1) != n || g > INT32_MAX || k > INT32_MAX || m_indices.dim() != 1 || !ints_ok(m_indices, dev, dy.size(0)))
+    return py::none();
+  if (out.has_value() && (!operand_ok(*out, dev) || out->size(0) != dy.size(0) || out->size(1) != k)) return py::none();
+  int32_t* status = status_ptr(c10::nullopt, dev);
+  if (status == nullptr) return py::none();
+  Tensor dx = out.has_value() ? *out : make({dy.size(0), k}, at::kBFloat16, dy);
+  dg_input_grad_args a{};
+  a.dy = dy.data_ptr();
+  a.w_packed = w.data_ptr();
+  a.dx = dx.data_ptr();
+  a.m_indices = m_indices.data_ptr<int32_t>();
+  a.num_groups = static_cast<int32_t>(g);
+  a.m_total = static_cast<int32_t>(dy.size(0));
+  a.n = static_cast<int32_t>(n);
+  a.k = static_cast<int32_t>(k);
+  a.block_n = static_cast<int32_t>(block_n);
+  a.status = status;
+  if (dg_grouped_input_grad(&a, stream_of(dev)) != DG_OK) return py::none();
+  if (!out.has_value() && a.m_total > 0) {
+    dg_clear_rows_args c{};
+    c.elem = DG_OUT_BF16;
+    c.num_rows = a.m_total;
+    c.hidden = a.k;
+    c.rows = a.dx;
+    c.m_indices = a.m_indices;
+    // (declined after the product was enqueued: the Python path computes the same once more)
+    if (dg_clear_padding_rows(&c, stream_of(dev)) != DG_OK) return py::none();
+  }
+  return py::cast(dx);
+}
+
+py::object weight_grad_impl(const Tensor& dy, const Tensor& x, const Tensor& m_indices, int64_t groups, const OptTensor& out, bool f32,
+                            bool accumulate, int64_t tile) {
+  const int dev = current(dy);
+  if (dev < 0 || !operand_ok(dy, dev) || !operand_ok(x, dev) || x.size(0) != dy.size(0) || m_indices.dim() != 1 ||
+      !ints_ok(m_indices, dev, dy.size(0)) || groups < 1 || groups > DG_MAX_GROUPS)
+    return py::none();
+  const int64_t n = dy.size(1), k = x.size(1);
+  if (n < 16 || n % 16 != 0 || k < 64 || k % 64 != 0 || (accumulate && !out.has_value())) return py::none();
+  if (out.has_value()) {
+    const Tensor& o = *out;
+    if (!on(o, dev) || o.dim() != 4 || o.size(0) != groups || o.size(1) != k / 64 || o.size(2) != n || o.size(3) != 64 ||
+        (o.scalar_type() != at::kBFloat16 && o.scalar_type() != at::kFloat) || (accumulate && o.scalar_type() != at::kFloat))
+      return py::none();
+  }
+  int32_t* status = status_ptr(c10::nullopt, dev);
+  if (status == nullptr) return py::none();
+  Tensor dw = out.has_value() ? *out : make({groups, k / 64, n, 64}, f32 ? at::kFloat : at::kBFloat16, dy);
+  dg_weight_grad_args a{};
+  a.dy = dy.data_ptr();
+  a.x = x.data_ptr();
+  a.dw = dw.data_ptr();
+  a.m_indices = m_indices.data_ptr<int32_t>();
+  a.num_groups = static_cast<int32_t>(groups);
+  a.m_total = static_cast<int32_t>(dy.size(0));
+  a.n = static_cast<int32_t>(n);
+  a.k = static_cast<int32_t>(k);
+  a.out_kind = dw.scalar_type() == at::kFloat ? DG_OUT_F32 : DG_OUT_BF16;
+  a.accumulate = accumulate;
+  a.tile = static_cast<int32_t>(tile);
+  a.status = status;
+  if (dg_grouped_weight_grad(&a, stream_of(dev)) != DG_OK) return py::none();
+  return py::cast(dw);
+}
+
 void set_status_words(int64_t device, const Tensor& words) {
   TORCH_CHECK(device >= 0 && device < kMaxDevices, "device index out of range");
   TORCH_CHECK(words.is_cuda() && words.get_device() == device && words.scalar_type() == at::kInt &&
@@ -209,6 +511,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "native argument checks and launch for the grouped GEMM entry points (accepting half only)";
   m.def("masked", &masked, "enqueue dg_masked_gemm if every check passes; False otherwise");
   m.def("contiguous", &contiguous, "enqueue dg_contig_gemm if every check passes; False otherwise");
+  // results, or None with nothing enqueued
+  m.def("sort_tokens", [](const Tensor& x, const Tensor& ids, int64_t e, int64_t align, const OptTensor& out) {
+    return count_obj(sort_impl(x, ids, e, align, out));
+  });
+  m.def("unsort_tokens", [](const Tensor& y, const Tensor& dest, const Tensor& mi, const OptTensor& w, const OptTensor& out) {
+    return count_obj(unsort_impl(y, dest, mi, w, out));
+  });
+  m.def("unsort_tokens_grad", [](const Tensor& dout, const Tensor& y, const Tensor& dest, const Tensor& mi, const OptTensor& w, bool need) {
+    return count_obj(unsort_grad_impl(dout, y, dest, mi, w, need));
+  });
+  m.def("checkpoint_rows", [](const Tensor& x, int64_t kind) { return count_obj(checkpoint_impl(x, kind)); });
+  m.def("restore_rows", [](const Tensor& q, const Tensor& s, int64_t elem) { return count_obj(restore_impl(q, s, elem)); });
+  m.def("silu_mul_checkpoint", [](const Tensor& x, int64_t kind, const OptTensor& mi) { return count_obj(act_impl(x, kind, mi)); });
+  m.def("silu_mul_checkpoint_grad", [](const Tensor& q, const Tensor& s, const Tensor& d, const OptTensor& mi, bool need) {
+    return count_obj(act_grad_impl(q, s, d, mi, need));
+  });
+  m.def("input_grad", [](const Tensor& dy, const Tensor& w, const Tensor& mi, const OptTensor& out, int64_t bn) {
+    return count_obj(input_grad_impl(dy, w, mi, out, bn));
+  });
+  m.def("weight_grad", [](const Tensor& dy, const Tensor& x, const Tensor& mi, int64_t g, const OptTensor& out, bool f32, bool acc, int64_t tile) {
+    return count_obj(weight_grad_impl(dy, x, mi, g, out, f32, acc, tile));
+  });
   m.def("set_status_words", &set_status_words);
   m.def("stats", []() { return std::make_pair(g_accepted, g_declined); }, "(calls enqueued here, calls handed back)");
   // the header this file was compiled against; the caller compares it with the library's own

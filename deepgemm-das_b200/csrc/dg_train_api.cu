@@ -271,7 +271,8 @@ static int checkpoint_common(bool restore, const dg_checkpoint_args* a, void* st
   p.x_stride = a->x_stride;
   const bool vec = vec_rows(p.x, p.x_stride, p.H, a->elem) && aligned_to(p.q, 8);
   const long long units = (long long)p.rows * ((p.H + kCkBlock - 1) / kCkBlock);
-  const long long want = (units + kCkUnits * kCkGroups - 1) / (kCkUnits * kCkGroups);
+  const int per_block = vec ? kCkUnits<true> * kCkThreads / 8 : kCkUnits<false> * kCkThreads / 32;
+  const long long want = (units + per_block - 1) / per_block;
   if (want > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
   const unsigned grid = static_cast<unsigned>(want);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -331,7 +332,8 @@ static int act_checkpoint_common(bool grad, const dg_act_checkpoint_args* a, voi
                    (grad ? aligned16(p.dx) && vec_rows(p.dact, p.dact_stride, p.H, a->elem)
                          : vec_rows(p.x, p.x_stride, p.H, a->elem));
   const long long units = (long long)p.rows * ((p.H + kCkBlock - 1) / kCkBlock);
-  const long long want = (units + kCkActUnits * kCkGroups - 1) / (kCkActUnits * kCkGroups);
+  const int per_block = kCkActUnits * kCkThreads / (vec ? 8 : 32);
+  const long long want = (units + per_block - 1) / per_block;
   if (want > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
   const unsigned grid = static_cast<unsigned>(want);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

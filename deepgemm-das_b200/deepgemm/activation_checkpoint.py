@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _cabi
 from ._cabi import KIND_E4M3, KIND_I8
-from ._core import _launch
+from ._core import _glue, _launch
 from .token_sort import _ELEM, _grad_arg, _int_arg, _rows_arg
 
 _CODES = {"fp8": (KIND_E4M3, torch.float8_e4m3fn), "int8": (KIND_I8, torch.int8)}
@@ -61,8 +61,10 @@ def _check(c: Checkpoint, halves: int, what: str) -> None:
 def checkpoint_rows(x: torch.Tensor, *, kind: str = "fp8") -> Checkpoint:
     """x bf16 / fp16 / fp32 ``[M, H]`` (rows may lie apart) -> its checkpoint."""
     what = "checkpoint_rows"
-    _rows_arg(x, "x", what)
     code, qdtype = _kind(kind, what)
+    if _glue is not None and (made := _glue.checkpoint_rows(x, code)) is not None:
+        return Checkpoint(*made, x.dtype)
+    _rows_arg(x, "x", what)
     m, h = (int(v) for v in x.shape)
     q = torch.empty((m, h), dtype=qdtype, device=x.device)
     scale = torch.empty((m, _blocks(h)), dtype=torch.float32, device=x.device)
@@ -76,6 +78,9 @@ def restore_rows(checkpoint: Checkpoint) -> torch.Tensor:
     """The rows that a checkpoint holds, in the type they had: ``q * scale``, rounded once and at most
     the type's largest finite value."""
     what = "restore_rows"
+    if _glue is not None and checkpoint.dtype in _ELEM and \
+            (made := _glue.restore_rows(checkpoint.q, checkpoint.scale, _ELEM[checkpoint.dtype])) is not None:
+        return made
     _check(checkpoint, 1, what)
     q, scale, dtype = checkpoint
     m, h = (int(v) for v in q.shape)
@@ -92,8 +97,10 @@ def silu_mul_checkpoint(x: torch.Tensor, *, kind: str = "fp8", m_indices: Option
     ``act = gate * sigmoid(gate) * up`` in fp32 from x itself, rounded once.  Rows with ``m_indices < 0``
     are not read; their ``act`` is zero and their checkpoint holds zeros."""
     what = "silu_mul_checkpoint"
-    _rows_arg(x, "x", what)
     code, qdtype = _kind(kind, what)
+    if _glue is not None and (made := _glue.silu_mul_checkpoint(x, code, m_indices)) is not None:
+        return made[0], Checkpoint(made[1], made[2], x.dtype)
+    _rows_arg(x, "x", what)
     if x.shape[1] % 2:
         raise ValueError(f"{what}: the rows of x must hold a gate and an up half, got {x.shape[1]} columns")
     m, h = int(x.shape[0]), int(x.shape[1]) // 2
@@ -117,6 +124,9 @@ def silu_mul_checkpoint_grad(checkpoint: Checkpoint, dact: torch.Tensor, *, m_in
     those values once more (what the weight gradient behind it multiplies; None unless asked for).
     Rows with ``m_indices < 0`` are zero in both, whatever ``dact`` holds there."""
     what = "silu_mul_checkpoint_grad"
+    if _glue is not None and dact.dtype == checkpoint.dtype and \
+            (made := _glue.silu_mul_checkpoint_grad(checkpoint.q, checkpoint.scale, dact, m_indices, need_act)) is not None:
+        return made
     _check(checkpoint, 2, what)
     q, scale, dtype = checkpoint
     m, h = int(q.shape[0]), int(q.shape[1]) // 2

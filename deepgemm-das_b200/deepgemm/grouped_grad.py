@@ -17,7 +17,7 @@ import torch
 
 from . import _cabi
 from ._cabi import KIND_BF16
-from ._core import _launch, device_status_words, packed_weight_dims
+from ._core import _glue, _launch, device_status_words, packed_weight_dims
 from .token_sort import clear_padding_rows
 
 
@@ -42,6 +42,8 @@ def grouped_bf16_input_grad(dy: torch.Tensor, weight: torch.Tensor, m_indices: t
     """dy bf16 ``[M, N]``, weight the packed bf16 ``[G, K/64, N, 64]`` -> dx bf16 ``[M, K]``.  Rows with
     ``m_indices < 0`` are zero, or, in a given ``out``, left as they are."""
     what = "grouped_bf16_input_grad"
+    if _glue is not None and (made := _glue.input_grad(dy, weight, m_indices, out, block_n)) is not None:
+        return made
     _bf16_rows(dy, "dy", what)
     g, n, k = packed_weight_dims(weight, KIND_BF16)
     if weight.device != dy.device or weight.dtype != torch.bfloat16 or not weight.is_contiguous():
@@ -73,6 +75,9 @@ def grouped_bf16_weight_grad(dy: torch.Tensor, x: torch.Tensor, m_indices: torch
     type of ``out``), summed in fp32.  ``accumulate`` adds to a given fp32 ``out``, for micro-batches;
     otherwise groups without rows give zeros."""
     what = "grouped_bf16_weight_grad"
+    if _glue is not None and dtype in (torch.bfloat16, torch.float32) and \
+            (made := _glue.weight_grad(dy, x, m_indices, num_groups, out, dtype == torch.float32, accumulate, tile)) is not None:
+        return made
     _bf16_rows(dy, "dy", what)
     _bf16_rows(x, "x", what)
     if x.device != dy.device or x.shape[0] != dy.shape[0]:

@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
-from ._core import _launch, device_status_words
+from ._core import _glue, _launch, device_status_words
 
 _ELEM = {torch.bfloat16: _cabi.OUT_BF16, torch.float16: _cabi.OUT_F16, torch.float32: _cabi.OUT_F32}
 
@@ -71,6 +71,9 @@ def _out_arg(out: torch.Tensor, like: torch.Tensor, shape, what: str) -> torch.T
 
 
 def _sort(x, topk_ids, num_experts, align, out):
+    # the native glue does all of this if nothing is unusual; otherwise it has done nothing
+    if _glue is not None and (made := _glue.sort_tokens(x, topk_ids, num_experts, align, out)) is not None:
+        return made
     what = "sort_tokens"
     _rows_arg(x, "x", what)
     if topk_ids.device != x.device or topk_ids.dtype not in (torch.int32, torch.int64):
@@ -131,6 +134,8 @@ def _plan_args(y, plan, weights, what):
 def sort_tokens_grad(drows: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
     """Gradient of ``sort_tokens`` with respect to its tokens: ``dx[t] = sum_j drows[dest[t, j]]``,
     summed in fp32 and in order.  Rows that stand for no pair are not read."""
+    if _glue is not None and (dx := _glue.unsort_tokens(drows, plan.dest, plan.m_indices, None, None)) is not None:
+        return dx
     dest, _, _ = _plan_args(drows, plan, None, "sort_tokens_grad")
     return _unsort(drows, dest, None, None, "sort_tokens_grad")
 
@@ -140,6 +145,8 @@ def unsort_tokens_grad(dout: torch.Tensor, y: torch.Tensor, plan: TokenPlan, wei
     """Gradients of ``unsort_tokens``: ``dy[dest[t, j]] = weights[t, j] * dout[t]`` (zero in rows that
     stand for no pair) and ``dweights[t, j] = <dout[t], y[dest[t, j]]>`` in fp32 (zero for a pair
     without a row; None without weights)."""
+    if _glue is not None and (made := _glue.unsort_tokens_grad(dout, y, plan.dest, plan.m_indices, weights, need_dweights)) is not None:
+        return made
     what = "unsort_tokens_grad"
     dest, m_indices, weights = _plan_args(y, plan, weights, what)
     _rows_arg(dout, "dout", what)
@@ -212,8 +219,11 @@ def unsort_tokens(y: torch.Tensor, plan: TokenPlan, weights: Optional[torch.Tens
     j; y ``[rows, H]`` in the plan's layout, weights fp32 ``[T, top_k]`` or None for ones.  Pairs
     without a row add nothing.  Differentiable in y and weights; the gradient of y is zero in rows
     that stand for no pair."""
+    recorded = torch.is_grad_enabled() and (y.requires_grad or weights is not None and weights.requires_grad)
+    if _glue is not None and not recorded and (made := _glue.unsort_tokens(y, plan.dest, plan.m_indices, weights, out)) is not None:
+        return made
     dest, m_indices, w = _plan_args(y, plan, weights, "unsort_tokens")
-    if torch.is_grad_enabled() and (y.requires_grad or w is not None and w.requires_grad):
+    if recorded:
         if out is not None:
             raise ValueError("unsort_tokens: out cannot be given where a gradient is recorded")
         return _UnsortTokens.apply(y, w, dest, m_indices)
