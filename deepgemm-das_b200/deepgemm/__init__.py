@@ -70,6 +70,7 @@ from .token_sort import (TokenPlan, clear_padding_rows, sort_capacity, sort_toke
 from .activation_checkpoint import (Checkpoint, checkpoint_rows, restore_rows, silu_mul, silu_mul_checkpoint,
                                     silu_mul_checkpoint_grad)
 from .grouped_grad import grouped_bf16_input_grad, grouped_bf16_weight_grad
+from .moe_train import expert_mlp_bf16, moe_forward_bf16
 from .print_size import install_op_size_printer
 from ._core import check_device_status
 
