@@ -8,7 +8,7 @@
 // is exactly the tensor cores' operand for 64 steps of the contraction, and neither operand is
 // transposed anywhere.
 //
-// Tiles and roles.  CL = 2: a cluster of two blocks computes 256 (n) x 256 (k) with
+// Tiles and roles.  kSplit: below.  CL = 2: a cluster of two blocks computes 256 (n) x 256 (k) with
 // tcgen05.mma.cta_group::2, block r owning rows [128 r, 128 r + 128) of the tile (its part of dY, its
 // accumulator, its epilogue) and holding 128 of the 256 columns of X.  CL = 1: one block, 128 x 128,
 // for problems with few tiles.  Either way a ring stage holds 64 rows of 128 columns of each
@@ -32,6 +32,11 @@
 // front of the tensor cores: for every chunk that cost 1.0 us a chunk (a remote arrival with
 // cluster-wide release and an acquire to match, on the path of every stage), for ragged chunks
 // alone still 0.5 us a work item (32 groups of 300 to 3000 rows, 4096 x 7168: 1.65 ms instead of 1.55).
+// kSplit (CL = 1): few tiles and many rows.  A cluster of 2, 4 or 8 blocks takes one tile, each block
+// its share of the group's row blocks; the fp32 partial tiles stay in shared memory (in the ring,
+// which is idle by then) and each block adds its share of the tile's rows over the cluster, in the
+// order of the blocks, so no result depends on timing (1 group of 8000 rows, 512 x 768: 40.6 -> 19.4
+// us; 2 of 4000 rows, 256 x 256: 24.2 -> 12.7).
 // Groups without rows give zeros (or, added, nothing) and cost no products.
 //
 // Every mbarrier wait is bounded, as in the other kernels.
@@ -66,6 +71,8 @@ struct WgradParams {
   int32_t* status;
   int f32;                   // output type: fp32 (else bf16)
   int add;                   // fp32 only: add to what the output holds
+  int split;                 // kSplit: blocks of a cluster
+  void* dw;                  // kSplit: the output
   int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
 };
 
@@ -110,7 +117,16 @@ __device__ __forceinline__ void wg_store_commit() { asm volatile("cp.async.bulk.
 __device__ __forceinline__ void wg_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void wg_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-template <int CL, int S>
+__device__ __forceinline__ float4 wg_load_cluster(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
+  return v;
+}
+
+template <int CL, int S, bool kSplit = false>
 __global__ void __launch_bounds__(kWgThreads, 1)
 grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_d, const WgradParams p) {
@@ -125,8 +141,10 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   uint8_t* smem = smem_raw + (base - raw_addr);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  static_assert(!kSplit || CL == 1, "a split tile is computed by single blocks");
   const uint32_t rank = CL == 2 ? cluster_ctarank() : 0u;
-  const int unit = blockIdx.x / CL, units = gridDim.x / CL;
+  const int part = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = kSplit ? blockIdx.x / p.split : blockIdx.x / CL, units = kSplit ? gridDim.x / p.split : gridDim.x / CL;
 
   auto bar_ready = [&](int s) { return base + L::off_bar + 8u * s; };
   auto bar_empty = [&](int s) { return base + L::off_bar + 8u * (S + s); };
@@ -265,6 +283,11 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     it.k0 = (t - nt * p.k_tiles) * BT;
     it.b0 = it.g > 0 ? first[it.g - 1] : 0;
     it.blocks = first[it.g] - it.b0;
+    if constexpr (kSplit) {  // this block's share of them
+      const int lo = it.blocks * part / p.split, hi = it.blocks * (part + 1) / p.split;
+      it.b0 += lo;
+      it.blocks = hi - lo;
+    }
     return it;
   };
 
@@ -531,6 +554,26 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       const int n = w.n0 + static_cast<int>(rank) * 128 + q * 32;
       const int kb0 = w.k0 / 64;
       const int kbs = n < p.N ? min(BT / 64, kb_all - kb0) : 0;  // 64-column blocks to store
+      if constexpr (kSplit) {
+        // this block's partial tile, row r of it at 512 r, 16-byte pieces swizzled with the row
+        const int r = q * 32 + lane;
+        float* row = reinterpret_cast<float*>(smem + L::off_stage + r * 512);
+        if (w.blocks > 0) {
+          if (!mbar_wait_warp(bar_acc_full(0), 0, abort_flag, WG_SITE_ACC_FULL)) break;
+          tc_fence_after_sync();
+        }
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t v[32] = {};
+          if (w.blocks > 0) {
+            tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c, v);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(row + 4 * ((c / 4 + i) ^ (r & 7))) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        break;  // one tile for a cluster
+      }
       if (w.blocks == 0) {
         if (!p.add && kbs > 0) {
           before();
@@ -584,6 +627,48 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       ++tile;
     }
     if (lane == 0) wg_store_wait();  // the strip lives until its last store is done
+  }
+
+  if constexpr (kSplit) {
+    // ---- the cluster's partial tiles added up: rows [128 / split * part, ...) of the tile here
+    __syncthreads();
+    cluster_sync_all();
+    if (unit < n_items) {
+      const Item w = item_of(unit);
+      const int rows = 128 / p.split, r0 = part * rows;
+      const int kb_all = p.K / 64;
+      for (int i = tid; i < rows * 32; i += kWgThreads) {
+        const int r = r0 + (i >> 5), piece = i & 31;
+        const int n = w.n0 + r, k = w.k0 + 4 * piece;
+        if (n >= p.N || k >= p.K) continue;
+        const uint32_t at = base + L::off_stage + r * 512 + ((piece ^ (r & 7)) << 4);
+        float4 s = wg_load_cluster(mapa_shared(at, 0));
+        for (int b = 1; b < p.split; ++b) {
+          const float4 v = wg_load_cluster(mapa_shared(at, b));
+          s.x += v.x;
+          s.y += v.y;
+          s.z += v.z;
+          s.w += v.w;
+        }
+        const size_t o = ((static_cast<size_t>(w.g) * kb_all + k / 64) * p.N + n) * 64 + k % 64;
+        if (p.f32) {
+          float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.dw) + o);
+          if (p.add) {
+            const float4 v = *d;
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+          }
+          *d = s;
+        } else {
+          const __nv_bfloat162 h0 = __floats2bfloat162_rn(s.x, s.y), h1 = __floats2bfloat162_rn(s.z, s.w);
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.dw) + o) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+        }
+      }
+    }
+    cluster_sync_all();  // nobody leaves while another block reads its partial tile
   }
 
   // ---- tear-down

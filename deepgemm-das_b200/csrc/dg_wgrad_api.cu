@@ -7,9 +7,10 @@ namespace {
 using namespace dg;
 using namespace dg::host;
 
-template <int CL, int S>
+template <int CL, int S, bool kSplit = false>
 int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& dev, cudaStream_t stream) {
-  auto kernel = grouped_wgrad_kernel<CL, S>;
+  auto kernel = grouped_wgrad_kernel<CL, S, kSplit>;
+  const int cluster = kSplit ? p.split : CL;
   constexpr int BT = 128 * CL;
   p.n_tiles = (p.N + BT - 1) / BT;
   p.k_tiles = (p.K + BT - 1) / BT;
@@ -44,7 +45,7 @@ int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& 
 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
@@ -64,18 +65,22 @@ int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& 
     if (max_units[devid] == 0) {
       cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem);
       if (e != cudaSuccess) return cuda_fail(e);
-      cudaLaunchConfig_t q = cfg;
-      q.gridDim = dim3(dev.sm_count / CL * CL, 1, 1);
-      q.dynamicSmemBytes = dev.max_smem;
-      int n = 0;
-      e = cudaOccupancyMaxActiveClusters(&n, kernel, &q);
-      if (e != cudaSuccess) return cuda_fail(e);
-      if (n < 1) return DG_ERR_TOO_LARGE;
-      max_units[devid] = n < dev.sm_count / CL ? n : dev.sm_count / CL;
+      if (!kSplit) {
+        cudaLaunchConfig_t q = cfg;
+        q.gridDim = dim3(dev.sm_count / CL * CL, 1, 1);
+        q.dynamicSmemBytes = dev.max_smem;
+        int n = 0;
+        e = cudaOccupancyMaxActiveClusters(&n, kernel, &q);
+        if (e != cudaSuccess) return cuda_fail(e);
+        if (n < 1) return DG_ERR_TOO_LARGE;
+        max_units[devid] = n < dev.sm_count / CL ? n : dev.sm_count / CL;
+      } else {
+        max_units[devid] = 0x7fffffff / 8;  // a cluster for every tile: none waits for another
+      }
     }
   }
   const long long units = items < max_units[devid] ? items : max_units[devid];
-  cfg.gridDim = dim3(static_cast<unsigned>(CL * units), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster * units), 1, 1);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm_dy, tm_x, tm_d, p);
   if (e != cudaSuccess) return cuda_fail(e);
   count_launches(1);
@@ -91,7 +96,7 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   if (a->num_groups < 1 || a->m_total < 0 || a->n < 16 || a->n % 16 != 0 || a->k < 64 || a->k % 64 != 0) return DG_ERR_BAD_SHAPE;
   if (a->out_kind != DG_OUT_BF16 && a->out_kind != DG_OUT_F32) return DG_ERR_BAD_ARGUMENT;
   if (a->accumulate != 0 && a->out_kind != DG_OUT_F32) return DG_ERR_BAD_ARGUMENT;  // sums are kept in 32 bits
-  if (a->tile != 0 && a->tile != 128 && a->tile != 256) return DG_ERR_BAD_ARGUMENT;
+  if (a->tile != 0 && a->tile != 128 && a->tile != 256 && a->tile != 1) return DG_ERR_BAD_ARGUMENT;
   if (a->num_groups > DG_MAX_GROUPS || a->m_total > DG_MAX_CONTIG_ROWS) return DG_ERR_TOO_LARGE;
   if ((long long)a->num_groups * (a->k / 64) > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
   if (!a->dw || (a->m_total > 0 && (!a->dy || !a->x || !a->m_indices))) return DG_ERR_NULL_POINTER;
@@ -112,14 +117,30 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   p.status = a->status;
   p.f32 = a->out_kind == DG_OUT_F32;
   p.add = a->accumulate != 0;
-  int tile = a->tile;
-  if (tile == 0) {
-    // 256 x 256 tiles move half the operand bytes per product; 128 x 128 ones give four times the
-    // work items, which small problems need to reach every SM.
-    const long long items = (long long)p.G * ((p.N + 255) / 256) * ((p.K + 255) / 256);
-    tile = items >= dev->sm_count / 2 ? 256 : 128;
-  }
+  p.dw = a->dw;
+  // 256 x 256 tiles move half the operand bytes per product, which pays when a group has rows enough
+  // and there are tiles enough; else 128 x 128 ones, whose epilogues are shorter and which reach more
+  // SMs.  Measured, 128 against 256, us: 32 groups of 1024 rows, 4096 x 7168: TILE_A; 256 of 128 rows,
+  // 1024 x 1792: 244 / 322; 16 of 64 rows, 4096 x 1024: 41 / 50; 32 of 300 rows, 1024 x 512: 24.5 /
+  // 24.2; 4 of 1000 rows, 1024 x 1024 (64 tiles of 256): 17.0 / 14.9; 8 of 2000 rows, 512 x 512 (32
+  // tiles): 19.1 / 22.4.
+  const long long rows = p.M / p.G;
+  const long long items256 = (long long)p.G * ((p.N + 255) / 256) * ((p.K + 255) / 256);
+  const long long items128 = (long long)p.G * ((p.N + 127) / 128) * ((p.K + 127) / 128);
+  const int tile = a->tile != 0 ? a->tile : (rows >= 320 && items256 >= 48 ? 256 : 128);
+  // Fewer 128 x 128 tiles than a half of the SMs and a long way along the rows: a tile is split, as
+  // often as there are SMs for it and four row blocks for every part.  us without and with: 1 group of
+  // 16000 rows, 256 x 64: 74.8 / 20.1; of 8000 rows, 512 x 768: 40.6 / 19.4; of 2000 rows, 128 x 128: 14.3 /
+  // 10.7; but 2 of 1000 rows, 256 x 256: 10.3 / 11.1.
+  int split = 1;
+  while (rows >= 1536 && split < 8 && items128 * split * 2 <= dev->sm_count && rows >= 128LL * 4 * split * 2) split *= 2;
+  if (a->tile == 1) split = 4;  // (asked for)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((a->tile == 0 && tile == 128 && split > 1) || a->tile == 1) {
+    p.split = split;
+    return WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem ? launch_wgrad<1, kWgStages, true>(a, p, *dev, st)
+                                                                         : launch_wgrad<1, kWgStages - 1, true>(a, p, *dev, st);
+  }
   // the table of very many rows takes the room of a ring stage
   if (WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem)
     return tile == 256 ? launch_wgrad<2, kWgStages>(a, p, *dev, st) : launch_wgrad<1, kWgStages>(a, p, *dev, st);

@@ -615,7 +615,7 @@ typedef struct dg_weight_grad_args {
   int32_t k;                /* multiple of 64 */
   int32_t out_kind;         /* DG_OUT_BF16 or DG_OUT_F32 */
   int32_t accumulate;       /* DG_OUT_F32 only */
-  int32_t tile;             /* 0 = choose; 128 / 256 */
+  int32_t tile;             /* 0 = choose; 128 / 256 = that tile; 1 = 128 with every tile split over four blocks */
   int32_t reserved;
   int32_t*       status;    /* NULL, or int32[DG_STATUS_WORDS] */
 } dg_weight_grad_args;

@@ -84,7 +84,7 @@ def test_input_grad_is_exact_on_whole_numbers(name, n, k, block_n):
 
 @pytest.mark.parametrize("name", LAYOUTS)
 @pytest.mark.parametrize("n,k", SIZES)
-@pytest.mark.parametrize("tile", [128, 256, 0])
+@pytest.mark.parametrize("tile", [128, 256, 0, 1])
 @pytest.mark.parametrize("dtype,add", [(torch.bfloat16, False), (torch.float32, False), (torch.float32, True)])
 def test_weight_grad_is_exact_on_whole_numbers(name, n, k, tile, dtype, add):
     counts, align, tail = LAYOUTS[name]
@@ -106,7 +106,7 @@ def test_weight_grad_is_exact_on_whole_numbers(name, n, k, tile, dtype, add):
     deepgemm.check_device_status()
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, 256, 1])
 def test_weight_grad_of_any_order_of_blocks_and_stray_rows(tile):
     """A group's blocks need not lie together, a block may hold rows that stand for nothing between
     others, and rows of another group than its first row's count for nothing."""
@@ -142,7 +142,7 @@ def test_groups_out_of_range_are_reported():
         deepgemm.check_device_status()
 
 
-@pytest.mark.parametrize("counts,n,k,tile", [([700, 50, 1300], 1024, 768, 256), ([700, 50, 1300], 304, 320, 128)])
+@pytest.mark.parametrize("counts,n,k,tile", [([700, 50, 1300], 1024, 768, 256), ([700, 50, 1300], 304, 320, 128), ([7000, 50, 1300], 304, 320, 0), ([5000], 128, 64, 0)])
 def test_random_values(counts, n, k, tile):
     mi = layout(counts, 128)
     gen = torch.Generator().manual_seed(1)
@@ -251,7 +251,7 @@ def test_refusals():
             call()
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, 256, 1])
 def test_the_most_rows_and_groups(tile):
     """4096 blocks of 128 rows, 1024 groups in a scattered order: the largest table."""
     m, g, n, k = 4096 * 128, 1024, 16, 64
