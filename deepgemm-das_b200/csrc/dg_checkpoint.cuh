@@ -60,7 +60,7 @@ struct CkValues<T, false> {
   T val[4] = {T(), T(), T(), T()};
   __device__ __forceinline__ void load(const T* row, int c0, int lane, int cols, bool on) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) val[i] = on && c0 + lane + 32 * i < cols ? row[c0 + lane + 32 * i] : T();
+    for (int i = 0; i < 4; ++i) val[i] = load_value(row + c0 + lane + 32 * i, on && c0 + lane + 32 * i < cols);
   }
   __device__ __forceinline__ void store(T* row, int c0, int lane, int cols) const {
 #pragma unroll

@@ -39,6 +39,28 @@ __device__ __forceinline__ uint2 load_once8(const void* p, bool on) {
   return v;
 }
 
+// One value of two or four bytes, likewise.
+template <class T>
+__device__ __forceinline__ T load_value(const T* p, bool on) {
+  T v;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t b;
+    asm volatile(
+        "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.u32 %0, 0;\n\t@on ld.global.nc.u32 %0, [%1];\n\t}"
+        : "=&r"(b)
+        : "l"(p), "r"(static_cast<uint32_t>(on)));
+    v = *reinterpret_cast<const T*>(&b);
+  } else {
+    uint16_t b;
+    asm volatile(
+        "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.u16 %0, 0;\n\t@on ld.global.nc.u16 %0, [%1];\n\t}"
+        : "=&h"(b)
+        : "l"(p), "r"(static_cast<uint32_t>(on)));
+    v = *reinterpret_cast<const T*>(&b);
+  }
+  return v;
+}
+
 template <class T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -75,7 +97,7 @@ struct Eight {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = c0 + lane + LANES * i;
-        val[i] = on && c < cols ? row[c] : T();
+        val[i] = load_value(row + c, on && c < cols);
       }
     }
   }

@@ -40,10 +40,7 @@ struct TokenSortParams {
   int rep;              // copies of the shared-memory histogram (fewer lanes meet at one address)
 };
 
-#ifndef SORT_T
-#define SORT_T 1024
-#endif
-constexpr int kSortThreads = SORT_T;
+constexpr int kSortThreads = 1024;
 constexpr int kSortMaxChunk = 2048;  // pairs of one block
 
 __device__ __forceinline__ int sort_id(const TokenSortParams& p, long long i) {
@@ -91,6 +88,10 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(int32_t* hist, int chunk
   if (lane == 0) hist[(size_t)chunks * G + e] = running;
 }
 
+// Values of VB bytes that a lane moves at once, and those of a warp.
+__host__ __device__ constexpr int sort_each(int vb) { return vb == 16 ? 4 : (vb == 4 ? 8 : 16); }
+__host__ __device__ constexpr int sort_seg(int vb) { return 32 * sort_each(vb); }
+
 template <int VB>
 struct BytesOf;
 template <>
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
   int32_t* hist = dest_s + p.tokens_per_block * p.top_k;  // [2][G][rep]
   __shared__ int bad_s, list_n;
   __shared__ int list[kSortThreads];
+  __shared__ int warp_sum[32];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long R = (long long)p.T * p.top_k;
@@ -125,6 +127,7 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
   const bool first = blockIdx.y == 0;
 
   if (tid == 0) bad_s = 0;
+  for (int i = tid; i < np; i += kSortThreads) dest_s[i] = sort_id(p, p0 + i);
   if (p.hist == nullptr) {
     for (int i = tid; i < 2 * p.G * p.rep; i += kSortThreads) hist[i] = 0;
     __syncthreads();
@@ -169,30 +172,34 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
       count[e] = p.hist[(size_t)gridDim.x * p.G + e];
     }
     __syncthreads();  // bad_s is zero before the ids below are looked at
-    for (long long i = p0 + tid; i < p0 + np; i += kSortThreads)
-      if (sort_id(p, i) >= p.G) bad_s = 1;
+    for (int i = tid; i < np; i += kSortThreads)
+      if (dest_s[i] >= p.G) bad_s = 1;
   }
   __syncthreads();
-  if (warp == 0) {
-    int running = 0;
-    for (int e0 = 0; e0 < p.G; e0 += 32) {
-      const int e = e0 + lane;
-      const int v = e < p.G ? (count[e] + p.align - 1) / p.align * p.align : 0;
-      int x = v;
+  // where the experts begin: a thread for each (G <= 1024 = kSortThreads)
+  {
+    static_assert(DG_MAX_GROUPS <= kSortThreads, "");
+    const int v = tid < p.G ? (count[tid] + p.align - 1) / p.align * p.align : 0;
+    int x = v;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (e < p.G) offset[e] = running + x - v;
-      running += __shfl_sync(0xffffffffu, x, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    if (lane == 0) offset[p.G] = running;
-    __syncwarp();
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int before_warp = 0;
+    if (warp * 32 < p.G)
+      for (int w = 0; w < warp; ++w) before_warp += warp_sum[w];
+    if (tid < p.G) offset[tid] = before_warp + x - v;
+    if (tid == p.G - 1) offset[p.G] = before_warp + x;
+    __syncthreads();
+  }
+  if (warp == 0) {
     // stable places of this block's pairs, 32 at a time
     for (int i0 = 0; i0 < np; i0 += 32) {
       const int i = i0 + lane;
-      const int e = i < np ? sort_id(p, p0 + i) : -1;
+      const int e = i < np ? dest_s[i] : -1;
       const bool in = e >= 0 && e < p.G;
       const unsigned same = __match_any_sync(0xffffffffu, in ? e : -1);
       const int rank = __popc(same & ((1u << lane) - 1u));
@@ -217,9 +224,9 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
   }
   if (tid == 0 && first && bad_s && p.status != nullptr) atomicCAS(p.status, DG_DEV_OK, DG_DEV_BAD_GROUP_INDEX);
 
-  // rows: a warp takes 4 x 32 vectors of one token at a time
+  // rows: a warp takes kEach x 32 values of one token at a time
   const int nv = p.row_bytes / VB;
-  constexpr int kSeg = 128;
+  constexpr int kEach = sort_each(VB), kSeg = sort_seg(VB);
   const int segs_all = (nv + kSeg - 1) / kSeg;
   const int segs_per = (segs_all + gridDim.y - 1) / gridDim.y;
   const int seg0 = blockIdx.y * segs_per, seg1 = min(seg0 + segs_per, segs_all);
@@ -228,16 +235,16 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
   for (int u = warp; u < nt * segs; u += kSortThreads / 32) {
     const int t = u / segs, v0 = (seg0 + u - t * segs) * kSeg + lane;
     const V* src = reinterpret_cast<const V*>(static_cast<const char*>(p.x) + (long long)(t0 + t) * p.x_stride);
-    V v[4];
+    V v[kEach];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kEach; ++i)
       if (v0 + 32 * i < nv) v[i] = __ldg(src + v0 + 32 * i);
     for (int j = 0; j < p.top_k; ++j) {
       const int d = dest_s[t * p.top_k + j];
       if (d < 0) continue;
       V* dst = reinterpret_cast<V*>(rows + (size_t)d * p.row_bytes);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kEach; ++i)
         if (v0 + 32 * i < nv) dst[v0 + 32 * i] = v[i];
     }
   }
@@ -270,7 +277,7 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
         const int i = u / segs, v0 = (seg0 + u - i * segs) * kSeg + lane;
         V* dst = reinterpret_cast<V*>(rows + (size_t)list[i] * p.row_bytes);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < kEach; ++k)
           if (v0 + 32 * k < nv) dst[v0 + 32 * k] = V{};
       }
       __syncthreads();
@@ -287,47 +294,56 @@ struct TokenUnsortParams {
   long long y_stride;    // values between rows of y
 };
 
-// out[t] = sum_j w * y[dest]: a warp takes 256 columns of one token; the rows of its pairs are
-// fetched together (up to eight in flight) and added in order.
+// out[t] = sum_j w * y[dest]: a warp takes kPairs pairs of one token at once and 8 / kPairs pieces of
+// 256 columns, i.e. always has eight pieces of rows on their way, and adds the pairs in order.  (With
+// one piece whatever top_k is, 16384 tokens x 7168 with top_k = 1 took 170 us; now 83.)
 constexpr int kUnsortThreads = 256;
-template <class T, bool VEC>
+template <class T, bool VEC, int kPairs>
 __global__ void __launch_bounds__(kUnsortThreads) token_unsort_kernel(const TokenUnsortParams p) {
+  constexpr int kPieces = 8 / kPairs;
   const int lane = threadIdx.x & 31;
-  const unsigned segs = (p.H + 255u) / 256u;
+  const unsigned segs = (p.H + 256u * kPieces - 1u) / (256u * kPieces);
   const unsigned u = blockIdx.x * (kUnsortThreads / 32u) + (threadIdx.x >> 5);  // the host keeps units below 2^32
   const unsigned t = u / segs;
   if (t >= static_cast<unsigned>(p.T)) return;
-  const int c0 = static_cast<int>(u - t * segs) * 256;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+  const int c0 = static_cast<int>(u - t * segs) * 256 * kPieces;
+  float acc[kPieces][8] = {};
+  for (int j0 = 0; j0 < p.top_k; j0 += kPairs) {
     int d = -1;
     float w = 1.0f;
-    if (lane < 8 && j0 + lane < p.top_k) {
+    if (lane < kPairs && j0 + lane < p.top_k) {
       const size_t i = (size_t)t * p.top_k + j0 + lane;
       d = p.dest[i];
       if (d >= p.rows) d = -1;
       if (p.weights) w = p.weights[i];
     }
-    Eight<T, VEC, 32> v[8];
-    int dj[8];
+    Eight<T, VEC, 32> v[kPairs][kPieces];
+    int dj[kPairs];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kPairs; ++j) {
       dj[j] = __shfl_sync(0xffffffffu, d, j);
-      v[j].load(static_cast<const T*>(p.y) + (size_t)max(dj[j], 0) * p.y_stride, c0, lane, p.H, dj[j] >= 0);
+      const T* row = static_cast<const T*>(p.y) + (size_t)max(dj[j], 0) * p.y_stride;
+#pragma unroll
+      for (int s = 0; s < kPieces; ++s) v[j][s].load(row, c0 + 256 * s, lane, p.H, dj[j] >= 0);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kPairs; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
       if (dj[j] >= 0) {  // a pair without a row adds nothing, whatever its weight is
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(wj, v[j].get(i), acc[i]);
+        for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[s][i] = fmaf(wj, v[j][s].get(i), acc[s][i]);
       }
     }
   }
-  Eight<T, VEC, 32> o;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o.set(i, acc[i]);
-  o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0, lane, p.H);
+  for (int s = 0; s < kPieces; ++s) {
+    Eight<T, VEC, 32> o;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) o.set2(i, acc[s][i], acc[s][i + 1]);
+    o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0 + 256 * s, lane, p.H);
+  }
 }
 
 struct TokenUnsortGradParams {
@@ -364,14 +380,19 @@ __device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indice
   }
 }
 
-// One block takes `per` pairs of one token, a warp 256 columns at a time: its piece of dout[t]
-// stays in registers while the rows of eight pairs go by, all of them on their way before the first
-// is used.  A pair's product is summed over a lane's columns, the lanes and the warps in that fixed
-// order.
+// One block takes `per` pairs of one token, a warp kPairs of them and 8 / kPairs pieces of 256 columns
+// at a time (VEC): its pieces of dout[t] stay in registers while those of the pairs' rows go by, all
+// eight of them on their way before the first is used.  A pair's product is summed over a lane's
+// columns, the lanes and the warps in that fixed order.
+// Value by value (not VEC) a piece is eight loads instead of one, and two pieces are enough; with eight
+// the loads no longer stood together (4096 tokens x top-4 x 1002 fp32: 106 us instead of 53).
 constexpr int kUnsortGradWarps = 8;
-template <class T, bool VEC>
+__host__ __device__ constexpr int grad_pieces(bool vec, int pairs) { return vec ? 8 / pairs : (pairs == 1 ? 2 : 1); }
+template <class T, bool VEC, int kPairs>
 __global__ void __launch_bounds__(32 * kUnsortGradWarps) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
-  __shared__ float part[kUnsortGradWarps][8];
+  static_assert(VEC || kPairs <= 2, "");
+  constexpr int kPieces = grad_pieces(VEC, kPairs);
+  __shared__ float part[kUnsortGradWarps][kPairs];
   const int warps = blockDim.x >> 5;
   const unsigned splits = (p.top_k + p.per - 1) / p.per;
   const unsigned token_blocks = static_cast<unsigned>(p.T) * splits;
@@ -384,52 +405,60 @@ __global__ void __launch_bounds__(32 * kUnsortGradWarps) token_unsort_grad_kerne
   const int j_begin = static_cast<int>(blockIdx.x - t * splits) * p.per;
   const int j_end = min(j_begin + p.per, p.top_k);
   const T* dout = static_cast<const T*>(p.dout) + (size_t)t * p.dout_stride;
-  for (int j0 = j_begin; j0 < j_end; j0 += 8) {
+  for (int j0 = j_begin; j0 < j_end; j0 += kPairs) {
     int d_lane = -1;
     float w_lane = 1.0f;
-    if (lane < 8 && j0 + lane < j_end) {
+    if (lane < kPairs && j0 + lane < j_end) {
       const size_t i = (size_t)t * p.top_k + j0 + lane;
       d_lane = p.dest[i];
       if (d_lane >= p.rows) d_lane = -1;
       if (p.weights) w_lane = p.weights[i];
     }
-    float dot[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c0 = warp * 256; c0 < p.H; c0 += warps * 256) {
-      Eight<T, VEC, 32> g;
-      g.load(dout, c0, lane, p.H);
-      if (p.dw != nullptr) {
-        Eight<T, VEC, 32> v[8];
+    float dot[kPairs] = {};
+    for (int c0 = warp * 256 * kPieces; c0 < p.H; c0 += warps * 256 * kPieces) {
+      Eight<T, VEC, 32> g[kPieces];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+      for (int s = 0; s < kPieces; ++s) g[s].load(dout, c0 + 256 * s, lane, p.H);
+      if (p.dw != nullptr) {
+        Eight<T, VEC, 32> v[kPairs][kPieces];
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
           const int d = __shfl_sync(0xffffffffu, d_lane, j);
-          v[j].load(static_cast<const T*>(p.y) + (size_t)max(d, 0) * p.y_stride, c0, lane, p.H, d >= 0);
+          const T* row = static_cast<const T*>(p.y) + (size_t)max(d, 0) * p.y_stride;
+#pragma unroll
+          for (int s = 0; s < kPieces; ++s) v[j][s].load(row, c0 + 256 * s, lane, p.H, d >= 0);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // columns behind the row's end and rows of no pair hold zeros
+        for (int j = 0; j < kPairs; ++j)  // columns behind the row's end and rows of no pair hold zeros
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dot[j] = fmaf(g.get(i), v[j].get(i), dot[j]);
+          for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[s].get(i), v[j][s].get(i), dot[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kPairs; ++j) {
         const int d = __shfl_sync(0xffffffffu, d_lane, j);
         const float w = __shfl_sync(0xffffffffu, w_lane, j);
         if (d < 0) continue;
-        Eight<T, VEC, 32> o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o.set(i, w * g.get(i));
-        o.store(static_cast<T*>(p.dy) + (size_t)d * p.H, c0, lane, p.H);
+        for (int s = 0; s < kPieces; ++s) {
+          Eight<T, VEC, 32> o;
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) o.set2(i, w * g[s].get(i), w * g[s].get(i + 1));
+          o.store(static_cast<T*>(p.dy) + (size_t)d * p.H, c0 + 256 * s, lane, p.H);
+        }
       }
     }
     if (p.dw != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kPairs; ++j) {
         const int d = __shfl_sync(0xffffffffu, d_lane, j);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
         if (lane == 0) part[warp][j] = d < 0 ? 0.0f : dot[j];  // (0 * dout is NaN where dout is infinite)
       }
       __syncthreads();
-      if (threadIdx.x < 8 && j0 + static_cast<int>(threadIdx.x) < j_end) {
+      if (threadIdx.x < kPairs && j0 + static_cast<int>(threadIdx.x) < j_end) {
         float s = part[0][threadIdx.x];
         for (int w = 1; w < warps; ++w) s += part[w][threadIdx.x];
         p.dw[(size_t)t * p.top_k + j0 + threadIdx.x] = s;

@@ -34,6 +34,18 @@ void by_type(int elem, bool vec, F f) {
   }
 }
 
+// f(n): n = 1, 2, 4 or 8 pairs of a token that a warp handles at once, beside 8 / n pieces of 256
+// columns: always eight rows' pieces on their way.
+template <int N>
+struct Num { static constexpr int value = N; };
+template <class F>
+void by_pairs(int pairs, F f) {
+  if (pairs <= 1) f(Num<1>{});
+  else if (pairs <= 2) f(Num<2>{});
+  else if (pairs <= 4) f(Num<4>{});
+  else f(Num<8>{});
+}
+
 int launched(int n) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e);
@@ -50,13 +62,10 @@ int blocks_for(long long units, int per_block, const DeviceInfo& dev, int per_sm
 }
 
 // The pairs above which a block does not count all of them itself.
-constexpr long long kSortSelfCount = 65536;
+constexpr long long kSortSelfCount = 16384;
 
-#ifndef SORT_PER_SM
-#define SORT_PER_SM 1
-#endif
 int sort_tokens_per_block(int tokens, int top_k, int sms) {
-  long long per = (tokens + SORT_PER_SM * (long long)sms - 1) / (SORT_PER_SM * (long long)sms);
+  long long per = ((long long)tokens + sms - 1) / sms;
   const long long most = kSortMaxChunk / top_k;
   if (per > most) per = most;
   return static_cast<int>(per < 1 ? 1 : per);
@@ -138,9 +147,10 @@ int dg_token_sort(const dg_token_sort_args* a, void* stream) {
   const unsigned long long all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.rows) |
                                  static_cast<unsigned long long>(p.row_bytes) | static_cast<unsigned long long>(p.x_stride);
   const int vb = (all & 15u) == 0 ? 16 : ((all & 3u) == 0 ? 4 : 2);
-  // few tokens: the columns are split as well, so that more SMs take part
-  const int segs = (p.row_bytes / vb + 127) / 128;
-  int split = chunks < 2 * dev->sm_count ? (2 * dev->sm_count + chunks - 1) / chunks : 1;
+  // few tokens: the columns are split as well, so that more SMs take part (one block on each: a second
+  // round would pay for the counting again)
+  const int segs = (p.row_bytes / vb + sort_seg(vb) - 1) / sort_seg(vb);
+  int split = chunks < dev->sm_count ? dev->sm_count / chunks : 1;
   if (split > segs) split = segs;
   const dim3 grid(chunks, split, 1);
   const int smem = (3 * p.G + 1 + p.tokens_per_block * p.top_k + (p.hist ? 0 : 2 * p.G * p.rep)) * 4;
@@ -177,12 +187,22 @@ int dg_token_unsort(const dg_token_unsort_args* a, void* stream) {
   p.rows = a->num_rows;
   p.y_stride = a->y_stride;
   const bool vec = vec_rows(p.y, p.y_stride, p.H, a->elem) && aligned16(p.out);
-  const long long units = (long long)p.T * ((p.H + 255) / 256);
-  if (units > 0xffffff00LL) return DG_ERR_TOO_LARGE;
-  const unsigned grid = static_cast<unsigned>((units + kUnsortThreads / 32 - 1) / (kUnsortThreads / 32));
+  int rc2 = DG_OK;
   by_type(a->elem, vec, [&](auto t, auto v) {
-    token_unsort_kernel<decltype(t), decltype(v)::value><<<grid, kUnsortThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    by_pairs(p.top_k, [&](auto pairs) {
+      constexpr int kPairs = decltype(pairs)::value;
+      constexpr int kCols = 256 * (8 / kPairs);
+      const long long units = (long long)p.T * ((p.H + kCols - 1) / kCols);  // < 2^31 tokens x pairs, rows < 2^31 values
+      const long long grid = (units + kUnsortThreads / 32 - 1) / (kUnsortThreads / 32);
+      if (grid > 0x1fffffffLL) {
+        rc2 = DG_ERR_TOO_LARGE;
+        return;
+      }
+      token_unsort_kernel<decltype(t), decltype(v)::value, kPairs>
+          <<<static_cast<unsigned>(grid), kUnsortThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    });
   });
+  if (rc2 != DG_OK) return rc2;
   return launched(1);
 }
 
@@ -217,17 +237,22 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
   p.dout_stride = a->dout_stride;
   // few tokens: a block for every pair, so that more SMs take part
   p.per = (long long)p.T >= 4LL * dev->sm_count ? p.top_k : 1;
-  // as many warps as divide the row's 256-column pieces evenly
-  const int pieces = (p.H + 255) / 256, turns = (pieces + kUnsortGradWarps - 1) / kUnsortGradWarps;
-  const int warps = (pieces + turns - 1) / turns;
   p.clear_blocks = a->clear && p.rows > 0 ? blocks_for(p.rows, 16, *dev, 2) : 0;
   const long long grid = (long long)p.T * ((p.top_k + p.per - 1) / p.per) + p.clear_blocks;
   if (grid == 0) return DG_OK;
   const bool vec = vec_rows(p.dout, p.dout_stride, p.H, a->elem) && aligned16(p.dy) &&
                    (!p.dw || vec_rows(p.y, p.y_stride, p.H, a->elem));
   by_type(a->elem, vec, [&](auto t, auto v) {
-    token_unsort_grad_kernel<decltype(t), decltype(v)::value>
-        <<<static_cast<unsigned>(grid), 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    constexpr bool V = decltype(v)::value;
+    by_pairs(p.per, [&](auto pairs) {
+      constexpr int kPairs = V || decltype(pairs)::value <= 2 ? decltype(pairs)::value : 2;
+      constexpr int kCols = 256 * grad_pieces(V, kPairs);
+      // as many warps as divide the row's pieces evenly
+      const int pieces = (p.H + kCols - 1) / kCols;
+      const int turns = (pieces + kUnsortGradWarps - 1) / kUnsortGradWarps, warps = (pieces + turns - 1) / turns;
+      token_unsort_grad_kernel<decltype(t), V, kPairs>
+          <<<static_cast<unsigned>(grid), 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    });
   });
   return launched(1);
 }

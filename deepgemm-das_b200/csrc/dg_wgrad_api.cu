@@ -120,7 +120,7 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   p.dw = a->dw;
   // 256 x 256 tiles move half the operand bytes per product, which pays when a group has rows enough
   // and there are tiles enough; else 128 x 128 ones, whose epilogues are shorter and which reach more
-  // SMs.  Measured, 128 against 256, us: 32 groups of 1024 rows, 4096 x 7168: TILE_A; 256 of 128 rows,
+  // SMs.  Measured, 128 against 256, us: 32 groups of 1024 rows, 4096 x 7168: 2018 / 1469; 256 of 128 rows,
   // 1024 x 1792: 244 / 322; 16 of 64 rows, 4096 x 1024: 41 / 50; 32 of 300 rows, 1024 x 512: 24.5 /
   // 24.2; 4 of 1000 rows, 1024 x 1024 (64 tiles of 256): 17.0 / 14.9; 8 of 2000 rows, 512 x 512 (32
   // tiles): 19.1 / 22.4.
