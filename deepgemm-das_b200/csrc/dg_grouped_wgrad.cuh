@@ -37,6 +37,13 @@
 // which is idle by then) and each block adds its share of the tile's rows over the cluster, in the
 // order of the blocks, so no result depends on timing (1 group of 8000 rows, 512 x 768: 40.6 -> 19.4
 // us; 2 of 4000 rows, 256 x 256: 24.2 -> 12.7).
+// Precision.  The tensor cores' fp32 accumulation rounds towards zero: the sum of R rows comes out
+// smaller by about 0.65e-9 R of itself (measured: relative error 1.0e-6 at 1024 rows, 9.1e-6 at 8192;
+// plain fp32 sums 2.5e-7).  Beside a bf16 result that is nothing.  An fp32 result is made of segments
+// of at most kWgSegment row blocks, each accumulated by itself and added to the ones before it with
+// correct rounding, in order: by the TMA's reduce-add, which waits for the store before it, or, where
+// tiles are split, in registers.  (32 groups of 1024 rows, 4096 x 7168, i.e. two segments each: 2.2 ms
+// instead of 1.6; groups of up to 896 rows are one segment.)
 // Groups without rows give zeros (or, added, nothing) and cost no products.
 //
 // Every mbarrier wait is bounded, as in the other kernels.
@@ -56,6 +63,7 @@ constexpr uint32_t kWgStageBytes = 2 * kWgOperand;
 constexpr uint32_t kWgTailBox = 64 * 2 * 16;       // 64 columns x 16 rows
 constexpr uint32_t kWgTailBytes = 4 * kWgTailBox;  // 128 columns of both operands
 
+constexpr int kWgSegment = 7;       // row blocks: 896 rows, 0.9e-6
 constexpr int kWgIrregular = 255;  // rows that count lie between others: looked up where they are used
 
 enum : int { WG_SITE_EMPTY = 21, WG_SITE_TAIL_EMPTY = 22, WG_SITE_READY = 23, WG_SITE_ACC_EMPTY = 24, WG_SITE_ACC_FULL = 25,
@@ -71,6 +79,7 @@ struct WgradParams {
   int32_t* status;
   int f32;                   // output type: fp32 (else bf16)
   int add;                   // fp32 only: add to what the output holds
+  int segment;               // most row blocks that are accumulated at once
   int split;                 // kSplit: blocks of a cluster
   void* dw;                  // kSplit: the output
   int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
@@ -126,7 +135,8 @@ __device__ __forceinline__ float4 wg_load_cluster(uint32_t cluster_addr) {
   return v;
 }
 
-template <int CL, int S, bool kSplit = false>
+// kSegments: items may be more than one segment (without it, a tenth less time where an item is short).
+template <int CL, int S, bool kSegments, bool kSplit = false>
 __global__ void __launch_bounds__(kWgThreads, 1)
 grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_d, const WgradParams p) {
@@ -291,6 +301,17 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     return it;
   };
 
+  // An item's blocks in segments (a group without rows is one empty segment).
+  auto segments = [&](const Item& w) { return kSegments && w.blocks > p.segment ? (w.blocks + p.segment - 1) / p.segment : 1; };
+  auto segment = [&](const Item& whole, int i, int of) {
+    if (!kSegments || of == 1) return whole;
+    Item w = whole;
+    const int lo = whole.blocks * i / of;
+    w.b0 += lo;
+    w.blocks = whole.blocks * (i + 1) / of - lo;
+    return w;
+  };
+
   // A block whose table entry is n: steps of 16 rows of its first and second 64 rows that come from
   // the ring, and ragged steps behind them (all eight steps of an irregular block).
   auto ring_steps = [&](int n, int half) { return n == kWgIrregular ? 0 : max(0, min(4, n / 16 - 4 * half)); };
@@ -303,7 +324,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       uint32_t it = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
-        const Item w = item_of(item);
+        const Item w = item_of(item);  // (segments follow one another: nothing to do for them here)
         const int n = w.n0 + static_cast<int>(rank) * 128, k = w.k0 + static_cast<int>(rank) * 128;
         for (int i = 0; ok && i < w.blocks; ++i) {
           const int b = blocks[w.b0 + i];
@@ -370,67 +391,74 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       uint32_t it = 0, tile = 0, tail = 0, stages_known = 0, items_known = 0, tails_known = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
-        const Item w = item_of(item);
-        if (w.blocks == 0) continue;
-        const uint32_t buf = tile & 1u;
-        int n_next = valid[blocks[w.b0]];
-        if (items_known <= tile && (items_known = poll_above(items_addr, tile, WG_SITE_ACC_EMPTY)) == 0) break;
-        tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + buf * BT;
-        uint32_t acc = 0;  // the first product of an item overwrites
-        auto step = [&](uint64_t a_desc, uint64_t b_desc) {
-          if constexpr (CL == 2)
-            umma_ss_pair<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
-          else
-            umma_ss<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
-          acc = 1;
-        };
-        auto commit = [&](uint32_t bar) {
-          if constexpr (CL == 2) umma_commit_pair(bar, 3); else umma_commit(bar);
-        };
-        for (int i = 0; ok && i < w.blocks; ++i) {
-          const int n = n_next;
-          if (i + 1 < w.blocks) n_next = valid[blocks[w.b0 + i + 1]];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int steps = ring_steps(n, half);
-            if (steps == 0) break;
-            const int s = it % S;
-            if (stages_known <= it) {
-              if ((stages_known = poll_above(stages_addr, it, WG_SITE_READY)) == 0) {
-                ok = false;
-                break;
-              }
-              tc_fence_after_sync();
-            }
-            ++it;
-            const uint32_t at = base + L::off_stage + s * kWgStageBytes;
-            const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
-            const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
-            if (steps == 4) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) step(a_desc + 128u * k, b_desc + 128u * k);  // 2048 bytes on in every box
-            } else {
-              for (int k = 0; k < steps; ++k) step(a_desc + 128u * k, b_desc + 128u * k);
-            }
-            commit(bar_empty(s));
+        const Item whole = item_of(item);
+        if (whole.blocks == 0) continue;
+        const int segs = segments(whole);
+        for (int sg = 0; ok && sg < segs; ++sg) {
+          const Item w = segment(whole, sg, segs);
+          const uint32_t buf = tile & 1u;
+          int n_next = valid[blocks[w.b0]];
+          if (items_known <= tile && (items_known = poll_above(items_addr, tile, WG_SITE_ACC_EMPTY)) == 0) {
+            ok = false;
+            break;
           }
-          for (int r = ragged_steps(n); ok && r > 0; --r) {
-            if (tails_known <= tail) {
-              if ((tails_known = poll_above(tails_addr, tail, WG_SITE_TAIL_READY)) == 0) {
-                ok = false;
-                break;
+          tc_fence_after_sync();
+          const uint32_t d_tmem = tmem_base + buf * BT;
+          uint32_t acc = 0;  // the first product of a segment overwrites
+          auto step = [&](uint64_t a_desc, uint64_t b_desc) {
+            if constexpr (CL == 2)
+              umma_ss_pair<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
+            else
+              umma_ss<UMMA_F16>(d_tmem, a_desc, b_desc, kIdesc, acc);
+            acc = 1;
+          };
+          auto commit = [&](uint32_t bar) {
+            if constexpr (CL == 2) umma_commit_pair(bar, 3); else umma_commit(bar);
+          };
+          for (int i = 0; ok && i < w.blocks; ++i) {
+            const int n = n_next;
+            if (i + 1 < w.blocks) n_next = valid[blocks[w.b0 + i + 1]];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int steps = ring_steps(n, half);
+              if (steps == 0) break;
+              const int s = it % S;
+              if (stages_known <= it) {
+                if ((stages_known = poll_above(stages_addr, it, WG_SITE_READY)) == 0) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after_sync();
               }
-              tc_fence_after_sync();
+              ++it;
+              const uint32_t at = base + L::off_stage + s * kWgStageBytes;
+              const uint64_t a_desc = umma_desc_mn_sw128(at, kWgBoxBytes);
+              const uint64_t b_desc = umma_desc_mn_sw128(at + kWgOperand, kWgBoxBytes);
+              if (steps == 4) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) step(a_desc + 128u * k, b_desc + 128u * k);  // 2048 bytes on in every box
+              } else {
+                for (int k = 0; k < steps; ++k) step(a_desc + 128u * k, b_desc + 128u * k);
+              }
+              commit(bar_empty(s));
             }
-            ++tail;
-            const uint32_t at = base + L::off_tail;
-            step(umma_desc_mn_sw128(at, kWgTailBox), umma_desc_mn_sw128(at + 2 * kWgTailBox, kWgTailBox));
-            commit(bar_tail_empty);
+            for (int r = ragged_steps(n); ok && r > 0; --r) {
+              if (tails_known <= tail) {
+                if ((tails_known = poll_above(tails_addr, tail, WG_SITE_TAIL_READY)) == 0) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after_sync();
+              }
+              ++tail;
+              const uint32_t at = base + L::off_tail;
+              step(umma_desc_mn_sw128(at, kWgTailBox), umma_desc_mn_sw128(at + 2 * kWgTailBox, kWgTailBox));
+              commit(bar_tail_empty);
+            }
           }
+          if (ok) commit(bar_acc_full(buf));
+          ++tile;
         }
-        if (ok) commit(bar_acc_full(buf));
-        ++tile;
       }
       if (*abort_flag) {
         int local_abort = 0;
@@ -447,27 +475,34 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       uint32_t it = 0, tile = 0, tail = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
-        const Item w = item_of(item);
-        if (w.blocks == 0) continue;
-        if (!mbar_wait_bounded(bar_acc_empty(tile & 1u), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) break;
-        post(items_addr, ++tile);
-        for (int i = 0; ok && i < w.blocks; ++i) {
-          const int n = valid[blocks[w.b0 + i]];
-          for (int half = 0; half < 2; ++half) {
-            if (ring_steps(n, half) == 0) break;
-            if (!mbar_wait_bounded(bar_ready(it % S), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
-              ok = false;
-              break;
-            }
-            post(stages_addr, ++it);
+        const Item whole = item_of(item);
+        if (whole.blocks == 0) continue;
+        const int segs = segments(whole);
+        for (int sg = 0; ok && sg < segs; ++sg) {
+          const Item w = segment(whole, sg, segs);
+          if (!mbar_wait_bounded(bar_acc_empty(tile & 1u), ((tile >> 1) & 1u) ^ 1u, abort_flag, WG_SITE_ACC_EMPTY)) {
+            ok = false;
+            break;
           }
-          for (int r = ragged_steps(n); ok && r > 0; --r) {
-            if (!mbar_wait_bounded(bar_tail_ready, tail & 1u, abort_flag, WG_SITE_TAIL_READY)) {
-              ok = false;
-              break;
+          post(items_addr, ++tile);
+          for (int i = 0; ok && i < w.blocks; ++i) {
+            const int n = valid[blocks[w.b0 + i]];
+            for (int half = 0; half < 2; ++half) {
+              if (ring_steps(n, half) == 0) break;
+              if (!mbar_wait_bounded(bar_ready(it % S), (it / S) & 1u, abort_flag, WG_SITE_READY)) {
+                ok = false;
+                break;
+              }
+              post(stages_addr, ++it);
             }
-            if constexpr (CL == 2) wg_fence_cluster();  // the other block's stores
-            post(tails_addr, ++tail);
+            for (int r = ragged_steps(n); ok && r > 0; --r) {
+              if (!mbar_wait_bounded(bar_tail_ready, tail & 1u, abort_flag, WG_SITE_TAIL_READY)) {
+                ok = false;
+                break;
+              }
+              if constexpr (CL == 2) wg_fence_cluster();  // the other block's stores
+              post(tails_addr, ++tail);
+            }
           }
         }
       }
@@ -533,6 +568,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
                                    CL == 2 ? mapa_shared(bar_acc_empty(1), 0) : bar_acc_empty(1)};
     const int kb_all = p.K / 64;
     uint32_t tile = 0;
+    bool add = p.add != 0;
     // 128 bytes of this lane's row, 16 at a time, where the 128-byte swizzle puts them
     auto put = [&](int piece, uint4 v) {
       *reinterpret_cast<uint4*>(strip_p + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
@@ -545,7 +581,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (p.add) wg_add_3d(&tm_d, strip, x, n, z); else wg_store_3d(&tm_d, strip, x, n, z);
+        if (kSegments ? add : p.add != 0) wg_add_3d(&tm_d, strip, x, n, z); else wg_store_3d(&tm_d, strip, x, n, z);
         wg_store_commit();
       }
     };
@@ -555,26 +591,43 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       const int kb0 = w.k0 / 64;
       const int kbs = n < p.N ? min(BT / 64, kb_all - kb0) : 0;  // 64-column blocks to store
       if constexpr (kSplit) {
-        // this block's partial tile, row r of it at 512 r, 16-byte pieces swizzled with the row
-        const int r = q * 32 + lane;
-        float* row = reinterpret_cast<float*>(smem + L::off_stage + r * 512);
-        if (w.blocks > 0) {
-          if (!mbar_wait_warp(bar_acc_full(0), 0, abort_flag, WG_SITE_ACC_FULL)) break;
-          tc_fence_after_sync();
-        }
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t v[32] = {};
-          if (w.blocks > 0) {
-            tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c, v);
-            tmem_ld_wait();
-          }
+        // this block's partial tile: a lane's row of it in registers over the segments, then in shared
+        // memory, row r at 512 r, 16-byte pieces swizzled with the row
+        float sum[128];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(row + 4 * ((c / 4 + i) ^ (r & 7))) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
+        const int segs = w.blocks > 0 ? segments(w) : 0;
+        bool ok = true;
+        for (int sg = 0; sg < segs; ++sg, ++tile) {
+          const uint32_t buf = tile & 1u;
+          if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[c + i] += __uint_as_float(v[i]);
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty[buf]);
+        }
+        if (ok) {  // every copy and product is done: the ring is free
+          const int r = q * 32 + lane;
+          float* row = reinterpret_cast<float*>(smem + L::off_stage + r * 512);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            *reinterpret_cast<float4*>(row + 4 * (i ^ (r & 7))) = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
         }
         break;  // one tile for a cluster
       }
       if (w.blocks == 0) {
+        add = false;
         if (!p.add && kbs > 0) {
           before();
 #pragma unroll
@@ -584,47 +637,57 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
         }
         continue;
       }
-      const uint32_t buf = tile & 1u;
-      if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) break;
-      tc_fence_after_sync();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT;
-      for (int b = 0; b < kbs; ++b) {
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32(t_row + b * 64, r0);
-        tmem_ld_32x32(t_row + b * 64 + 32, r1);
-        tmem_ld_wait();
-        const int z = w.g * kb_all + kb0 + b;
-        if (p.f32) {
-          before();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) put(i, make_uint4(r0[4 * i], r0[4 * i + 1], r0[4 * i + 2], r0[4 * i + 3]));
-          after(0, n, z);
-          before();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) put(i, make_uint4(r1[4 * i], r1[4 * i + 1], r1[4 * i + 2], r1[4 * i + 3]));
-          after(32, n, z);
-        } else {
-          auto two = [](uint32_t a, uint32_t b2) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b2));
-            return *reinterpret_cast<const uint32_t*>(&h);
-          };
-          before();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            put(i, make_uint4(two(r0[8 * i], r0[8 * i + 1]), two(r0[8 * i + 2], r0[8 * i + 3]),
-                              two(r0[8 * i + 4], r0[8 * i + 5]), two(r0[8 * i + 6], r0[8 * i + 7])));
-            put(4 + i, make_uint4(two(r1[8 * i], r1[8 * i + 1]), two(r1[8 * i + 2], r1[8 * i + 3]),
-                                  two(r1[8 * i + 4], r1[8 * i + 5]), two(r1[8 * i + 6], r1[8 * i + 7])));
-          }
-          after(0, n, z);
+      const int segs = segments(w);
+      bool ok = true;
+      for (int sg = 0; sg < segs; ++sg) {
+        const uint32_t buf = tile & 1u;
+        if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) {
+          ok = false;
+          break;
         }
+        tc_fence_after_sync();
+        if constexpr (kSegments) add = p.add || sg > 0;
+        if (kSegments && sg > 0 && lane == 0) wg_store_wait();  // the segment before is in memory
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT;
+        for (int b = 0; b < kbs; ++b) {
+          uint32_t r0[32], r1[32];
+          tmem_ld_32x32(t_row + b * 64, r0);
+          tmem_ld_32x32(t_row + b * 64 + 32, r1);
+          tmem_ld_wait();
+          const int z = w.g * kb_all + kb0 + b;
+          if (p.f32) {
+            before();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) put(i, make_uint4(r0[4 * i], r0[4 * i + 1], r0[4 * i + 2], r0[4 * i + 3]));
+            after(0, n, z);
+            before();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) put(i, make_uint4(r1[4 * i], r1[4 * i + 1], r1[4 * i + 2], r1[4 * i + 3]));
+            after(32, n, z);
+          } else {
+            auto two = [](uint32_t a, uint32_t b2) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b2));
+              return *reinterpret_cast<const uint32_t*>(&h);
+            };
+            before();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              put(i, make_uint4(two(r0[8 * i], r0[8 * i + 1]), two(r0[8 * i + 2], r0[8 * i + 3]),
+                                two(r0[8 * i + 4], r0[8 * i + 5]), two(r0[8 * i + 6], r0[8 * i + 7])));
+              put(4 + i, make_uint4(two(r1[8 * i], r1[8 * i + 1]), two(r1[8 * i + 2], r1[8 * i + 3]),
+                                    two(r1[8 * i + 4], r1[8 * i + 5]), two(r1[8 * i + 6], r1[8 * i + 7])));
+            }
+            after(0, n, z);
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CL == 2) mbar_arrive_remote(acc_empty[buf]); else mbar_arrive(acc_empty[buf]);
+        }
+        ++tile;
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CL == 2) mbar_arrive_remote(acc_empty[buf]); else mbar_arrive(acc_empty[buf]);
-      }
-      ++tile;
+      if (!ok) break;
     }
     if (lane == 0) wg_store_wait();  // the strip lives until its last store is done
   }

@@ -7,9 +7,12 @@ namespace {
 using namespace dg;
 using namespace dg::host;
 
-template <int CL, int S, bool kSplit = false>
+template <int S>
+struct Stages { static constexpr int value = S; };
+
+template <int CL, int S, bool kSegments, bool kSplit = false>
 int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& dev, cudaStream_t stream) {
-  auto kernel = grouped_wgrad_kernel<CL, S, kSplit>;
+  auto kernel = grouped_wgrad_kernel<CL, S, kSegments, kSplit>;
   const int cluster = kSplit ? p.split : CL;
   constexpr int BT = 128 * CL;
   p.n_tiles = (p.N + BT - 1) / BT;
@@ -118,6 +121,7 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   p.f32 = a->out_kind == DG_OUT_F32;
   p.add = a->accumulate != 0;
   p.dw = a->dw;
+  p.segment = p.f32 ? kWgSegment : DG_MAX_CONTIG_ROWS / 128;
   // 256 x 256 tiles move half the operand bytes per product, which pays when a group has rows enough
   // and there are tiles enough; else 128 x 128 ones, whose epilogues are shorter and which reach more
   // SMs.  Measured, 128 against 256, us: 32 groups of 1024 rows, 4096 x 7168: 2018 / 1469; 256 of 128 rows,
@@ -136,15 +140,17 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   while (rows >= 1536 && split < 8 && items128 * split * 2 <= dev->sm_count && rows >= 128LL * 4 * split * 2) split *= 2;
   if (a->tile == 1) split = 4;  // (asked for)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((a->tile == 0 && tile == 128 && split > 1) || a->tile == 1) {
-    p.split = split;
-    return WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem ? launch_wgrad<1, kWgStages, true>(a, p, *dev, st)
-                                                                         : launch_wgrad<1, kWgStages - 1, true>(a, p, *dev, st);
-  }
+  const bool splits = (a->tile == 0 && tile == 128 && split > 1) || a->tile == 1;
+  p.split = split;
+  auto go = [&](auto stages) {
+    constexpr int S = decltype(stages)::value;
+    if (splits) return launch_wgrad<1, S, true, true>(a, p, *dev, st);
+    if (p.f32) return tile == 256 ? launch_wgrad<2, S, true>(a, p, *dev, st) : launch_wgrad<1, S, true>(a, p, *dev, st);
+    return tile == 256 ? launch_wgrad<2, S, false>(a, p, *dev, st) : launch_wgrad<1, S, false>(a, p, *dev, st);
+  };
   // the table of very many rows takes the room of a ring stage
-  if (WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem)
-    return tile == 256 ? launch_wgrad<2, kWgStages>(a, p, *dev, st) : launch_wgrad<1, kWgStages>(a, p, *dev, st);
-  return tile == 256 ? launch_wgrad<2, kWgStages - 1>(a, p, *dev, st) : launch_wgrad<1, kWgStages - 1>(a, p, *dev, st);
+  if (WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem) return go(Stages<kWgStages>{});
+  return go(Stages<kWgStages - 1>{});
 }
 
 }  // extern "C"
