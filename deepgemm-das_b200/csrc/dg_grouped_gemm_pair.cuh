@@ -59,14 +59,38 @@ struct PairTile {
   int half_mask;   // bit r set: rows of half r may be stored
 };
 
+constexpr int kBTGroup = 8;
 template <bool kBT>
 struct PairDecoder {
   const KernelParams& p;
   const int32_t* tbl;
   int cursor;
-  __device__ PairDecoder(const KernelParams& p_, const int32_t* tbl_) : p(p_), tbl(tbl_), cursor(0) {}
+  int group_units = 0, n_units;  // kBT: up to kBTGroup units of one group from `cursor` on
+  __device__ PairDecoder(const KernelParams& p_, const int32_t* tbl_, int n_items)
+      : p(p_), tbl(tbl_), cursor(0), n_units(kBT ? n_items / p_.n_tiles : 0) {}
   __device__ __forceinline__ PairTile get(int item) {
     PairTile t;
+    if constexpr (kBT) {
+      // Up to eight units of one group at a time, all of them for a column tile before the next one: a
+      // weight tile is then fetched for all of them at about the same time (in the order of the
+      // units, 4 groups of 1024 rows, 4096 -> 7168 read 477 MB from DRAM instead of 281, the weights
+      // twice), and the units' rows stay in L2 over the tiles.
+      while (item >= (cursor + group_units) * p.n_tiles) {  // items only grow
+        cursor += group_units;
+        const int e = tbl[cursor] >> 16;
+        group_units = 1;
+        while (group_units < kBTGroup && cursor + group_units < n_units && (tbl[cursor + group_units] >> 16) == e) ++group_units;
+      }
+      const int local = item - cursor * p.n_tiles;
+      const int nt = local / group_units;
+      const int e = tbl[cursor + local - nt * group_units];
+      t.g = e >> 16;
+      t.half_mask = (e >> 12) & 3;
+      t.row0 = (e & 0xFFF) * 128;  // a unit begins at any block of 128 rows
+      t.n0 = nt * kPairBN;
+      t.rows_valid = min(256, p.M - t.row0);
+      return t;
+    }
     if (p.mode == MODE_MASKED) {
       const int32_t* cnt = tbl;
       const int32_t* pref = tbl + p.G;
@@ -83,7 +107,7 @@ struct PairDecoder {
       const int e = tbl[ui];
       t.g = e >> 16;
       t.half_mask = (e >> 12) & 3;
-      t.row0 = (e & 0xFFF) * (kBT ? 128 : 256);  // kBT: a unit begins at any block of 128 rows
+      t.row0 = (e & 0xFFF) * 256;
       t.n0 = (item - ui * p.n_tiles) * kPairBN;
       t.rows_valid = min(256, p.M - t.row0);
     }
@@ -178,7 +202,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
   } else if (kBT) {
     // Units of two neighbouring 128-row blocks of one group, from the group's first block on: the
     // super blocks of 256 rows need not begin at multiples of 256, so groups padded to 128 rows
-    // leave at most one half unit each (32 uneven groups of 32768 rows, 4096 -> 7168: 1.67 -> 1.60 ms).
+    // leave at most one half unit each (32768 rows in 32 uneven groups, 4096 -> 7168: 1.67 -> 1.60 ms).
     const int blocks = (p.M + 127) / 128;
     for (int b = tid; b < blocks; b += blockDim.x) {
       const int e = p.sched[(size_t)b * 128];
@@ -269,7 +293,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
       // ---- TMA producer (both blocks)
       const uint64_t pol_a = l2_policy_evict_last();
       const uint64_t pol_b = l2_policy_evict_last();  // prefill re-reads weight panels from L2
-      PairDecoder<kBT> dec(p, tbl);
+      PairDecoder<kBT> dec(p, tbl, n_items);
       uint32_t it = 0;
       bool ok = true;
       for (int item = pair; ok && item < n_items; item += num_pairs) {
@@ -402,7 +426,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
     const int row_in_half = q * 32 + lane;
     const uint32_t acc_empty_leader[2] = {mapa_shared(bar_acc_empty(0), 0),
                                           mapa_shared(bar_acc_empty(1), 0)};
-    PairDecoder<kBT> dec(p, tbl);
+    PairDecoder<kBT> dec(p, tbl, n_items);
     uint32_t tile = 0;
     for (int item = pair; item < n_items; item += num_pairs, ++tile) {
       const PairTile t = dec.get(item);
