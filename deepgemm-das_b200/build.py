@@ -89,7 +89,7 @@ def glue_command() -> list[str]:
             "-I", sysconfig.get_paths()["include"], "-I", cuda_inc,
             GLUE_SRC, "-o", GLUE_PATH,
             "-L", LIB_DIR, "-ldeepgemm_b200", "-L", os.path.join(tdir, "lib"),
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
             "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + os.path.join(tdir, "lib")]
 
 

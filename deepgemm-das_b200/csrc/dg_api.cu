@@ -202,6 +202,7 @@ struct Problem {
   const int32_t* offsets;
   int G, M, N, K, block_n, expected_m;
   int narrow;  // filled by validate_and_launch: KernelParams::narrow
+  int clear;     // b_trans: rows with m_indices < 0 are set to zero
   int b_trans;   // 1: dg_grouped_input_grad (contiguous layout, bf16): N = columns of D, K = contraction = rows of a weight block
   int dense;     // 1: dg_dense_gemm (row-major weights, no masked_m, any N, out_kind honoured)
   int out_kind;  // DG_OUT_BF16 / DG_OUT_F16 / DG_OUT_F32
@@ -257,6 +258,7 @@ int launch(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   p.debug_acc = static_cast<uint32_t*>(pr.debug_acc);
   p.status = pr.status;
   p.b_rowmajor = pr.dense;
+  p.clear = pr.clear;
   p.out_kind = pr.out_kind;
   p.signal = pr.signal;
   p.group_window = pr.group_window;
@@ -410,6 +412,7 @@ int launch_pair(const Problem& pr, const DeviceInfo& dev, cudaStream_t stream) {
   p.debug_acc = static_cast<uint32_t*>(pr.debug_acc);
   p.status = pr.status;
   p.b_rowmajor = pr.dense;
+  p.clear = pr.clear;
   p.out_kind = pr.out_kind;
   p.group_window = pr.group_window;
   p.scatter_tag = pr.scatter_tag;
@@ -917,6 +920,7 @@ int dg_grouped_input_grad(const dg_input_grad_args* a, void* stream) {
   pr.scale_mode = DG_SCALE_NONE;
   pr.mode = MODE_CONTIG;
   pr.b_trans = 1;
+  pr.clear = a->clear != 0;
   pr.a = a->dy;
   pr.b = a->w_packed;
   pr.d = a->dx;

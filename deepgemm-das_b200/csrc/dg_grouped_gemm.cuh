@@ -108,6 +108,7 @@ struct KernelParams {
   const void* gather_a;  // the [size_m][K] activation the rows are gathered from
   int block_m, num_blocks, num_sorted, real_topk, size_m;
   int tbl_groups;  // MODE_SORTED: entries per array of the schedule table (the most runs it holds)
+  int clear;   // kBT: the epilogue warps set the rows of D with m_indices < 0 to zero before their first tile
   int narrow;  // masked / compact: 0 = tiles stay BN columns wide, 1 = the kernel may narrow them
                // (down to 32 columns) when few groups have rows, 128 / 64 / 32 = forced width
 };
@@ -492,6 +493,21 @@ struct ItemDecoder {
     return t;
   }
 };
+
+// kBT: rows of D that stand for nothing are set to zero by the epilogue warps (`warps` of them in the
+// grid, this one number `first`) while the first tile's products run; nothing else writes them.
+__device__ __forceinline__ void clear_padding(const KernelParams& p, int first, int warps, int lane) {
+  for (int rb = 0; rb < p.M; rb += 32 * warps) {
+    const int mine = rb + lane * warps + first;
+    unsigned mask = __ballot_sync(0xffffffffu, mine < p.M && p.sched[mine] < 0);
+    while (mask) {
+      const int i = __ffs(mask) - 1;
+      mask &= mask - 1;
+      uint4* row = reinterpret_cast<uint4*>(p.d + static_cast<size_t>(rb + i * warps + first) * p.N);
+      for (int v = lane; v < p.N / 8; v += 32) row[v] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
 
 // kGather: the instantiation behind MODE_SORTED, with four more warps that fetch the rows of a
 // tile by index (the other instantiations carry none of that code).
@@ -929,6 +945,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
   } else if (warp < 6) {
     // ---- epilogue: this warp may touch TMEM lanes [32q, 32q+32)
     const int q = warp & 3;
+    if (kBT && p.clear) clear_padding(p, blockIdx.x * 4 + q, gridDim.x * 4, lane);
     ItemDecoder dec(p, tbl, bn_eff, nt_eff, split_from);
     uint32_t tile = 0;
     for (int item = blockIdx.x; item < n_items; item += gridDim.x, ++tile) {

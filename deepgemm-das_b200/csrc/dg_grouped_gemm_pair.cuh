@@ -426,6 +426,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
     const int row_in_half = q * 32 + lane;
     const uint32_t acc_empty_leader[2] = {mapa_shared(bar_acc_empty(0), 0),
                                           mapa_shared(bar_acc_empty(1), 0)};
+    if (kBT && p.clear) clear_padding(p, blockIdx.x * 4 + q, gridDim.x * 4, lane);
     PairDecoder<kBT> dec(p, tbl, n_items);
     uint32_t tile = 0;
     for (int item = pair; item < n_items; item += num_pairs, ++tile) {

@@ -13,6 +13,7 @@
 //
 // It is not part of the C ABI boundary (include/deepgemm_b200.h has no torch types); it is a
 // client of it, like the ctypes marshalling.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -225,7 +226,7 @@ inline int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) 
 inline bool ints_ok(const Tensor& t, int dev, int64_t n) { return on(t, dev) && t.scalar_type() == at::kInt && t.numel() == n; }
 inline void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 inline Tensor make(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
-  return at::empty(size, at::TensorOptions().dtype(type).device(like.device()));
+  return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);  // at::empty without the dispatcher
 }
 inline py::object count_obj(py::object o) {
   count(!o.is_none());
@@ -448,18 +449,9 @@ py::object input_grad_impl(const Tensor& dy, const Tensor& w, const Tensor& m_in
   a.n = static_cast<int32_t>(n);
   a.k = static_cast<int32_t>(k);
   a.block_n = static_cast<int32_t>(block_n);
+  a.clear = !out.has_value();
   a.status = status;
   if (dg_grouped_input_grad(&a, stream_of(dev)) != DG_OK) return py::none();
-  if (!out.has_value() && a.m_total > 0) {
-    dg_clear_rows_args c{};
-    c.elem = DG_OUT_BF16;
-    c.num_rows = a.m_total;
-    c.hidden = a.k;
-    c.rows = a.dx;
-    c.m_indices = a.m_indices;
-    // (declined after the product was enqueued: the Python path computes the same once more)
-    if (dg_clear_padding_rows(&c, stream_of(dev)) != DG_OK) return py::none();
-  }
   return py::cast(dx);
 }
 

@@ -330,7 +330,7 @@ class InputGradArgs(C.Structure):
         ("n", C.c_int32),
         ("k", C.c_int32),
         ("block_n", C.c_int32),
-        ("reserved", C.c_int32),
+        ("clear", C.c_int32),
         ("status", C.c_void_p),
     ]
 

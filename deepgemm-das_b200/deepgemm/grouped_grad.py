@@ -18,7 +18,6 @@ import torch
 from . import _cabi
 from ._cabi import KIND_BF16
 from ._core import _glue, _launch, device_status_words, packed_weight_dims
-from .token_sort import clear_padding_rows
 
 
 def _bf16_rows(t: torch.Tensor, name: str, what: str) -> torch.Tensor:
@@ -60,11 +59,9 @@ def grouped_bf16_input_grad(dy: torch.Tensor, weight: torch.Tensor, m_indices: t
             raise RuntimeError(f"{what}: out must be {(m, k)} on {dy.device}, got {tuple(out.shape)} on {out.device}")
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device) if out is None else out
     args = _cabi.InputGradArgs(dy=dy.data_ptr(), w_packed=weight.data_ptr(), dx=dx.data_ptr(), m_indices=m_indices.data_ptr(),
-                               num_groups=g, m_total=m, n=n, k=k, block_n=int(block_n),
+                               num_groups=g, m_total=m, n=n, k=k, block_n=int(block_n), clear=int(out is None),
                                status=device_status_words(dy.device).data_ptr())
     _launch(_cabi.lib.dg_grouped_input_grad, args, dy.device, what)
-    if out is None and m:
-        clear_padding_rows(dx, m_indices)
     return dx
 
 
