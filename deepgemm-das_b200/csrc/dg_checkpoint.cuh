@@ -47,8 +47,8 @@ struct CkValues {
     h[1].load(row, c0 + 64, lane, cols, on);
   }
   __device__ __forceinline__ void store(T* row, int c0, int lane, int cols) const {
-    h[0].store(row, c0, lane, cols);
-    h[1].store(row, c0 + 64, lane, cols);
+    h[0].template store<true>(row, c0, lane, cols);
+    h[1].template store<true>(row, c0 + 64, lane, cols);
   }
   __device__ __forceinline__ float get(int i) const { return h[i / 8].get(i % 8); }
   __device__ __forceinline__ void set2(int i, float a, float b) { h[i / 8].set2(i % 8, a, b); }

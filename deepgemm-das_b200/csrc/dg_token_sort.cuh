@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kUnsortThreads) token_unsort_kernel(const Toke
     Eight<T, VEC, 32> o;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) o.set2(i, acc[s][i], acc[s][i + 1]);
-    o.store(static_cast<T*>(p.out) + (size_t)t * p.H, c0 + 256 * s, lane, p.H);
+    o.template store<true>(static_cast<T*>(p.out) + (size_t)t * p.H, c0 + 256 * s, lane, p.H);
   }
 }
 
