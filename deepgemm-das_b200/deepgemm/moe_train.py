@@ -8,7 +8,8 @@ tokens, the packed bf16 expert weights and the routing weights all receive gradi
 
 Between the passes a layer keeps, for every routed row, a byte for each of its hidden values and of
 its gate and up values (``activation_checkpoint``) and the down GEMM's result in bf16; the activation
-itself is computed again from the checkpoint.  CUDA tensors only.
+itself is computed again from the checkpoint.  CUDA tensors only.  A step can be captured into a
+CUDA graph, as long as no eager autograd graph of the same leaves is alive meanwhile.
 """
 from __future__ import annotations
 

@@ -142,7 +142,8 @@ def sort_tokens_grad(drows: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
 
 def unsort_tokens_grad(dout: torch.Tensor, y: torch.Tensor, plan: TokenPlan, weights: Optional[torch.Tensor] = None, *,
                        need_dweights: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Gradients of ``unsort_tokens``: ``dy[dest[t, j]] = weights[t, j] * dout[t]`` (zero in rows that
+    """Gradients of ``unsort_tokens`` (with the whole plan: every row with ``m_indices >= 0`` is named
+    by one pair): ``dy[dest[t, j]] = weights[t, j] * dout[t]`` (zero in rows that
     stand for no pair) and ``dweights[t, j] = <dout[t], y[dest[t, j]]>`` in fp32 (zero for a pair
     without a row; None without weights)."""
     if _glue is not None and (made := _glue.unsort_tokens_grad(dout, y, plan.dest, plan.m_indices, weights, need_dweights)) is not None:

@@ -7,7 +7,9 @@
  * kernels as a plain batched GEMM on unpacked weights (dg_dense_gemm); and the memory-bound
  * steps of an MoE layer around them: quantise + group + pad (dg_quant_group_rows, also for a
  * vLLM-style routing list: dg_group_sorted_rows), SiLU * up + requantise
- * (dg_silu_mul_quant_rows), weighted top-k sum (dg_combine_rows), weight packing.
+ * (dg_silu_mul_quant_rows), weighted top-k sum (dg_combine_rows), weight packing.  For training in
+ * bf16: tokens sorted by expert and back, activation checkpoints in 8 bits, the gradients of the
+ * grouped GEMM.
  *
  * The reference library has no C ABI of its own: its shared object is a PyTorch
  * extension whose C++ entry points take at::Tensor.  Each function below names the

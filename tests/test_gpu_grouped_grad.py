@@ -289,3 +289,23 @@ def test_long_sums_keep_their_precision(tile):
     for _ in range(3):
         assert torch.equal(got, grouped_bf16_weight_grad(dy, x, mi, 3, dtype=torch.float32, tile=tile))
         assert torch.equal(added, grouped_bf16_weight_grad(dy, x, mi, 3, out=start.clone(), accumulate=True, tile=tile))
+
+
+def test_offsets_beyond_32_bits():
+    """Results of more than 2^31 elements: their last group and rows, where 32-bit offsets have wrapped."""
+    gen = torch.Generator().manual_seed(5)
+    g, n, k = 80, 4096, 7168
+    dy, x = whole(gen, 128, n, lim=2).to(DEV), whole(gen, 128, k, lim=2).to(DEV)
+    mi = torch.full((128,), g - 1, dtype=torch.int32, device=DEV)
+    out = grouped_bf16_weight_grad(dy, x, mi, g)
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-1], grouped_bf16_weight_grad(dy, x, torch.zeros_like(mi), 1)[0])
+    assert not bool(out[:-1].any())
+    del out
+    m, n = 2432 * 128, 16
+    dy = whole(gen, m, n, lim=2).to(DEV)
+    w = packed(whole(gen, 2, n, k, lim=2)).to(DEV)
+    mi = (torch.arange(m, device=DEV) >= m // 2).int()
+    dx = grouped_bf16_input_grad(dy, w, mi)
+    assert dx.numel() > 2 ** 31
+    assert torch.equal(dx[-256:], grouped_bf16_input_grad(dy[-256:].contiguous(), w, mi[-256:].contiguous()))
