@@ -726,7 +726,10 @@ int validate_and_launch(Problem& pr, cudaStream_t stream) {
     // rows per group (padding included) decide whether 256-row super blocks are mostly real
     // rows; measured on 32768 routed rows over 256 / 128 / 64 / 32 groups the two-CTA tiles win
     // from about 380 allocated rows per group upwards and lose at 256
-    const bool big_groups = (pr.mode == MODE_CONTIG) ? (rows / pr.G >= 320) : (pr.expected_m >= 256);
+    // Used transposed (units of two blocks from a group's first one on), a group of three blocks is
+    // better off without: 128 groups of 300 rows, 4096 -> 1792, 695 us with and 644 without; of four with:
+    // 64 groups of 400 rows, 2048 -> 2048, 207 and 237.
+    const bool big_groups = (pr.mode == MODE_CONTIG) ? (rows / pr.G >= (pr.b_trans ? 416 : 320)) : (pr.expected_m >= 256);
     const long long pair_items = (rows / 256) * (pr.N / 256);
     if (pr.mode == MODE_COMPACT)
       bn = (pr.N >= 256 && (rows / 128) * (pr.N / 256) >= dev->sm_count) ? 256 : 128;
