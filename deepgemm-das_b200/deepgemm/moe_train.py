@@ -26,7 +26,7 @@ from .token_sort import clear_padding_rows, sort_tokens, unsort_tokens
 
 class _ExpertMlp(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, w13, w2, m_indices, kind):
+    def forward(ctx, rows, w13, w2, m_indices, kind, recorded):
         m = rows.shape[0]
         h = torch.empty((m, w13.shape[2]), dtype=torch.bfloat16, device=rows.device)
         m_grouped_bf16_gemm_nt_contiguous(rows, w13, h, m_indices)
@@ -35,7 +35,7 @@ class _ExpertMlp(torch.autograd.Function):
         y = torch.empty((m, w2.shape[2]), dtype=torch.bfloat16, device=rows.device)
         m_grouped_bf16_gemm_nt_contiguous(act, w2, y, m_indices)
         clear_padding_rows(y, m_indices)
-        entered = checkpoint_rows(rows, kind=kind) if ctx.needs_input_grad[1] else (None, None)
+        entered = checkpoint_rows(rows, kind=kind) if recorded and ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(entered[0], entered[1], kept.q, kept.scale, w13, w2, m_indices)
         return y
 
@@ -45,6 +45,8 @@ class _ExpertMlp(torch.autograd.Function):
         rows_q, rows_scale, q, scale, w13, w2, m_indices = ctx.saved_tensors
         need_rows, need_w13, need_w2 = ctx.needs_input_grad[:3]
         dy = dy.contiguous()
+        if dy.data_ptr() % 16:  # a piece of a larger gradient, begun where the products cannot read it
+            dy = dy.clone()
         drows = dw13 = dw2 = None
         # rows that stand for no pair are neither written here nor read by what follows
         dact = torch.empty((dy.shape[0], w2.shape[1] * 64), dtype=torch.bfloat16, device=dy.device)
@@ -57,7 +59,7 @@ class _ExpertMlp(torch.autograd.Function):
             dw13 = grouped_bf16_weight_grad(dh, restore_rows(Checkpoint(rows_q, rows_scale, torch.bfloat16)), m_indices, w13.shape[0])
         if need_rows:
             drows = grouped_bf16_input_grad(dh, w13, m_indices)
-        return drows, dw13, dw2, None, None
+        return drows, dw13, dw2, None, None, None
 
 
 def expert_mlp_bf16(rows: torch.Tensor, m_indices: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *,
@@ -79,7 +81,7 @@ def expert_mlp_bf16(rows: torch.Tensor, m_indices: torch.Tensor, w13: torch.Tens
         raise ValueError(f"{what}: w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not belong together")
     if checkpoint not in ("fp8", "int8"):
         raise ValueError(f"{what}: checkpoint must be 'fp8' or 'int8', got {checkpoint!r}")
-    return _ExpertMlp.apply(rows, w13, w2, m_indices, checkpoint)
+    return _ExpertMlp.apply(rows, w13, w2, m_indices, checkpoint, torch.is_grad_enabled())
 
 
 def moe_forward_bf16(hidden: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor, w13: torch.Tensor,

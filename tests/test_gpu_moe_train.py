@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import deepgemm
-from deepgemm import expert_mlp_bf16, moe_forward_bf16, sort_tokens, unsort_tokens
+from deepgemm import _cabi, expert_mlp_bf16, moe_forward_bf16, sort_tokens, unsort_tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -194,6 +194,36 @@ def test_a_training_step_captured_into_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(eager, captured):
         assert torch.equal(a, b)
+
+
+def test_a_gradient_that_begins_anywhere():
+    """The layer's result as a piece of a longer vector: its gradient is a contiguous piece of that
+    vector's, six bytes behind a 16-byte boundary."""
+    gen = torch.Generator().manual_seed(5)
+    rows = torch.randn(128, 128, generator=gen).bfloat16().to(DEV)
+    mi = torch.zeros(128, dtype=torch.int32, device=DEV)
+    w13, w2 = (torch.randn(1, 2, 256, 64, generator=gen) / 11).bfloat16().to(DEV), (torch.randn(1, 2, 128, 64, generator=gen) / 11).bfloat16().to(DEV)
+    lead, g = torch.zeros(3, dtype=torch.bfloat16, device=DEV), torch.randn(3 + 128 * 128, generator=gen).bfloat16().to(DEV)
+    leaves = [t.requires_grad_() for t in (rows, w13, w2)]
+    got = torch.autograd.grad(torch.cat([lead, expert_mlp_bf16(leaves[0], mi, *leaves[1:]).flatten()]), leaves, g)
+    want = torch.autograd.grad(expert_mlp_bf16(leaves[0], mi, *leaves[1:]), leaves, g[3:].clone().view(128, 128))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_without_a_gradient_no_rows_are_kept():
+    rows = torch.ones(128, 128, dtype=torch.bfloat16, device=DEV)
+    mi = torch.zeros(128, dtype=torch.int32, device=DEV)
+    w13 = torch.ones(1, 2, 256, 64, dtype=torch.bfloat16, device=DEV).requires_grad_()
+    w2 = torch.ones(1, 2, 128, 64, dtype=torch.bfloat16, device=DEV).requires_grad_()
+
+    def launches(run):
+        before = _cabi.query(_cabi.QUERY_LAUNCH_COUNT)
+        with run:
+            expert_mlp_bf16(rows, mi, w13, w2)
+        return _cabi.query(_cabi.QUERY_LAUNCH_COUNT) - before
+
+    assert launches(torch.enable_grad()) == launches(torch.no_grad()) + 1
 
 
 def test_refusals():
