@@ -305,7 +305,7 @@ __device__ __forceinline__ CkUnit ck_unit(int k, int rows, int blocks) {
 // Rows into a checkpoint.
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) checkpoint_rows_kernel(const CheckpointParams p) {
-  constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkUnits<VEC>;
+  constexpr int kLanes = CkValues<T, VEC>::kLanes, U = kCkUnits<VEC>;
   const int lane = threadIdx.x & (kLanes - 1);
   const int blocks = (p.H + kCkBlock - 1) / kCkBlock;
   CkUnit w[U];

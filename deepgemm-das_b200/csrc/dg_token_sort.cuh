@@ -101,10 +101,12 @@ struct BytesOf<4> { using type = uint32_t; };
 template <>
 struct BytesOf<2> { using type = uint16_t; };
 
-// Plan and copy in one launch.  Every block counts all pairs itself (their ids stay in L2: 32768
-// pairs are 128 KB), so no block waits for another; it then places the pairs of its own tokens and
-// copies their rows, each read once and written top_k times.  blockIdx.y splits the columns of a
-// row when there are few tokens.
+// Plan and copy in one launch.  Every block counts all pairs itself (their ids stay in L2; where they
+// are many, the two kernels above have counted), so no block waits for another; it then places the
+// pairs of its own tokens and copies their rows, each read once and written top_k times.  blockIdx.y
+// splits the columns of a row when there are few tokens.  Nine tenths of the bytes are written, and
+// HBM takes writes at 3.9 TB/s (a plain fill) where it copies at 6.5: 4096 tokens x top-8 x 7168 bf16 in
+// 32 experts padded to 128 rows, 586 MB: 122 us = 4.8 TB/s, 111 us without padding.
 template <int VB>
 __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSortParams p) {
   using V = typename BytesOf<VB>::type;
@@ -179,7 +181,9 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSor
   // where the experts begin: a thread for each (G <= 1024 = kSortThreads)
   {
     static_assert(DG_MAX_GROUPS <= kSortThreads, "");
-    const int v = tid < p.G ? (count[tid] + p.align - 1) / p.align * p.align : 0;
+    // (unsigned: pairs + align - 1 may pass 2^31 where no place does)
+    const unsigned align = p.align;
+    const int v = tid < p.G ? static_cast<int>((static_cast<unsigned>(count[tid]) + align - 1u) / align * align) : 0;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

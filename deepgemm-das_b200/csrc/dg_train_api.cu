@@ -61,7 +61,9 @@ int blocks_for(long long units, int per_block, const DeviceInfo& dev, int per_sm
   return static_cast<int>(want < 1 ? 1 : (want < most ? want : most));
 }
 
-// The pairs above which a block does not count all of them itself.
+// The pairs above which a block does not count all of them itself, but two launches before the sort do
+// (us without and with them, 32 experts x 1024 bf16: 4800 pairs 10.3 / 12.0, 16384 14.5 / 15.4, 32768 21.8 /
+// 21.5, 65536 43.8 / 40.4).
 constexpr long long kSortSelfCount = 16384;
 
 int sort_tokens_per_block(int tokens, int top_k, int sms) {
@@ -235,7 +237,8 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
   p.rows = a->num_rows;
   p.y_stride = a->y_stride;
   p.dout_stride = a->dout_stride;
-  // few tokens: a block for every pair, so that more SMs take part
+  // few tokens: a block for every pair, so that more SMs take part (top-8 x 7168 bf16, us with and without:
+  // 148 tokens 7.5 / 8.0, 296 14.7 / 14.9, 600 34.1 / 32.6, 2400 128 / 108)
   p.per = (long long)p.T >= 4LL * dev->sm_count ? p.top_k : 1;
   p.clear_blocks = a->clear && p.rows > 0 ? blocks_for(p.rows, 16, *dev, 2) : 0;
   const long long grid = (long long)p.T * ((p.top_k + p.per - 1) / p.per) + p.clear_blocks;
