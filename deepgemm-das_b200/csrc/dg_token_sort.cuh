@@ -298,13 +298,27 @@ struct TokenUnsortParams {
   long long y_stride;    // values between rows of y
 };
 
-// out[t] = sum_j w * y[dest]: a warp takes kPairs pairs of one token at once and 8 / kPairs pieces of
-// 256 columns, i.e. always has eight pieces of rows on their way, and adds the pairs in order.  (With
-// one piece whatever top_k is, 16384 tokens x 7168 with top_k = 1 took 170 us; now 83.)
+// out[t] = sum_j w * y[dest]: a warp takes kPairs pairs of one token at once and kPieces pieces of 256
+// columns of their rows, all of them on their way before the first is used, and adds the pairs in
+// order.  What a lane holds (kPairs x kPieces pieces on their way, kPieces sums) is kept to 64
+// registers, so that 32 warps share an SM: with eight pieces whatever type and top_k are, and 128
+// registers or more, 4096 tokens x top-4 x 7168 bf16 took 49.3 us instead of 40.6 (7.2 TB/s), 16384 x top-1
+// 77 instead of 73, in fp32 171 instead of 141, with rows of 2043 bf16 47 instead of 35; only 16384 x
+// top-2 x 4096 was better off, 62 and 64.
 constexpr int kUnsortThreads = 256;
+__host__ __device__ constexpr int unsort_pairs(bool vec, int bytes, int pairs) {  // at most
+  const int most = vec && bytes == 2 ? 8 : 4;
+  return pairs < most ? pairs : most;
+}
+__host__ __device__ constexpr int unsort_pieces(bool vec, int bytes, int pairs) {
+  if (!vec) return pairs == 1 ? 2 : 1;
+  if (bytes == 4) return pairs <= 2 ? 2 : 1;
+  return pairs == 1 ? 4 : (pairs == 8 ? 1 : 2);
+}
 template <class T, bool VEC, int kPairs>
-__global__ void __launch_bounds__(kUnsortThreads) token_unsort_kernel(const TokenUnsortParams p) {
-  constexpr int kPieces = 8 / kPairs;
+__global__ void __launch_bounds__(kUnsortThreads, 4) token_unsort_kernel(const TokenUnsortParams p) {
+  static_assert(unsort_pairs(VEC, sizeof(T), kPairs) == kPairs, "");
+  constexpr int kPieces = unsort_pieces(VEC, sizeof(T), kPairs);
   const int lane = threadIdx.x & 31;
   const unsigned segs = (p.H + 256u * kPieces - 1u) / (256u * kPieces);
   const unsigned u = blockIdx.x * (kUnsortThreads / 32u) + (threadIdx.x >> 5);  // the host keeps units below 2^32
@@ -384,18 +398,28 @@ __device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indice
   }
 }
 
-// One block takes `per` pairs of one token, a warp kPairs of them and 8 / kPairs pieces of 256 columns
-// at a time (VEC): its pieces of dout[t] stay in registers while those of the pairs' rows go by, all
-// eight of them on their way before the first is used.  A pair's product is summed over a lane's
-// columns, the lanes and the warps in that fixed order.
-// Value by value (not VEC) a piece is eight loads instead of one, and two pieces are enough; with eight
-// the loads no longer stood together (4096 tokens x top-4 x 1002 fp32: 106 us instead of 53).
-constexpr int kUnsortGradWarps = 8;
-__host__ __device__ constexpr int grad_pieces(bool vec, int pairs) { return vec ? 8 / pairs : (pairs == 1 ? 2 : 1); }
+// One block takes `per` pairs of one token, a warp kPairs of them and kPieces pieces of 256 columns at
+// a time: its pieces of dout[t] stay in registers while those of the pairs' rows go by, all of them on
+// their way before the first is used.  A pair's product is summed over a lane's columns, the lanes
+// and the warps in that fixed order.
+// Value by value (not VEC) a piece is eight loads instead of one, and one or two pieces are enough.  As
+// above, what a lane holds is kept to 64 registers (VEC; 48 if not): blocks of eight warps with up to 128
+// took 129 us instead of 105 for 16384 tokens x top-1 x 7168 bf16 (6.7 TB/s), 289 instead of 206 for fp32,
+// 425 instead of 337 for 4096 x top-8 x 7168 fp32, 55 instead of 46 for 4096 x top-4 x 1002 fp32.  Streaming
+// stores are 3 to 5 % of that.
+constexpr int kUnsortGradWarps = 4;
+__host__ __device__ constexpr int grad_pairs(bool vec, int bytes, int pairs) {  // at most
+  const int most = !vec ? 2 : (bytes == 4 ? 4 : 8);
+  return pairs < most ? pairs : most;
+}
+__host__ __device__ constexpr int grad_pieces(bool vec, int bytes, int pairs) {
+  return !vec ? (pairs == 1 ? 2 : 1) : (bytes == 4 ? 4 : 8) / pairs;
+}
+__host__ __device__ constexpr int grad_blocks(bool vec) { return vec ? 8 : 10; }  // resident on an SM
 template <class T, bool VEC, int kPairs>
-__global__ void __launch_bounds__(32 * kUnsortGradWarps) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
-  static_assert(VEC || kPairs <= 2, "");
-  constexpr int kPieces = grad_pieces(VEC, kPairs);
+__global__ void __launch_bounds__(32 * kUnsortGradWarps, grad_blocks(VEC)) token_unsort_grad_kernel(const TokenUnsortGradParams p) {
+  static_assert(grad_pairs(VEC, sizeof(T), kPairs) == kPairs, "");
+  constexpr int kPieces = grad_pieces(VEC, sizeof(T), kPairs);
   __shared__ float part[kUnsortGradWarps][kPairs];
   const int warps = blockDim.x >> 5;
   const unsigned splits = (p.top_k + p.per - 1) / p.per;
@@ -449,7 +473,7 @@ __global__ void __launch_bounds__(32 * kUnsortGradWarps) token_unsort_grad_kerne
           Eight<T, VEC, 32> o;
 #pragma unroll
           for (int i = 0; i < 8; i += 2) o.set2(i, w * g[s].get(i), w * g[s].get(i + 1));
-          o.store(static_cast<T*>(p.dy) + (size_t)d * p.H, c0 + 256 * s, lane, p.H);
+          o.template store<true>(static_cast<T*>(p.dy) + (size_t)d * p.H, c0 + 256 * s, lane, p.H);
         }
       }
     }

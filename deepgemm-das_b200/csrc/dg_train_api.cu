@@ -34,8 +34,7 @@ void by_type(int elem, bool vec, F f) {
   }
 }
 
-// f(n): n = 1, 2, 4 or 8 pairs of a token that a warp handles at once, beside 8 / n pieces of 256
-// columns: always eight rows' pieces on their way.
+// f(n): n = 1, 2, 4 or 8 pairs of a token that a warp handles at once.
 template <int N>
 struct Num { static constexpr int value = N; };
 template <class F>
@@ -192,15 +191,17 @@ int dg_token_unsort(const dg_token_unsort_args* a, void* stream) {
   int rc2 = DG_OK;
   by_type(a->elem, vec, [&](auto t, auto v) {
     by_pairs(p.top_k, [&](auto pairs) {
-      constexpr int kPairs = decltype(pairs)::value;
-      constexpr int kCols = 256 * (8 / kPairs);
+      constexpr int kBytes = static_cast<int>(sizeof(decltype(t)));
+      constexpr bool V = decltype(v)::value;
+      constexpr int kPairs = unsort_pairs(V, kBytes, decltype(pairs)::value);
+      constexpr int kCols = 256 * unsort_pieces(V, kBytes, kPairs);
       const long long units = (long long)p.T * ((p.H + kCols - 1) / kCols);  // < 2^31 tokens x pairs, rows < 2^31 values
       const long long grid = (units + kUnsortThreads / 32 - 1) / (kUnsortThreads / 32);
       if (grid > 0x1fffffffLL) {
         rc2 = DG_ERR_TOO_LARGE;
         return;
       }
-      token_unsort_kernel<decltype(t), decltype(v)::value, kPairs>
+      token_unsort_kernel<decltype(t), V, kPairs>
           <<<static_cast<unsigned>(grid), kUnsortThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     });
   });
@@ -248,8 +249,9 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
   by_type(a->elem, vec, [&](auto t, auto v) {
     constexpr bool V = decltype(v)::value;
     by_pairs(p.per, [&](auto pairs) {
-      constexpr int kPairs = V || decltype(pairs)::value <= 2 ? decltype(pairs)::value : 2;
-      constexpr int kCols = 256 * grad_pieces(V, kPairs);
+      constexpr int kBytes = static_cast<int>(sizeof(decltype(t)));
+      constexpr int kPairs = grad_pairs(V, kBytes, decltype(pairs)::value);
+      constexpr int kCols = 256 * grad_pieces(V, kBytes, kPairs);
       // as many warps as divide the row's pieces evenly
       const int pieces = (p.H + kCols - 1) / kCols;
       const int turns = (pieces + kUnsortGradWarps - 1) / kUnsortGradWarps, warps = (pieces + turns - 1) / turns;
