@@ -228,6 +228,13 @@ inline void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).st
 inline Tensor make(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);  // at::empty without the dispatcher
 }
+// `size` values of an int32 buffer from `first` on, as a tensor of its own (no dispatcher, no allocation)
+inline Tensor part(const Tensor& whole, int64_t first, at::IntArrayRef size) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + first);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+  return t;
+}
 inline py::object count_obj(py::object o) {
   count(!o.is_none());
   return o;
@@ -245,8 +252,12 @@ py::object sort_impl(const Tensor& x, const Tensor& ids, int64_t experts, int64_
   if (out.has_value() && (!on(*out, dev) || out->scalar_type() != x.scalar_type() || out->dim() != 2 || out->size(0) != cap || out->size(1) != h))
     return py::none();
   Tensor rows = out.has_value() ? *out : make({cap, h}, x.scalar_type(), x);
-  Tensor dest = make({t, k}, at::kInt, x), m_indices = make({cap}, at::kInt, x), counts = make({experts}, at::kInt, x),
-         offsets = make({experts}, at::kInt, x), m_total = make({1}, at::kInt, x), scratch;
+  // the plan's five arrays in one buffer, each on a 16-byte boundary
+  const int64_t at_m = (t * k + 3) / 4 * 4, at_c = at_m + (cap + 3) / 4 * 4, at_o = at_c + (experts + 3) / 4 * 4,
+                at_t = at_o + (experts + 3) / 4 * 4;
+  Tensor ints = make({at_t + 1}, at::kInt, x), scratch;
+  Tensor dest = part(ints, 0, {t, k}), m_indices = part(ints, at_m, {cap}), counts = part(ints, at_c, {experts}),
+         offsets = part(ints, at_o, {experts}), m_total = part(ints, at_t, {1});
   dg_token_sort_args a{};
   a.elem_bytes = static_cast<int32_t>(x.element_size());
   a.ids64 = ids.scalar_type() == at::kLong;
