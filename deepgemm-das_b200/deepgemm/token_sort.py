@@ -90,8 +90,10 @@ def _sort(x, topk_ids, num_experts, align, out):
     ids = topk_ids if topk_ids.is_contiguous() else topk_ids.contiguous()
     dev = x.device
     rows = torch.empty((cap, h), dtype=x.dtype, device=dev) if out is None else _out_arg(out, x, (cap, h), what)
-    ints = torch.empty(t * k + cap + 2 * num_experts + 1, dtype=torch.int32, device=dev)
-    dest, m_indices, counts, offsets, m_total = ints.split([t * k, cap, num_experts, num_experts, 1])
+    sizes = [t * k, cap, num_experts, num_experts, 1]  # in one buffer, each on a 16-byte boundary
+    rooms = [(n + 3) // 4 * 4 for n in sizes]
+    parts = torch.empty(sum(rooms), dtype=torch.int32, device=dev).split(rooms)
+    dest, m_indices, counts, offsets, m_total = (part[:n] for part, n in zip(parts, sizes))
     need = int(_cabi.lib.dg_token_sort_scratch_bytes(t, k, num_experts))
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     args = _cabi.TokenSortArgs(

@@ -226,6 +226,25 @@ def test_without_a_gradient_no_rows_are_kept():
     assert launches(torch.enable_grad()) == launches(torch.no_grad()) + 1
 
 
+def test_in_inference_mode_and_with_a_plan_copied():
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(70, 128, generator=gen).bfloat16().to(DEV)
+    ids = torch.randint(-1, 4, (70, 2), generator=gen).to(DEV)
+    w = torch.rand(70, 2, generator=gen).to(DEV)
+    w13, w2 = (torch.randn(4, 2, 256, 64, generator=gen) / 11).bfloat16().to(DEV), (torch.randn(4, 2, 128, 64, generator=gen) / 11).bfloat16().to(DEV)
+    want = moe_forward_bf16(x, ids, w, w13, w2)
+    with torch.inference_mode():
+        assert torch.equal(moe_forward_bf16(x, ids, w, w13, w2), want)
+    rows, plan = sort_tokens(x, ids, 4)
+    copied = type(plan)(*[t.clone() for t in plan])
+    for a, b in zip(plan, copied):
+        assert a.is_contiguous() and a.data_ptr() % 16 == 0
+    plan.counts.zero_()  # the plan's arrays are apart
+    plan.offsets.fill_(-5)
+    assert torch.equal(plan.dest, copied.dest) and torch.equal(plan.m_indices, copied.m_indices) and torch.equal(plan.m_total, copied.m_total)
+    assert torch.equal(unsort_tokens(rows, plan, w), unsort_tokens(rows, copied, w))
+
+
 def test_refusals():
     x = torch.zeros(128, 128, dtype=torch.bfloat16, device=DEV)
     mi = torch.zeros(128, dtype=torch.int32, device=DEV)
