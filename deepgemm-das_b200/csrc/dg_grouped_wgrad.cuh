@@ -16,7 +16,7 @@
 // blocks of the group in ascending order, 64 rows (a chunk) at a time.
 //   warp 0      TMA producer (each block its own copies)
 //   warp 1      UMMA issuer (leader)
-//   warps 2..5  epilogue: accumulator -> bf16 or fp32 -> 32-row strip in shared memory -> TMA store
+//   warps 2..5  epilogue (fp32: 8..11 too): accumulator -> bf16 or fp32 -> 32-row strip in shared memory -> TMA store
 //               (or TMA reduce-add, when the gradient is added to what is there)
 //   warp 6      ragged steps.  The products run in steps of 16 rows.  Rows that stand for nothing
 //               (padding, rows behind the last group) must not reach a sum, whatever they hold (NaN,
@@ -41,9 +41,12 @@
 // smaller by about 0.65e-9 R of itself (measured: relative error 1.0e-6 at 1024 rows, 9.1e-6 at 8192;
 // plain fp32 sums 2.5e-7).  Beside a bf16 result that is nothing.  An fp32 result is made of segments
 // of at most kWgSegment row blocks, each accumulated by itself and added to the ones before it with
-// correct rounding, in order: by the TMA's reduce-add, which waits for the store before it, or, where
-// tiles are split, in registers.  (32 groups of 1024 rows, 4096 x 7168, i.e. two segments each: 2.2 ms
-// instead of 1.6; groups of up to 896 rows are one segment.)
+// correct rounding, in order, in the epilogue's registers: eight epilogue warps (kWide), each with
+// half of a tile's columns, hold a lane's 128 sums.  32 groups of 1024 rows, 4096 x 7168, i.e. two segments
+// each, fp32: 1.78 ms, added to what is there 2.29; with four warps and the segments added in memory by the
+// TMA's reduce-add 2.2 and 2.7; 8 groups of 4096 rows 1.71 instead of 2.07.  Groups of one segment are on
+// average where they were (768 rows 1.58 and 1.60 ms, 896 rows 1.72 and 1.51, 512 rows, 4096 x 4096, 361 and
+// 404 us); bf16 results (1.44 ms) need no segments and keep four warps and the sixth ring stage.
 // Groups without rows give zeros (or, added, nothing) and cost no products.
 //
 // Every mbarrier wait is bounded, as in the other kernels.
@@ -57,6 +60,7 @@ namespace dg {
 
 constexpr int kWgStages = 6;                       // five where the table below needs the room
 constexpr int kWgThreads = 256;
+constexpr int kWgWideThreads = 384;                // kWide: warps 8..11 are a second set of epilogue warps
 constexpr uint32_t kWgBoxBytes = 64 * 128;         // 64 columns x 64 rows
 constexpr uint32_t kWgOperand = 2 * kWgBoxBytes;   // 128 columns x 64 rows
 constexpr uint32_t kWgStageBytes = 2 * kWgOperand;
@@ -85,14 +89,15 @@ struct WgradParams {
   int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
 };
 
-template <int S>
+// EPI: epilogue warps, 4 KB each.
+template <int S, int EPI>
 struct WgradSmem {
   static constexpr int off_stage = 0;
   static constexpr int off_tail = off_stage + S * kWgStageBytes;
-  static constexpr int off_strip = off_tail + kWgTailBytes;  // 4 KB for each epilogue warp
+  static constexpr int off_strip = off_tail + kWgTailBytes;
   // ready[S], empty[S], tail_ready, tail_empty, acc_full[2], acc_empty[2], drain
   static constexpr int kNumBars = 2 * S + 7;
-  static constexpr int off_bar = off_strip + 4 * 4096;
+  static constexpr int off_bar = off_strip + EPI * 4096;
   static constexpr int off_misc = off_bar + kNumBars * 8;  // tmem slot, abort, stages ready, items ready, tails ready
   static constexpr int off_table = off_misc + 24;
   // table: first[G + 1] (int32), the groups' 128-row blocks in order (uint16), rows that count (uint8)
@@ -103,7 +108,8 @@ struct WgradSmem {
   static_assert(S * static_cast<int>(kWgStageBytes) >= DG_MAX_CONTIG_ROWS / 128 * 2, "");
   static_assert(off_table % 4 == 0 && off_strip % 1024 == 0 && off_tail % 1024 == 0, "");
 };
-static_assert(WgradSmem<kWgStages - 1>::total(DG_MAX_GROUPS, DG_MAX_CONTIG_ROWS / 128) <= 232448, "");
+static_assert(WgradSmem<kWgStages - 1, 4>::total(DG_MAX_GROUPS, DG_MAX_CONTIG_ROWS / 128) <= 232448, "");
+static_assert(WgradSmem<kWgStages - 2, 8>::total(DG_MAX_GROUPS, DG_MAX_CONTIG_ROWS / 128) <= 232448, "");
 
 // An arrival on another block's mbarrier that orders nothing (the copies it announces are ordered by
 // the barrier's byte count).
@@ -135,12 +141,19 @@ __device__ __forceinline__ float4 wg_load_cluster(uint32_t cluster_addr) {
   return v;
 }
 
-// kSegments: items may be more than one segment (without it, a tenth less time where an item is short).
+// kSegments: items may be more than one segment.
+// Such items without kSplit take eight epilogue warps (kWide).
+__host__ __device__ constexpr bool wg_wide(bool segments, bool split) { return segments && !split; }
+__host__ __device__ constexpr int wg_threads(bool segments, bool split) {
+  return wg_wide(segments, split) ? kWgWideThreads : kWgThreads;
+}
 template <int CL, int S, bool kSegments, bool kSplit = false>
-__global__ void __launch_bounds__(kWgThreads, 1)
+__global__ void __launch_bounds__(wg_threads(kSegments, kSplit), 1)
 grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_d, const WgradParams p) {
-  using L = WgradSmem<S>;
+  constexpr bool kWide = wg_wide(kSegments, kSplit);
+  constexpr int kThreads = wg_threads(kSegments, kSplit), kEpi = kWide ? 8 : 4;
+  using L = WgradSmem<S, kEpi>;
   constexpr int BT = 128 * CL;  // tile edge
   constexpr uint32_t kIdesc = umma_idesc(1u, 1u, BT, BT) | kIdescAMn | kIdescBMn;
   constexpr int kTmemCols = 2 * BT;
@@ -185,7 +198,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
     mbar_init(bar_tail_empty, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_acc_full(b), 1);
-      mbar_init(bar_acc_empty(b), 4 * CL);
+      mbar_init(bar_acc_empty(b), kEpi * CL);
     }
     mbar_init(bar_drain, 1);
     fence_mbar_init();
@@ -197,11 +210,11 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   // Table: the 128-row blocks of every group in ascending order (counting sort, stable).
   {
     int16_t* of_block = reinterpret_cast<int16_t*>(smem + L::off_stage);
-    for (int g = tid; g <= p.G; g += kWgThreads) first[g] = 0;
+    for (int g = tid; g <= p.G; g += kThreads) first[g] = 0;
     __syncthreads();
     bool bad = false;
 #pragma unroll 4
-    for (int b = warp; b < p.m_blocks; b += kWgThreads / 32) {
+    for (int b = warp; b < p.m_blocks; b += kThreads / 32) {
       int m[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -560,15 +573,16 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       }
     }
   } else {
-    // ---- epilogue: rows n0 + 128 rank + 32 q .. + 31 of the tile
-    const int q = warp & 3;
-    const uint32_t strip = base + L::off_strip + q * 4096;
-    uint8_t* strip_p = smem + L::off_strip + q * 4096;
+    // ---- epilogue: rows n0 + 128 rank + 32 q .. + 31 of the tile; kWide: warps 2..5 the first half of its
+    // columns, 8..11 the second
+    constexpr int kCols = kWide ? BT / 2 : BT;
+    const int q = warp & 3, half = kWide ? warp >> 3 : 0;
+    const uint32_t strip = base + L::off_strip + (half * 4 + q) * 4096;
+    uint8_t* strip_p = smem + L::off_strip + (half * 4 + q) * 4096;
     const uint32_t acc_empty[2] = {CL == 2 ? mapa_shared(bar_acc_empty(0), 0) : bar_acc_empty(0),
                                    CL == 2 ? mapa_shared(bar_acc_empty(1), 0) : bar_acc_empty(1)};
     const int kb_all = p.K / 64;
     uint32_t tile = 0;
-    bool add = p.add != 0;
     // 128 bytes of this lane's row, 16 at a time, where the 128-byte swizzle puts them
     auto put = [&](int piece, uint4 v) {
       *reinterpret_cast<uint4*>(strip_p + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
@@ -581,15 +595,22 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (kSegments ? add : p.add != 0) wg_add_3d(&tm_d, strip, x, n, z); else wg_store_3d(&tm_d, strip, x, n, z);
+        if (p.add) wg_add_3d(&tm_d, strip, x, n, z); else wg_store_3d(&tm_d, strip, x, n, z);
         wg_store_commit();
+      }
+    };
+    auto release = [&](uint32_t buf) {  // the accumulator's columns are in registers
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CL == 2) mbar_arrive_remote(acc_empty[buf]); else mbar_arrive(acc_empty[buf]);
       }
     };
     for (int item = unit; item < n_items; item += units) {
       const Item w = item_of(item);
       const int n = w.n0 + static_cast<int>(rank) * 128 + q * 32;
-      const int kb0 = w.k0 / 64;
-      const int kbs = n < p.N ? min(BT / 64, kb_all - kb0) : 0;  // 64-column blocks to store
+      const int kb0 = w.k0 / 64 + half * (kCols / 64);
+      const int kbs = n < p.N ? max(0, min(kCols / 64, kb_all - kb0)) : 0;  // 64-column blocks to store
       if constexpr (kSplit) {
         // this block's partial tile: a lane's row of it in registers over the segments, then in shared
         // memory, row r at 512 r, 16-byte pieces swizzled with the row
@@ -627,7 +648,6 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
         break;  // one tile for a cluster
       }
       if (w.blocks == 0) {
-        add = false;
         if (!p.add && kbs > 0) {
           before();
 #pragma unroll
@@ -637,57 +657,67 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
         }
         continue;
       }
-      const int segs = segments(w);
-      bool ok = true;
-      for (int sg = 0; sg < segs; ++sg) {
-        const uint32_t buf = tile & 1u;
-        if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) {
-          ok = false;
-          break;
+      if constexpr (kWide) {
+        // this lane's row of the half tile, summed over the segments in registers
+        float sum[kCols];
+        const int segs = segments(w);
+        bool ok = true;
+        for (int sg = 0; sg < segs; ++sg, ++tile) {
+          const uint32_t buf = tile & 1u;
+          if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT + half * kCols;
+#pragma unroll
+          for (int c = 0; c < kCols; c += 16) {
+            uint32_t v[16];
+            tmem_ld_32x16(t_row + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c + i] = sg == 0 ? __uint_as_float(v[i]) : sum[c + i] + __uint_as_float(v[i]);
+          }
+          release(buf);
         }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          if (c / 64 >= kbs) continue;
+          before();
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            put(i, make_uint4(__float_as_uint(sum[c + 4 * i]), __float_as_uint(sum[c + 4 * i + 1]), __float_as_uint(sum[c + 4 * i + 2]),
+                              __float_as_uint(sum[c + 4 * i + 3])));
+          after(c % 64, n, w.g * kb_all + kb0 + c / 64);
+        }
+      } else if constexpr (!kSplit) {
+        const uint32_t buf = tile & 1u;
+        if (!mbar_wait_warp(bar_acc_full(buf), (tile >> 1) & 1u, abort_flag, WG_SITE_ACC_FULL)) break;
         tc_fence_after_sync();
-        if constexpr (kSegments) add = p.add || sg > 0;
-        if (kSegments && sg > 0 && lane == 0) wg_store_wait();  // the segment before is in memory
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT;
         for (int b = 0; b < kbs; ++b) {
           uint32_t r0[32], r1[32];
           tmem_ld_32x32(t_row + b * 64, r0);
           tmem_ld_32x32(t_row + b * 64 + 32, r1);
           tmem_ld_wait();
-          const int z = w.g * kb_all + kb0 + b;
-          if (p.f32) {
-            before();
+          auto two = [](uint32_t a, uint32_t b2) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b2));
+            return *reinterpret_cast<const uint32_t*>(&h);
+          };
+          before();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) put(i, make_uint4(r0[4 * i], r0[4 * i + 1], r0[4 * i + 2], r0[4 * i + 3]));
-            after(0, n, z);
-            before();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) put(i, make_uint4(r1[4 * i], r1[4 * i + 1], r1[4 * i + 2], r1[4 * i + 3]));
-            after(32, n, z);
-          } else {
-            auto two = [](uint32_t a, uint32_t b2) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b2));
-              return *reinterpret_cast<const uint32_t*>(&h);
-            };
-            before();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              put(i, make_uint4(two(r0[8 * i], r0[8 * i + 1]), two(r0[8 * i + 2], r0[8 * i + 3]),
-                                two(r0[8 * i + 4], r0[8 * i + 5]), two(r0[8 * i + 6], r0[8 * i + 7])));
-              put(4 + i, make_uint4(two(r1[8 * i], r1[8 * i + 1]), two(r1[8 * i + 2], r1[8 * i + 3]),
-                                    two(r1[8 * i + 4], r1[8 * i + 5]), two(r1[8 * i + 6], r1[8 * i + 7])));
-            }
-            after(0, n, z);
+          for (int i = 0; i < 4; ++i) {
+            put(i, make_uint4(two(r0[8 * i], r0[8 * i + 1]), two(r0[8 * i + 2], r0[8 * i + 3]),
+                              two(r0[8 * i + 4], r0[8 * i + 5]), two(r0[8 * i + 6], r0[8 * i + 7])));
+            put(4 + i, make_uint4(two(r1[8 * i], r1[8 * i + 1]), two(r1[8 * i + 2], r1[8 * i + 3]),
+                                  two(r1[8 * i + 4], r1[8 * i + 5]), two(r1[8 * i + 6], r1[8 * i + 7])));
           }
+          after(0, n, w.g * kb_all + kb0 + b);
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CL == 2) mbar_arrive_remote(acc_empty[buf]); else mbar_arrive(acc_empty[buf]);
-        }
+        release(buf);
         ++tile;
       }
-      if (!ok) break;
     }
     if (lane == 0) wg_store_wait();  // the strip lives until its last store is done
   }
@@ -700,7 +730,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       const Item w = item_of(unit);
       const int rows = 128 / p.split, r0 = part * rows;
       const int kb_all = p.K / 64;
-      for (int i = tid; i < rows * 32; i += kWgThreads) {
+      for (int i = tid; i < rows * 32; i += kThreads) {
         const int r = r0 + (i >> 5), piece = i & 31;
         const int n = w.n0 + r, k = w.k0 + 4 * piece;
         if (n >= p.N || k >= p.K) continue;

@@ -19,7 +19,7 @@ int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& 
   p.k_tiles = (p.K + BT - 1) / BT;
   const long long items = (long long)p.G * p.n_tiles * p.k_tiles;
   if (items > 0x7fffffffLL) return DG_ERR_TOO_LARGE;
-  const int smem = WgradSmem<S>::total(p.G, p.m_blocks);
+  const int smem = WgradSmem<S, wg_wide(kSegments, kSplit) ? 8 : 4>::total(p.G, p.m_blocks);
   if (smem > dev.max_smem) return DG_ERR_TOO_LARGE;
 
   CUtensorMap tm_dy, tm_x, tm_d;
@@ -52,7 +52,7 @@ int launch_wgrad(const dg_weight_grad_args* a, WgradParams p, const DeviceInfo& 
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kWgThreads, 1, 1);
+  cfg.blockDim = dim3(wg_threads(kSegments, kSplit), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -145,11 +145,12 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   auto go = [&](auto stages) {
     constexpr int S = decltype(stages)::value;
     if (splits) return launch_wgrad<1, S, true, true>(a, p, *dev, st);
-    if (p.f32) return tile == 256 ? launch_wgrad<2, S, true>(a, p, *dev, st) : launch_wgrad<1, S, true>(a, p, *dev, st);
+    // (a stage's room for the strips of four more epilogue warps)
+    if (p.f32) return tile == 256 ? launch_wgrad<2, S - 1, true>(a, p, *dev, st) : launch_wgrad<1, S - 1, true>(a, p, *dev, st);
     return tile == 256 ? launch_wgrad<2, S, false>(a, p, *dev, st) : launch_wgrad<1, S, false>(a, p, *dev, st);
   };
   // the table of very many rows takes the room of a ring stage
-  if (WgradSmem<kWgStages>::total(p.G, p.m_blocks) <= dev->max_smem) return go(Stages<kWgStages>{});
+  if (WgradSmem<kWgStages, 4>::total(p.G, p.m_blocks) <= dev->max_smem) return go(Stages<kWgStages>{});
   return go(Stages<kWgStages - 1>{});
 }
 
