@@ -344,33 +344,14 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
       // long ago costs this thread about 200 cycles, comparable with the four UMMAs of a
       // stage: the watcher warp does the waits and posts "stages ready" / "items ready" in
       // plain shared-memory words, which this thread re-reads only when its copy is used up.
-      // Ordering: the watcher observes the mbarrier (acquire), then publishes with st.release;
-      // this thread's volatile loads of one shared-memory word after another are performed in
-      // program order, and tcgen05.fence::after_thread_sync orders the UMMAs after the load
-      // that saw the new count.  The operands themselves are read by the tensor core only.
-      auto poll_above = [&](uint32_t addr, uint32_t have, int site) -> uint32_t {
-        uint32_t v;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-        }
-        const uint64_t t0 = global_timer_ns();
-        uint32_t spins = 0;
-        while (true) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-          if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
-            if (!*abort_flag) *abort_flag = site;
-            return 0;
-          }
-        }
-      };
+      // Ordering: the watcher observes the mbarrier (acquire), then publishes with a release that
+      // this thread's reads acquire, and tcgen05.fence::after_thread_sync orders the UMMAs after
+      // the load that saw the new count.  The operands themselves are read by the tensor core only.
       uint32_t it = 0, tile = 0, stages_known = 0, items_known = 0;
       bool ok = true;
       for (int item = pair; ok && item < n_items; item += num_pairs, ++tile) {
         const uint32_t buf = tile & 1u;
-        if (items_known <= tile && (items_known = poll_above(items_addr, tile, SITE_MMA_ACC_EMPTY)) == 0) {
+        if (items_known <= tile && (items_known = poll_above(items_addr, tile, abort_flag, SITE_MMA_ACC_EMPTY)) == 0) {
           ok = false;
           break;
         }
@@ -379,7 +360,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
         for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (stages_known <= it) {
-            if ((stages_known = poll_above(stages_addr, it, SITE_MMA_FULL)) == 0) {
+            if ((stages_known = poll_above(stages_addr, it, abort_flag, SITE_MMA_FULL)) == 0) {
               ok = false;
               break;
             }
@@ -412,14 +393,14 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
         if (!mbar_wait_bounded(bar_acc_empty(tile & 1u), ((tile >> 1) & 1u) ^ 1u, abort_flag,
                                SITE_MMA_ACC_EMPTY))
           break;
-        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(items_addr), "r"(tile + 1u) : "memory");
+        post_count(items_addr, tile + 1u);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (!mbar_wait_bounded(bar_full(it % STAGES), (it / STAGES) & 1u, abort_flag, SITE_MMA_FULL)) {
             ok = false;
             break;
           }
           ++it;
-          asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(stages_addr), "r"(it) : "memory");
+          post_count(stages_addr, it);
         }
       }
     }

@@ -282,14 +282,14 @@ grouped_gemm_w4_kernel(const __grid_constant__ CUtensorMap tm_tok,
                                SITE_MMA_ACC_EMPTY))
           break;
         idesc_ring[tile & 7u] = kIdescBase | ((n_tok >> 3) << 17);
-        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(items_addr), "r"(tile + 1u) : "memory");
+        post_count(items_addr, tile + 1u);
         for (int wb = 0; wb < wblocks; ++wb) {
           if (!mbar_wait_bounded(bar_rfull(it % RS), (it / RS) & 1u, abort_flag, SITE_MMA_FULL)) {
             ok = false;
             break;
           }
           ++it;
-          asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(ready_addr), "r"(it) : "memory");
+          post_count(ready_addr, it);
         }
       }
     }
@@ -300,34 +300,13 @@ grouped_gemm_w4_kernel(const __grid_constant__ CUtensorMap tm_tok,
       // nor touches an mbarrier: the watcher warp posts, in plain shared-memory words, how
       // many items (descriptor ready, accumulator free) and rounds (weights and tokens in
       // place) may be issued, and this thread re-reads a word only when its last copy is used up.
-      // Ordering: the watcher observes the mbarrier (acquire), then publishes with st.release;
-      // this thread's volatile loads of one shared-memory word after another are performed in
-      // program order, and tcgen05.fence::after_thread_sync orders the UMMAs after the load
-      // that saw the new count.  The operands themselves are read by the tensor core only.
-      auto poll_above = [&](uint32_t addr, uint32_t have, int site) -> uint32_t {
-        // returns a value > have, or 0 after giving up (abort flag set); the timer is only read
-        // once the word has been found unchanged a few times (reading it costs ~100 cycles)
-        uint32_t v;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-        }
-        const uint64_t t0 = global_timer_ns();
-        uint32_t spins = 0;
-        while (true) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-          if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
-            if (!*abort_flag) *abort_flag = site;
-            return 0;
-          }
-        }
-      };
+      // Ordering: the watcher observes the mbarrier (acquire), then publishes with a release that
+      // this thread's reads acquire, and tcgen05.fence::after_thread_sync orders the UMMAs after
+      // the load that saw the new count.  The operands themselves are read by the tensor core only.
       uint32_t it = 0, tile = 0, rounds_known = 0, items_known = 0;
       bool ok = true;
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x, ++tile) {
-        if (items_known <= tile && (items_known = poll_above(items_addr, tile, SITE_MMA_ACC_EMPTY)) == 0) {
+        if (items_known <= tile && (items_known = poll_above(items_addr, tile, abort_flag, SITE_MMA_ACC_EMPTY)) == 0) {
           ok = false;
           break;
         }
@@ -338,7 +317,7 @@ grouped_gemm_w4_kernel(const __grid_constant__ CUtensorMap tm_tok,
         for (int wb = 0; wb < wblocks; ++wb, ++it) {
           const int s = it % RS;
           if (rounds_known <= it) {
-            if ((rounds_known = poll_above(ready_addr, it, SITE_MMA_FULL)) == 0) {
+            if ((rounds_known = poll_above(ready_addr, it, abort_flag, SITE_MMA_FULL)) == 0) {
               ok = false;
               break;
             }

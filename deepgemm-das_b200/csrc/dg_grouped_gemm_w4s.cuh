@@ -308,7 +308,7 @@ grouped_gemm_w4_smem_kernel(const __grid_constant__ CUtensorMap tm_tok,
                                SITE_MMA_ACC_EMPTY))
           break;
         idesc_ring[tile & 7u] = idesc;
-        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(items_addr), "r"(tile + 1u) : "memory");
+        post_count(items_addr, tile + 1u);
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait_bounded(bar_tfull(a), tph, abort_flag, SITE_WS_TOK_FULL)) {
             ok = false;
@@ -319,7 +319,7 @@ grouped_gemm_w4_smem_kernel(const __grid_constant__ CUtensorMap tm_tok,
             break;
           }
           ++it;
-          asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(ready_addr), "r"(it) : "memory");
+          post_count(ready_addr, it);
           if (++u == SLOTS) {
             u = 0;
             uph ^= 1u;
@@ -334,34 +334,14 @@ grouped_gemm_w4_smem_kernel(const __grid_constant__ CUtensorMap tm_tok,
   } else if (warp == 1) {
     if (lane == 0) {
       // ---- UMMA issuer: A = token tile a, B = unpacked weights of slot u.  Ordering: the watcher
-      // observes the mbarriers (acquire), then publishes with st.release; this thread's volatile
-      // loads of one shared-memory word after another are performed in program order, and
-      // tcgen05.fence::after_thread_sync orders the UMMAs after the load that saw the new count.
-      auto poll_above = [&](uint32_t addr, uint32_t have, int site) -> uint32_t {
-        // returns a value > have, or 0 after giving up (abort flag set); the timer is only read
-        // once the word has been found unchanged a few times
-        uint32_t v;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-        }
-        const uint64_t t0 = global_timer_ns();
-        uint32_t spins = 0;
-        while (true) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-          if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
-            if (!*abort_flag) *abort_flag = site;
-            return 0;
-          }
-        }
-      };
+      // observes the mbarriers (acquire), then publishes with a release that this thread's reads
+      // acquire, and tcgen05.fence::after_thread_sync orders the UMMAs after the load that saw the
+      // new count.
       int u = 0, a = 0;
       uint32_t it = 0, tile = 0, ready_known = 0, items_known = 0;
       bool ok = true;
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x, ++tile) {
-        if (items_known <= tile && (items_known = poll_above(items_addr, tile, SITE_MMA_ACC_EMPTY)) == 0) {
+        if (items_known <= tile && (items_known = poll_above(items_addr, tile, abort_flag, SITE_MMA_ACC_EMPTY)) == 0) {
           ok = false;
           break;
         }
@@ -371,7 +351,7 @@ grouped_gemm_w4_smem_kernel(const __grid_constant__ CUtensorMap tm_tok,
         const uint32_t d_tmem = tmem_base + buf * kWsBN;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           if (ready_known <= it) {
-            if ((ready_known = poll_above(ready_addr, it, SITE_MMA_FULL)) == 0) {
+            if ((ready_known = poll_above(ready_addr, it, abort_flag, SITE_MMA_FULL)) == 0) {
               ok = false;
               break;
             }

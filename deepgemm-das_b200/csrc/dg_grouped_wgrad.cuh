@@ -25,7 +25,7 @@
 //               use (a group usually ends in one).  Steps whose 16 rows all count, nearly every one,
 //               come from the ring.
 //   warp 7      watcher (leader): waits on the barriers in the UMMA issuer's place and posts counts in
-//               plain shared-memory words.  The issuer has 512 cycles for a chunk (four instructions
+//               plain shared-memory words (store-release, load-acquire).  The issuer has 512 cycles for a chunk (four instructions
 //               of 256 x 256 x 16); a first look at a barrier alone takes 200 of them.
 // Which rows count is known beforehand: every block of the grid reads all of m_indices once (from
 // L2) and keeps a byte for each 128 rows.  Two earlier forms cleared the rows in the ring, in
@@ -383,24 +383,6 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       // ---- UMMA issuer.  It touches no barrier and looks a block of rows ahead in the table.
-      auto poll_above = [&](uint32_t addr, uint32_t have, int site) -> uint32_t {
-        uint32_t v;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-        }
-        const uint64_t t0 = global_timer_ns();
-        uint32_t spins = 0;
-        while (true) {
-          asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-          if (v > have) return v;
-          if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
-            if (!*abort_flag) *abort_flag = site;
-            return 0;
-          }
-        }
-      };
       uint32_t it = 0, tile = 0, tail = 0, stages_known = 0, items_known = 0, tails_known = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
@@ -411,7 +393,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
           const Item w = segment(whole, sg, segs);
           const uint32_t buf = tile & 1u;
           int n_next = valid[blocks[w.b0]];
-          if (items_known <= tile && (items_known = poll_above(items_addr, tile, WG_SITE_ACC_EMPTY)) == 0) {
+          if (items_known <= tile && (items_known = poll_above(items_addr, tile, abort_flag, WG_SITE_ACC_EMPTY)) == 0) {
             ok = false;
             break;
           }
@@ -437,7 +419,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
               if (steps == 0) break;
               const int s = it % S;
               if (stages_known <= it) {
-                if ((stages_known = poll_above(stages_addr, it, WG_SITE_READY)) == 0) {
+                if ((stages_known = poll_above(stages_addr, it, abort_flag, WG_SITE_READY)) == 0) {
                   ok = false;
                   break;
                 }
@@ -457,7 +439,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
             }
             for (int r = ragged_steps(n); ok && r > 0; --r) {
               if (tails_known <= tail) {
-                if ((tails_known = poll_above(tails_addr, tail, WG_SITE_TAIL_READY)) == 0) {
+                if ((tails_known = poll_above(tails_addr, tail, abort_flag, WG_SITE_TAIL_READY)) == 0) {
                   ok = false;
                   break;
                 }
@@ -482,9 +464,6 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
   } else if (warp == 7) {
     if (lane == 0 && rank == 0) {
       // ---- watcher
-      auto post = [&](uint32_t addr, uint32_t v) {
-        asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-      };
       uint32_t it = 0, tile = 0, tail = 0;
       bool ok = true;
       for (int item = unit; ok && item < n_items; item += units) {
@@ -497,7 +476,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
             ok = false;
             break;
           }
-          post(items_addr, ++tile);
+          post_count(items_addr, ++tile);
           for (int i = 0; ok && i < w.blocks; ++i) {
             const int n = valid[blocks[w.b0 + i]];
             for (int half = 0; half < 2; ++half) {
@@ -506,7 +485,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
                 ok = false;
                 break;
               }
-              post(stages_addr, ++it);
+              post_count(stages_addr, ++it);
             }
             for (int r = ragged_steps(n); ok && r > 0; --r) {
               if (!mbar_wait_bounded(bar_tail_ready, tail & 1u, abort_flag, WG_SITE_TAIL_READY)) {
@@ -514,7 +493,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
                 break;
               }
               if constexpr (CL == 2) wg_fence_cluster();  // the other block's stores
-              post(tails_addr, ++tail);
+              post_count(tails_addr, ++tail);
             }
           }
         }

@@ -81,6 +81,38 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, ok);
 }
 
+// ----------------------------------------------------------------------------- posted counts
+// A warp that waits on mbarriers in the place of another thread of the block posts what it has seen
+// as a count in a plain shared-memory word, and that thread reads it.  Release and acquire make what the
+// poster observed (copies, other warps' stores, descriptors it wrote) happen before what the reader
+// does next; a volatile read in the reader's place promises nothing of the kind.
+__device__ __forceinline__ void post_count(uint32_t addr, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t read_count(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// A value > have, or 0 after giving up (bounded like mbar_wait_bounded, abort flag set).  The timer is
+// only read once the word has been found unchanged a few times (reading it costs about 100 cycles).
+__device__ __forceinline__ uint32_t poll_above(uint32_t addr, uint32_t have, volatile int* abort_flag, int site) {
+  uint32_t v;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i)
+    if ((v = read_count(addr)) > have) return v;
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0;
+#pragma unroll 1
+  while (true) {
+    if ((v = read_count(addr)) > have) return v;
+    if ((++spins & 63u) == 0 && (*abort_flag || global_timer_ns() - t0 > 1500000000ull)) {
+      if (!*abort_flag) *abort_flag = site;
+      return 0;
+    }
+  }
+}
+
 // ----------------------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
