@@ -241,11 +241,10 @@ __device__ __forceinline__ void ck_values(const CkCodes<VEC>& q, float s, float 
     for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
   }
 }
-constexpr float kCkMaxF32 = 3.402823466e+38f;
 template <class T>
 __device__ __forceinline__ float ck_most();
 template <>
-__device__ __forceinline__ float ck_most<float>() { return kCkMaxF32; }
+__device__ __forceinline__ float ck_most<float>() { return 3.402823466e+38f; }
 template <>
 __device__ __forceinline__ float ck_most<__half>() { return 65504.0f; }
 template <>
@@ -413,7 +412,9 @@ __global__ void __launch_bounds__(kCkThreads) act_checkpoint_kernel(const ActChe
   }
 }
 
-// Backward from the checkpoint: 108.9 us = 6.6 TB/s for the same rows.
+// Backward from the checkpoint: 108.9 us = 6.6 TB/s for the same rows.  Gate and up are at most
+// the largest finite value of their type, as in restore_rows_kernel: an fp16 65504 that is held as
+// 65536 does not overflow the activation it is multiplied into.
 template <class T, bool VEC, int KIND>
 __global__ void __launch_bounds__(kCkThreads) act_checkpoint_grad_kernel(const ActCheckpointParams p) {
   constexpr int kLanes = CkValues<T, VEC>::kLanes, N = CkValues<T, VEC>::N, U = kCkActUnits;
@@ -447,8 +448,8 @@ __global__ void __launch_bounds__(kCkThreads) act_checkpoint_grad_kernel(const A
     CkValues<T, VEC> dg, du, a;
     if (!skip[k]) {
       float gv[N], uv[N];
-      ck_values<KIND, VEC>(qg[k], sg[k], kCkMaxF32, gv);
-      ck_values<KIND, VEC>(qu[k], su[k], kCkMaxF32, uv);
+      ck_values<KIND, VEC>(qg[k], sg[k], ck_most<T>(), gv);
+      ck_values<KIND, VEC>(qu[k], su[k], ck_most<T>(), uv);
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         float fg[2], fu[2], fa[2];

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import deepgemm
-from deepgemm import grouped_bf16_input_grad, grouped_bf16_weight_grad
+from deepgemm import grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -41,3 +41,21 @@ def test_ragged_steps_are_read_after_they_are_written(tile):
     for _ in range(50):
         assert torch.equal(grouped_bf16_weight_grad(*args, dtype=F32, tile=tile), want)
     deepgemm.check_device_status()
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_the_largest_values_stay_finite_in_the_backward_pass(dtype, kind):
+    """A value beside the largest of its type may be held by a code beyond it (255 / 256 of a power of two);
+    it counts as that largest value, so what is finite going forward is finite coming back."""
+    top = torch.finfo(dtype).max
+    x = torch.zeros(6, 2, 256, dtype=torch.float64)
+    for r, (g, u) in enumerate(((top, 1.0), (1.0, top), (top, -1.0), (-1.0, top), (-top, 1.0), (top, 0.5))):
+        x[r, 0, 130], x[r, 1, 130] = g, u
+    x = x.view(6, 512).to(dtype).to(DEV)
+    act, kept = silu_mul_checkpoint(x, kind=kind)
+    dx, again = silu_mul_checkpoint_grad(kept, torch.ones(6, 256, dtype=dtype, device=DEV))
+    assert bool(act.isfinite().all()) and bool(dx.isfinite().all()) and bool(again.isfinite().all())
+    # within what eight bits hold of the two factors, 2^-4 each
+    act, again = act.double(), again.double()
+    assert bool(((again - act).abs() <= act.abs() * (2.0 ** -4 + 2.0 ** -4 + 2.0 ** -8)).all())
