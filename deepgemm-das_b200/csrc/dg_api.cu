@@ -202,7 +202,7 @@ struct Problem {
   const int32_t* offsets;
   int G, M, N, K, block_n, expected_m;
   int narrow;  // filled by validate_and_launch: KernelParams::narrow
-  int clear;     // b_trans: rows with m_indices < 0 are set to zero
+  int clear;     // b_trans: rows that no tile writes are set to zero
   int b_trans;   // 1: dg_grouped_input_grad (contiguous layout, bf16): N = columns of D, K = contraction = rows of a weight block
   int dense;     // 1: dg_dense_gemm (row-major weights, no masked_m, any N, out_kind honoured)
   int out_kind;  // DG_OUT_BF16 / DG_OUT_F16 / DG_OUT_F32

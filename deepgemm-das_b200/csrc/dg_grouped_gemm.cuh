@@ -108,7 +108,7 @@ struct KernelParams {
   const void* gather_a;  // the [size_m][K] activation the rows are gathered from
   int block_m, num_blocks, num_sorted, real_topk, size_m;
   int tbl_groups;  // MODE_SORTED: entries per array of the schedule table (the most runs it holds)
-  int clear;   // kBT: the epilogue warps set the rows of D with m_indices < 0 to zero before their first tile
+  int clear;   // kBT: the epilogue warps set the rows of D that no tile writes to zero before their first tile
   int narrow;  // masked / compact: 0 = tiles stay BN columns wide, 1 = the kernel may narrow them
                // (down to 32 columns) when few groups have rows, 128 / 64 / 32 = forced width
 };
@@ -494,12 +494,15 @@ struct ItemDecoder {
   }
 };
 
-// kBT: rows of D that stand for nothing are set to zero by the epilogue warps (`warps` of them in the
-// grid, this one number `first`) while the first tile's products run; nothing else writes them.
+// kBT: the rows of D that no tile writes (their entry is negative, or the first one of their block
+// names no group) are set to zero by the epilogue warps (`warps` of them in the grid, this one number
+// `first`) while the first tile's products run; nothing else writes them.
 __device__ __forceinline__ void clear_padding(const KernelParams& p, int first, int warps, int lane) {
   for (int rb = 0; rb < p.M; rb += 32 * warps) {
     const int mine = rb + lane * warps + first;
-    unsigned mask = __ballot_sync(0xffffffffu, mine < p.M && p.sched[mine] < 0);
+    const bool unwritten = mine < p.M && (p.sched[mine] < 0 || static_cast<unsigned>(p.sched[mine & ~(kBM - 1)]) >=
+                                                                   static_cast<unsigned>(p.G));
+    unsigned mask = __ballot_sync(0xffffffffu, unwritten);
     while (mask) {
       const int i = __ffs(mask) - 1;
       mask &= mask - 1;

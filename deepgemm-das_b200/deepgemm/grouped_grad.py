@@ -39,7 +39,8 @@ def _indices(m_indices: torch.Tensor, rows: torch.Tensor, what: str) -> None:
 def grouped_bf16_input_grad(dy: torch.Tensor, weight: torch.Tensor, m_indices: torch.Tensor,
                             out: Optional[torch.Tensor] = None, *, block_n: int = 0) -> torch.Tensor:
     """dy bf16 ``[M, N]``, weight the packed bf16 ``[G, K/64, N, 64]`` -> dx bf16 ``[M, K]``.  Rows with
-    ``m_indices < 0`` are zero, or, in a given ``out``, left as they are."""
+    ``m_indices < 0``, and those of a block whose first entry names no group, are zero, or, in a given
+    ``out``, left as they are."""
     what = "grouped_bf16_input_grad"
     if _glue is not None and (made := _glue.input_grad(dy, weight, m_indices, out, block_n)) is not None:
         return made

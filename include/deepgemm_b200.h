@@ -584,7 +584,8 @@ DG_API int dg_ep_barrier(const dg_ep_barrier_args* args, void* stream);
 /* Gradient of the rows of the contiguous BF16 grouped GEMM (dg_contig_gemm with DG_KIND_BF16), on
  * the weight that the forward pass uses, in the layout it has there:
  *   dx[i][c] = bf16( sum over r of dy[i][r] * W[m_indices[i]][r][c] ),  W[g][r][c] = packed[g][c / 64][r][c % 64]
- * m_indices names one group for every 128 rows, as there. */
+ * m_indices names one group for every 128 rows, as there.  Rows that have none (a negative entry, or a
+ * block whose first entry is negative or >= num_groups) are not computed: see `clear`. */
 typedef struct dg_input_grad_args {
   const void*    dy;        /* [m_total][n] bf16 */
   const void*    w_packed;  /* [num_groups][k / 64][n][64] bf16 */
@@ -595,7 +596,7 @@ typedef struct dg_input_grad_args {
   int32_t n;                /* rows of a group's weight, multiple of 16 */
   int32_t k;                /* its columns, multiple of 64 */
   int32_t block_n;          /* 0 = choose; 128 / 256 = one-CTA tile width; 512 = two-CTA 256x256 tiles */
-  int32_t clear;            /* rows with m_indices < 0: 0 = left as they are, else set to zero */
+  int32_t clear;            /* rows of dx without a group: 0 = left as they are, else set to zero */
   int32_t*       status;    /* NULL, or int32[DG_STATUS_WORDS] */
 } dg_input_grad_args;
 DG_API int dg_grouped_input_grad(const dg_input_grad_args* args, void* stream);

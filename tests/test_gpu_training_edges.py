@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import deepgemm
-from deepgemm import grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
+from deepgemm import grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -59,3 +59,44 @@ def test_the_largest_values_stay_finite_in_the_backward_pass(dtype, kind):
     # within what eight bits hold of the two factors, 2^-4 each
     act, again = act.double(), again.double()
     assert bool(((again - act).abs() <= act.abs() * (2.0 ** -4 + 2.0 ** -4 + 2.0 ** -8)).all())
+
+
+def unnamed_blocks(groups):
+    """Blocks of 128 rows whose first entry names no group, with entries that do behind it."""
+    mi = torch.full((7 * 128 + 40,), -1, dtype=torch.int32)
+    for b, (first, others) in enumerate(((0, 0), (-1, 1), (1, 1), (groups, 0), (0, 0), (-1, 0), (2, 2), (-1, 1))):
+        mi[b * 128 + 1:b * 128 + 100], mi[b * 128] = others, first
+    named = ((mi[::128] >= 0) & (mi[::128] < groups)).repeat_interleave(128)[:mi.numel()]
+    return mi, named & (mi >= 0)
+
+
+def poison(*like):
+    """Leaves NaN in the blocks that the allocator hands out next."""
+    held = [torch.full(shape, float("nan"), dtype=dtype, device=DEV) for shape, dtype in like for _ in range(6)]
+    del held
+
+
+@pytest.mark.parametrize("block_n", [128, 256, 512, 0])
+def test_input_grad_writes_every_row_of_its_own_result(block_n):
+    gen = torch.Generator().manual_seed(1)
+    g, n, k = 3, 96, 512
+    mi, written = unnamed_blocks(g)
+    dy, w = whole(gen, mi.numel(), n), whole(gen, g, n, k, lim=2)
+    dyd, wd, md = dy.to(DEV), packed(w).to(DEV), mi.to(DEV)
+    deepgemm.check_device_status()
+    poison(((mi.numel(), k), BF))
+    got = grouped_bf16_input_grad(dyd, wd, md, block_n=block_n).cpu()
+    with pytest.raises(RuntimeError, match="expert index was outside"):
+        deepgemm.check_device_status()
+    want = torch.zeros(mi.numel(), k, dtype=BF)
+    for e in range(g):
+        r = written & (mi == e)
+        want[r] = (dy[r].double() @ w[e].double()).bfloat16()
+    assert torch.equal(got, want)
+    # in a buffer of the caller's the same rows are left as they are
+    buf = torch.full((mi.numel(), k), 3.0, dtype=BF, device=DEV)
+    grouped_bf16_input_grad(dyd, wd, md, buf, block_n=block_n)
+    want[~written] = 3.0
+    assert torch.equal(buf.cpu(), want)
+    with pytest.raises(RuntimeError):
+        deepgemm.check_device_status()
