@@ -379,16 +379,19 @@ struct TokenUnsortGradParams {
   int clear_blocks;          // blocks behind those of the tokens that clear rows
 };
 
-// Sets rows with m_indices < 0 to zero: block `b` of `nb`.  Most of them lie together, so the warps
-// take every so-many-th row; lane l looks at the warp's l-th.
+// Sets rows with m_indices < 0 to zero (groups > 0: and those of a 128-row block whose first entry is not
+// in [0, groups)): block `b` of `nb`.  Most of them lie together, so the warps take every so-many-th
+// row; lane l looks at the warp's l-th.
 template <class T, bool VEC>
-__device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indices, int rows, int H, int b, int nb) {
+__device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indices, int rows, int H, int b, int nb, int groups = 0) {
   const int lane = threadIdx.x & 31;
   const int warps = nb * (blockDim.x >> 5);
   const int first = b * (blockDim.x >> 5) + (threadIdx.x >> 5);
   for (long long rb = 0; rb < rows; rb += 32LL * warps) {
     const long long mine = rb + (long long)lane * warps + first;
-    unsigned mask = __ballot_sync(0xffffffffu, mine < rows && m_indices[mine] < 0);
+    const bool stands_for_none =
+        mine < rows && (m_indices[mine] < 0 || (groups > 0 && static_cast<unsigned>(m_indices[mine & ~127LL]) >= static_cast<unsigned>(groups)));
+    unsigned mask = __ballot_sync(0xffffffffu, stands_for_none);
     while (mask) {
       const int i = __ffs(mask) - 1;
       mask &= mask - 1;
@@ -499,8 +502,8 @@ __global__ void __launch_bounds__(32 * kUnsortGradWarps, grad_blocks(VEC)) token
 
 constexpr int kClearThreads = 128;
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kClearThreads) clear_rows_kernel(T* out, const int32_t* m_indices, int rows, int H) {
-  clear_rows_block<T, VEC>(out, m_indices, rows, H, blockIdx.x, gridDim.x);
+__global__ void __launch_bounds__(kClearThreads) clear_rows_kernel(T* out, const int32_t* m_indices, int rows, int H, int groups) {
+  clear_rows_block<T, VEC>(out, m_indices, rows, H, blockIdx.x, gridDim.x, groups);
 }
 
 }  // namespace dg

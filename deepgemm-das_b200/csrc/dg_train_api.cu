@@ -265,7 +265,7 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
 int dg_clear_padding_rows(const dg_clear_rows_args* a, void* stream) {
   if (a == nullptr) return DG_ERR_NULL_POINTER;
   if (bad_elem(a->elem)) return DG_ERR_BAD_KIND;
-  if (a->num_rows < 0 || a->hidden < 1) return DG_ERR_BAD_SHAPE;
+  if (a->num_rows < 0 || a->hidden < 1 || a->num_groups < 0) return DG_ERR_BAD_SHAPE;
   if (a->num_rows == 0) return DG_OK;
   if (!a->rows || !a->m_indices) return DG_ERR_NULL_POINTER;
   if (!aligned_to(a->rows, elem_size(a->elem))) return DG_ERR_BAD_ALIGNMENT;
@@ -276,7 +276,7 @@ int dg_clear_padding_rows(const dg_clear_rows_args* a, void* stream) {
   by_type(a->elem, vec_rows(a->rows, a->hidden, a->hidden, a->elem), [&](auto t, auto v) {
     using T = decltype(t);
     clear_rows_kernel<T, decltype(v)::value><<<grid, kClearThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<T*>(a->rows), a->m_indices, a->num_rows, a->hidden);
+        static_cast<T*>(a->rows), a->m_indices, a->num_rows, a->hidden, a->num_groups);
   });
   return launched(1);
 }

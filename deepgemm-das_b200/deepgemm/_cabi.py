@@ -421,7 +421,7 @@ class ClearRowsArgs(C.Structure):
         ("elem", C.c_int32),
         ("num_rows", C.c_int32),
         ("hidden", C.c_int32),
-        ("reserved", C.c_int32),
+        ("num_groups", C.c_int32),
         ("rows", C.c_void_p),
         ("m_indices", C.c_void_p),
     ]

@@ -34,7 +34,7 @@ class _ExpertMlp(torch.autograd.Function):
         del h
         y = torch.empty((m, w2.shape[2]), dtype=torch.bfloat16, device=rows.device)
         m_grouped_bf16_gemm_nt_contiguous(act, w2, y, m_indices)
-        clear_padding_rows(y, m_indices)
+        clear_padding_rows(y, m_indices, w2.shape[0])
         entered = checkpoint_rows(rows, kind=kind) if recorded and ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(entered[0], entered[1], kept.q, kept.scale, w13, w2, m_indices)
         return y
@@ -48,7 +48,8 @@ class _ExpertMlp(torch.autograd.Function):
         if dy.data_ptr() % 16:  # a piece of a larger gradient, begun where the products cannot read it
             dy = dy.clone()
         drows = dw13 = dw2 = None
-        # rows that stand for no pair are neither written here nor read by what follows
+        # rows that stand for no pair are neither written here nor read by what follows (rows of a block
+        # that names no expert are carried through the activation as they are, and dropped by the products)
         dact = torch.empty((dy.shape[0], w2.shape[1] * 64), dtype=torch.bfloat16, device=dy.device)
         grouped_bf16_input_grad(dy, w2, m_indices, dact)
         dh, act = silu_mul_checkpoint_grad(Checkpoint(q, scale, torch.bfloat16), dact, m_indices=m_indices, need_act=need_w2)
@@ -67,7 +68,8 @@ def expert_mlp_bf16(rows: torch.Tensor, m_indices: torch.Tensor, w13: torch.Tens
     """Both GEMMs of the experts with the activation between them, on rows sorted by expert
     (``sort_tokens`` with ``align`` 128 or 256): rows bf16 ``[M, K]``, w13 the packed bf16
     ``[E, K/64, 2 I, 64]`` (gate rows, then up rows), w2 the packed ``[E, I/64, K_out, 64]`` -> bf16
-    ``[M, K_out]``, zero in rows with ``m_indices < 0``.  Differentiable in rows, w13 and w2 (their
+    ``[M, K_out]``, zero in rows with ``m_indices < 0`` and in blocks of 128 rows whose first entry names
+    no expert.  Differentiable in rows, w13 and w2 (their
     gradients have the packed layout); ``checkpoint`` ("fp8" or "int8") is what the rows and the
     activation's inputs are kept in for the backward pass."""
     what = "expert_mlp_bf16"

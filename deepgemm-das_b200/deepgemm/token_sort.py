@@ -233,14 +233,18 @@ def unsort_tokens(y: torch.Tensor, plan: TokenPlan, weights: Optional[torch.Tens
     return _unsort(y, dest, w, out, "unsort_tokens")
 
 
-def clear_padding_rows(rows: torch.Tensor, m_indices: torch.Tensor) -> torch.Tensor:
-    """Sets the rows with ``m_indices < 0`` to zero, in place: what a grouped GEMM leaves unwritten."""
+def clear_padding_rows(rows: torch.Tensor, m_indices: torch.Tensor, num_groups: int = 0) -> torch.Tensor:
+    """Sets the rows with ``m_indices < 0`` to zero, in place.  ``num_groups``: all rows that a contiguous
+    grouped GEMM of as many groups leaves unwritten, i.e. also those of a block of 128 rows whose first
+    entry names no group."""
     what = "clear_padding_rows"
+    if not 0 <= num_groups <= _cabi.MAX_GROUPS:
+        raise ValueError(f"{what}: num_groups must be 0..{_cabi.MAX_GROUPS}, got {num_groups}")
     _rows_arg(rows, "rows", what)
     if not rows.is_contiguous():
         raise ValueError(f"{what}: rows must be contiguous")
     m_indices = _int_arg(m_indices, (rows.shape[0],), rows.device, "m_indices", what)
     args = _cabi.ClearRowsArgs(elem=_ELEM[rows.dtype], num_rows=int(rows.shape[0]), hidden=int(rows.shape[1]),
-                               rows=rows.data_ptr(), m_indices=m_indices.data_ptr())
+                               num_groups=int(num_groups), rows=rows.data_ptr(), m_indices=m_indices.data_ptr())
     _launch(_cabi.lib.dg_clear_padding_rows, args, rows.device, what)
     return rows

@@ -713,12 +713,14 @@ typedef struct dg_token_unsort_grad_args {
 } dg_token_unsort_grad_args;
 DG_API int dg_token_unsort_grad(const dg_token_unsort_grad_args* args, void* stream);
 
-/* Sets the rows with m_indices < 0 to zero. */
+/* Sets the rows with m_indices < 0 to zero.  num_groups > 0: those that dg_contig_gemm with as many groups
+ * leaves unwritten, i.e. also every row of a 128-row block whose first entry is negative or
+ * >= num_groups. */
 typedef struct dg_clear_rows_args {
   int32_t elem;
   int32_t num_rows;
   int32_t hidden;
-  int32_t reserved;
+  int32_t num_groups;       /* 0: the entries of the rows alone */
   void*          rows;      /* [num_rows][hidden] */
   const int32_t* m_indices; /* [num_rows] */
 } dg_clear_rows_args;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import deepgemm
-from deepgemm import grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
+from deepgemm import expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -100,3 +100,29 @@ def test_input_grad_writes_every_row_of_its_own_result(block_n):
     assert torch.equal(buf.cpu(), want)
     with pytest.raises(RuntimeError):
         deepgemm.check_device_status()
+
+
+def test_the_expert_part_writes_every_row_of_its_results():
+    gen = torch.Generator().manual_seed(2)
+    mi, written = unnamed_blocks(3)
+    md, wd = mi.to(DEV), written.to(DEV)
+    rows, g = torch.randn(mi.numel(), 128, generator=gen).bfloat16().to(DEV), torch.randn(mi.numel(), 128, generator=gen).bfloat16().to(DEV)
+    w13, w2 = (torch.randn(3, 2, 256, 64, generator=gen) / 11).bfloat16().to(DEV), (torch.randn(3, 2, 128, 64, generator=gen) / 11).bfloat16().to(DEV)
+    clean = torch.where(wd, md, -1)                  # the same, said in the entries themselves
+    clean[::128] = torch.where(wd[::128], md[::128], -1)
+
+    def run(m_indices):
+        leaves = [t.clone().requires_grad_() for t in (rows, w13, w2)]
+        poison((rows.shape, BF), ((mi.numel(), 256), BF), ((mi.numel(), 128), BF))
+        y = expert_mlp_bf16(leaves[0], m_indices, *leaves[1:])
+        poison((rows.shape, BF), ((mi.numel(), 256), BF), ((mi.numel(), 128), BF))
+        return [y.detach(), *torch.autograd.grad(y, leaves, g)]
+
+    want = run(clean)
+    deepgemm.check_device_status()
+    got = run(md)
+    with pytest.raises(RuntimeError, match="expert index was outside"):
+        deepgemm.check_device_status()
+    assert bool((got[0][~wd] == 0).all()) and bool((got[1][~wd] == 0).all())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
