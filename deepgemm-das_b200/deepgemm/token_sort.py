@@ -9,13 +9,14 @@ points, ``align=1`` with ``plan.counts`` / ``plan.offsets`` for the compact one.
 Rows that stand for no pair (an expert's padding, everything behind the last expert;
 ``plan.m_indices < 0``) are zero in what these functions allocate and are left as they are in a
 buffer that the caller passes as ``out``.  No function here synchronises, and each can be captured
-into a CUDA graph.
+into a CUDA graph.  Gradients are those of reverse mode; forward-mode differentiation is refused.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
@@ -56,6 +57,12 @@ def _rows_arg(t: torch.Tensor, name: str, what: str) -> torch.Tensor:
 def _grad_arg(t: torch.Tensor) -> torch.Tensor:
     """A gradient as autograd hands it over: expanded and transposed ones are laid out first."""
     return t if t.dim() == 2 and t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of them carries a tangent of forward-mode differentiation (which the autograd functions
+    below refuse: the native path would drop it)."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _int_arg(t: torch.Tensor, shape, device, name: str, what: str) -> torch.Tensor:
@@ -207,7 +214,7 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, al
     expert beginning at a multiple of ``align``.  A negative id is a pair without a row (an expert
     that lives elsewhere); an id >= num_experts is treated the same and reported by
     ``check_device_status``.  Differentiable in x.  ``out``: a buffer for the rows (no gradient)."""
-    if torch.is_grad_enabled() and x.requires_grad:
+    if torch.is_grad_enabled() and x.requires_grad or _has_tangent(x):
         if out is not None:
             raise ValueError("sort_tokens: out cannot be given where a gradient is recorded")
         made = _SortTokens.apply(x, topk_ids, num_experts, align)
@@ -222,7 +229,7 @@ def unsort_tokens(y: torch.Tensor, plan: TokenPlan, weights: Optional[torch.Tens
     j; y ``[rows, H]`` in the plan's layout, weights fp32 ``[T, top_k]`` or None for ones.  Pairs
     without a row add nothing.  Differentiable in y and weights; the gradient of y is zero in rows
     that stand for no pair."""
-    recorded = torch.is_grad_enabled() and (y.requires_grad or weights is not None and weights.requires_grad)
+    recorded = torch.is_grad_enabled() and (y.requires_grad or weights is not None and weights.requires_grad) or _has_tangent(y, weights)
     if _glue is not None and not recorded and (made := _glue.unsort_tokens(y, plan.dest, plan.m_indices, weights, out)) is not None:
         return made
     dest, m_indices, w = _plan_args(y, plan, weights, "unsort_tokens")

@@ -2,9 +2,11 @@
 results on them are compared for equality after the one rounding."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import deepgemm
-from deepgemm import expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul_checkpoint, silu_mul_checkpoint_grad
+from deepgemm import (expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
+                      silu_mul_checkpoint_grad, sort_tokens, unsort_tokens)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -126,3 +128,22 @@ def test_the_expert_part_writes_every_row_of_its_results():
     assert bool((got[0][~wd] == 0).all()) and bool((got[1][~wd] == 0).all())
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused_and_not_passed_by():
+    x = torch.randn(9, 64, device=DEV)
+    ids = torch.randint(0, 3, (9, 2), device=DEV)
+    rows, plan = sort_tokens(x, ids, 3)
+    w = torch.rand(9, 2, device=DEV)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: sort_tokens(dual(x), ids, 3), lambda: sort_tokens(dual(x), ids, 3, out=rows.clone()),
+                             lambda: unsort_tokens(dual(rows), plan, w), lambda: unsort_tokens(rows, plan, dual(w)),
+                             lambda: unsort_tokens(rows, plan, dual(w), out=x.clone()), lambda: silu_mul(dual(x))):
+                    with pytest.raises((RuntimeError, NotImplementedError, ValueError), match="jvp|forward|out cannot be given"):
+                        call()
+        # tensors without a tangent are not concerned
+        assert torch.equal(sort_tokens(x, ids, 3)[0], rows)
+        assert unsort_tokens(rows, plan, w).shape == x.shape
