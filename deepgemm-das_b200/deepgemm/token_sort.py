@@ -97,10 +97,9 @@ def _sort(x, topk_ids, num_experts, align, out):
     ids = topk_ids if topk_ids.is_contiguous() else topk_ids.contiguous()
     dev = x.device
     rows = torch.empty((cap, h), dtype=x.dtype, device=dev) if out is None else _out_arg(out, x, (cap, h), what)
-    sizes = [t * k, cap, num_experts, num_experts, 1]  # in one buffer, each on a 16-byte boundary
-    rooms = [(n + 3) // 4 * 4 for n in sizes]
-    parts = torch.empty(sum(rooms), dtype=torch.int32, device=dev).split(rooms)
-    dest, m_indices, counts, offsets, m_total = (part[:n] for part, n in zip(parts, sizes))
+    # tensors of their own (views of one buffer would share a version: writing counts would spoil the saved dest)
+    dest, m_indices, counts, offsets, m_total = (torch.empty(size, dtype=torch.int32, device=dev)
+                                                 for size in ((t, k), cap, num_experts, num_experts, 1))
     need = int(_cabi.lib.dg_token_sort_scratch_bytes(t, k, num_experts))
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     args = _cabi.TokenSortArgs(
@@ -110,7 +109,7 @@ def _sort(x, topk_ids, num_experts, align, out):
         m_total=m_total.data_ptr(), scratch=scratch.data_ptr() if need else None, scratch_bytes=need,
         status=device_status_words(dev).data_ptr(), clear=int(out is None))
     _launch(_cabi.lib.dg_token_sort, args, dev, what)
-    return rows, dest.view(t, k), m_indices, counts, offsets, m_total
+    return rows, dest, m_indices, counts, offsets, m_total
 
 
 def _unsort(y, dest, weights, out, what):

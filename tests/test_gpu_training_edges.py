@@ -6,7 +6,7 @@ import torch.autograd.forward_ad as fwad
 
 import deepgemm
 from deepgemm import (expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
-                      silu_mul_checkpoint_grad, sort_tokens, unsort_tokens)
+                      silu_mul_checkpoint_grad, sort_tokens, token_sort, unsort_tokens)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -147,3 +147,26 @@ def test_forward_mode_is_refused_and_not_passed_by():
         # tensors without a tangent are not concerned
         assert torch.equal(sort_tokens(x, ids, 3)[0], rows)
         assert unsort_tokens(rows, plan, w).shape == x.shape
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_the_arrays_of_a_plan_are_apart(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(token_sort, "_glue", None)
+    x = torch.randn(20, 64, device=DEV).requires_grad_()
+    ids = torch.randint(-1, 3, (20, 2), device=DEV)
+    w = torch.rand(20, 2, device=DEV).requires_grad_()
+    g = torch.randn(20, 64, device=DEV)
+    rows, plan = sort_tokens(x, ids, 3)
+    want = torch.autograd.grad(unsort_tokens(rows, plan, w), (x, w), g)
+    rows, plan = sort_tokens(x, ids, 3)
+    out = unsort_tokens(rows, plan, w)
+    dest, m_indices = plan.dest.clone(), plan.m_indices.clone()
+    plan.counts.zero_()
+    plan.offsets.fill_(-5)
+    plan.m_total.fill_(7)
+    for a, b in zip(torch.autograd.grad(out, (x, w), g), want):
+        assert torch.equal(a, b)
+    assert torch.equal(plan.dest, dest) and torch.equal(plan.m_indices, m_indices)
+    for t in plan:
+        assert t.is_contiguous() and t.data_ptr() % 16 == 0
