@@ -312,28 +312,31 @@ py::object unsort_impl(const Tensor& y, const Tensor& dest, const Tensor& m_indi
   return py::cast(o);
 }
 
-py::object unsort_grad_impl(const Tensor& dout, const Tensor& y, const Tensor& dest, const Tensor& m_indices, const OptTensor& weights,
+// without y: the gradient of the rows alone
+py::object unsort_grad_impl(const Tensor& dout, const OptTensor& y, const Tensor& dest, const Tensor& m_indices, const OptTensor& weights,
                             bool need_dweights) {
-  const int dev = current(y);
-  if (dev < 0 || !rows_ok(y, dev) || !rows_ok(dout, dev) || !on(dest, dev) || dest.scalar_type() != at::kInt || dest.dim() != 2 ||
-      !ints_ok(m_indices, dev, y.size(0)))
+  const int dev = current(dout);
+  if (dev < 0 || !rows_ok(dout, dev) || !on(dest, dev) || dest.scalar_type() != at::kInt || dest.dim() != 2)
     return py::none();
-  const int64_t t = dest.size(0), k = dest.size(1), h = y.size(1);
-  if (dout.scalar_type() != y.scalar_type() || dout.size(0) != t || dout.size(1) != h) return py::none();
+  const int64_t t = dest.size(0), k = dest.size(1), h = dout.size(1), rows = m_indices.numel();
+  if (dout.size(0) != t || rows > INT32_MAX || !ints_ok(m_indices, dev, rows)) return py::none();
+  if (y.has_value() ? (!rows_ok(*y, dev) || y->scalar_type() != dout.scalar_type() || y->size(0) != rows || y->size(1) != h)
+                    : (weights.has_value() && need_dweights))
+    return py::none();
   if (weights.has_value() && (!on(*weights, dev) || weights->scalar_type() != at::kFloat || weights->sizes() != dest.sizes())) return py::none();
-  Tensor dy = make({y.size(0), h}, y.scalar_type(), y), dw;
-  if (weights.has_value() && need_dweights) dw = make({t, k}, at::kFloat, y);
+  Tensor dy = make({rows, h}, dout.scalar_type(), dout), dw;
+  if (weights.has_value() && need_dweights) dw = make({t, k}, at::kFloat, dout);
   dg_token_unsort_grad_args a{};
-  a.elem = elem_of(y);
+  a.elem = elem_of(dout);
   a.num_tokens = static_cast<int32_t>(t);
   a.top_k = static_cast<int32_t>(k);
   a.hidden = static_cast<int32_t>(h);
-  a.num_rows = static_cast<int32_t>(y.size(0));
+  a.num_rows = static_cast<int32_t>(rows);
   a.clear = 1;
-  a.y_stride = row_stride(y);
+  a.y_stride = y.has_value() ? row_stride(*y) : h;
   a.dout_stride = row_stride(dout);
   a.dout = dout.data_ptr();
-  a.y = y.data_ptr();
+  a.y = y.has_value() ? y->data_ptr() : nullptr;
   a.dest = dest.data_ptr<int32_t>();
   a.weights = weights.has_value() ? weights->data_ptr<float>() : nullptr;
   a.m_indices = m_indices.data_ptr<int32_t>();
@@ -521,7 +524,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unsort_tokens", [](const Tensor& y, const Tensor& dest, const Tensor& mi, const OptTensor& w, const OptTensor& out) {
     return count_obj(unsort_impl(y, dest, mi, w, out));
   });
-  m.def("unsort_tokens_grad", [](const Tensor& dout, const Tensor& y, const Tensor& dest, const Tensor& mi, const OptTensor& w, bool need) {
+  m.def("unsort_tokens_grad", [](const Tensor& dout, const OptTensor& y, const Tensor& dest, const Tensor& mi, const OptTensor& w, bool need) {
     return count_obj(unsort_grad_impl(dout, y, dest, mi, w, need));
   });
   m.def("checkpoint_rows", [](const Tensor& x, int64_t kind) { return count_obj(checkpoint_impl(x, kind)); });

@@ -125,15 +125,19 @@ def _unsort(y, dest, weights, out, what):
 
 
 def _plan_args(y, plan, weights, what):
-    """The checked (y, dest, m_indices, weights) of the functions that walk a plan back."""
+    """The checked (dest, m_indices, weights) of the functions that walk a plan back; y: the sorted rows."""
     _rows_arg(y, "the sorted rows", what)
+    return _plan_of(y.shape[0], y.device, plan, weights, what)
+
+
+def _plan_of(num_rows, device, plan, weights, what):
     if plan.dest.dim() != 2:
         raise ValueError(f"{what}: plan.dest must be [T, top_k], got {tuple(plan.dest.shape)}")
-    dest = _int_arg(plan.dest, plan.dest.shape, y.device, "plan.dest", what)
-    m_indices = _int_arg(plan.m_indices, (y.shape[0],), y.device, "plan.m_indices", what)
+    dest = _int_arg(plan.dest, plan.dest.shape, device, "plan.dest", what)
+    m_indices = _int_arg(plan.m_indices, (num_rows,), device, "plan.m_indices", what)
     if weights is not None:
-        if weights.device != y.device or weights.dtype != torch.float32 or weights.shape != plan.dest.shape:
-            raise ValueError(f"{what}: weights must be fp32 {tuple(plan.dest.shape)} on {y.device}, "
+        if weights.device != device or weights.dtype != torch.float32 or weights.shape != plan.dest.shape:
+            raise ValueError(f"{what}: weights must be fp32 {tuple(plan.dest.shape)} on {device}, "
                              f"got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
         weights = weights if weights.is_contiguous() else weights.contiguous()
     return dest, m_indices, weights
@@ -148,30 +152,38 @@ def sort_tokens_grad(drows: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
     return _unsort(drows, dest, None, None, "sort_tokens_grad")
 
 
-def unsort_tokens_grad(dout: torch.Tensor, y: torch.Tensor, plan: TokenPlan, weights: Optional[torch.Tensor] = None, *,
+def unsort_tokens_grad(dout: torch.Tensor, y: Optional[torch.Tensor], plan: TokenPlan, weights: Optional[torch.Tensor] = None, *,
                        need_dweights: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of ``unsort_tokens`` (with the whole plan: every row with ``m_indices >= 0`` is named
     by one pair): ``dy[dest[t, j]] = weights[t, j] * dout[t]`` (zero in rows that
     stand for no pair) and ``dweights[t, j] = <dout[t], y[dest[t, j]]>`` in fp32 (zero for a pair
-    without a row; None without weights)."""
+    without a row; None without weights).  Only ``dweights`` reads y: without it y may be None."""
     if _glue is not None and (made := _glue.unsort_tokens_grad(dout, y, plan.dest, plan.m_indices, weights, need_dweights)) is not None:
         return made
     what = "unsort_tokens_grad"
-    dest, m_indices, weights = _plan_args(y, plan, weights, what)
-    _rows_arg(dout, "dout", what)
-    if dout.device != y.device or dout.dtype != y.dtype or tuple(dout.shape) != (dest.shape[0], y.shape[1]):
-        raise ValueError(f"{what}: dout must be {y.dtype} {(dest.shape[0], y.shape[1])} on {y.device}, "
-                         f"got {dout.dtype} {tuple(dout.shape)} on {dout.device}")
+    if y is not None:
+        dest, m_indices, weights = _plan_args(y, plan, weights, what)
+        _rows_arg(dout, "dout", what)
+        if dout.device != y.device or dout.dtype != y.dtype or tuple(dout.shape) != (dest.shape[0], y.shape[1]):
+            raise ValueError(f"{what}: dout must be {y.dtype} {(dest.shape[0], y.shape[1])} on {y.device}, "
+                             f"got {dout.dtype} {tuple(dout.shape)} on {dout.device}")
+    else:
+        if weights is not None and need_dweights:
+            raise ValueError(f"{what}: the gradient of the weights needs y")
+        _rows_arg(dout, "dout", what)
+        dest, m_indices, weights = _plan_of(plan.m_indices.numel(), dout.device, plan, weights, what)
+        if dout.shape[0] != dest.shape[0]:
+            raise ValueError(f"{what}: dout must have {dest.shape[0]} rows, got {tuple(dout.shape)}")
     t, k = (int(v) for v in dest.shape)
-    h, rows = int(y.shape[1]), int(y.shape[0])
-    dy = torch.empty((rows, h), dtype=y.dtype, device=y.device)
-    dw = torch.empty((t, k), dtype=torch.float32, device=y.device) if weights is not None and need_dweights else None
+    h, rows = int(dout.shape[1]), int(m_indices.shape[0])
+    dy = torch.empty((rows, h), dtype=dout.dtype, device=dout.device)
+    dw = torch.empty((t, k), dtype=torch.float32, device=dout.device) if weights is not None and need_dweights else None
     args = _cabi.TokenUnsortGradArgs(
-        elem=_ELEM[y.dtype], num_tokens=t, top_k=k, hidden=h, num_rows=rows, clear=1,
-        y_stride=y.stride(0) if rows > 1 else h, dout_stride=dout.stride(0) if t > 1 else h, dout=dout.data_ptr(),
-        y=y.data_ptr(), dest=dest.data_ptr(), weights=weights.data_ptr() if weights is not None else None,
+        elem=_ELEM[dout.dtype], num_tokens=t, top_k=k, hidden=h, num_rows=rows, clear=1,
+        y_stride=y.stride(0) if y is not None and rows > 1 else h, dout_stride=dout.stride(0) if t > 1 else h,
+        dout=dout.data_ptr(), y=y.data_ptr() if y is not None else None, dest=dest.data_ptr(), weights=weights.data_ptr() if weights is not None else None,
         m_indices=m_indices.data_ptr(), dy=dy.data_ptr(), dw=dw.data_ptr() if dw is not None else None)
-    _launch(_cabi.lib.dg_token_unsort_grad, args, y.device, what)
+    _launch(_cabi.lib.dg_token_unsort_grad, args, dout.device, what)
     return dy, dw
 
 
@@ -193,7 +205,8 @@ class _SortTokens(torch.autograd.Function):
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, dest, m_indices):
-        ctx.save_for_backward(y, weights, dest, m_indices)
+        # only the gradient of the weights reads y, the largest tensor of a layer
+        ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, weights, dest, m_indices)
         return _unsort(y, dest, weights, None, "unsort_tokens")
 
     @staticmethod

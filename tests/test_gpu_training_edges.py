@@ -6,7 +6,7 @@ import torch.autograd.forward_ad as fwad
 
 import deepgemm
 from deepgemm import (expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
-                      silu_mul_checkpoint_grad, sort_tokens, token_sort, unsort_tokens)
+                      silu_mul_checkpoint_grad, sort_tokens, token_sort, unsort_tokens, unsort_tokens_grad)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -170,3 +170,42 @@ def test_the_arrays_of_a_plan_are_apart(native, monkeypatch):
     assert torch.equal(plan.dest, dest) and torch.equal(plan.m_indices, m_indices)
     for t in plan:
         assert t.is_contiguous() and t.data_ptr() % 16 == 0
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+def test_the_sorted_rows_are_kept_for_the_weights_alone(weighted):
+    """Only the gradient of the weights reads the rows: without it they can go."""
+    x = torch.randn(512, 1024, device=DEV)
+    ids = torch.randint(0, 4, (512, 2), device=DEV)
+    rows, plan = sort_tokens(x, ids, 4)
+    leaf = rows.clone().requires_grad_()
+    w = torch.rand(512, 2, device=DEV) if weighted else None
+    g = torch.randn_like(x)
+    want = unsort_tokens_grad(g, rows, plan, w)[0]
+    del rows
+    y = leaf * 2
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = unsort_tokens(y, plan, w)
+    size = y.numel() * y.element_size()
+    del y
+    assert torch.cuda.memory_allocated() <= before + out.numel() * 4 - size + 4096
+    assert torch.equal(torch.autograd.grad(out, leaf, g)[0], want * 2)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_the_gradient_of_the_rows_without_the_rows(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(token_sort, "_glue", None)
+    x = torch.randn(30, 96, device=DEV).bfloat16()
+    ids = torch.randint(-1, 4, (30, 3), device=DEV)
+    w = torch.rand(30, 3, device=DEV)
+    rows, plan = sort_tokens(x, ids, 4, align=16)
+    for weights in (w, None):
+        want, _ = unsort_tokens_grad(x, rows, plan, weights)
+        got, none = unsort_tokens_grad(x, None, plan, weights, need_dweights=False)
+        assert none is None and torch.equal(got, want)
+    for call in (lambda: unsort_tokens_grad(x, None, plan, w), lambda: unsort_tokens_grad(x[:7], None, plan, w, need_dweights=False),
+                 lambda: unsort_tokens_grad(x, None, plan, w[:7], need_dweights=False)):
+        with pytest.raises(ValueError):
+            call()
