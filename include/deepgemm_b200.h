@@ -669,9 +669,9 @@ typedef struct dg_token_sort_args {
 /* Rows that hold any routing of `pairs` pairs: every expert in use ends in a padded block; -1 on
  * bad arguments. */
 DG_API int64_t dg_token_sort_capacity(int64_t pairs, int32_t num_groups, int32_t align);
-/* 0 when no scratch is needed (up to 65536 pairs). */
+/* Bytes of scratch that dg_token_sort needs: 0 up to 16384 pairs, where every block counts them all. */
 DG_API size_t dg_token_sort_scratch_bytes(int32_t num_tokens, int32_t top_k, int32_t num_groups);
-/* One launch (three above 65536 pairs). */
+/* One launch; three where there is scratch. */
 DG_API int dg_token_sort(const dg_token_sort_args* args, void* stream);
 
 /* out[t] = sum over j, in order and in fp32, of weights[t][j] * y[dest[t][j]]; pairs with dest < 0

@@ -5,8 +5,8 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import deepgemm
-from deepgemm import (expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
-                      silu_mul_checkpoint_grad, sort_tokens, token_sort, unsort_tokens, unsort_tokens_grad)
+from deepgemm import (_cabi, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
+                      silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort, unsort_tokens, unsort_tokens_grad)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -209,3 +209,32 @@ def test_the_gradient_of_the_rows_without_the_rows(native, monkeypatch):
                  lambda: unsort_tokens_grad(x, None, plan, w[:7], need_dweights=False)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("t,k", [(16384, 1), (16385, 1), (4096, 4), (5462, 3), (2048, 8), (2049, 8)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_sort_on_both_sides_of_counting_ahead(t, k, wide):
+    """Up to 16384 pairs every block counts them all, beyond that two launches count ahead."""
+    gen = torch.Generator().manual_seed(t)
+    e, h, align = 40, 16, 128
+    ids = torch.randint(-1, e, (t, k), generator=gen)
+    x = torch.randn(t, h, generator=gen).bfloat16().to(DEV)
+    before = _cabi.query(_cabi.QUERY_LAUNCH_COUNT)
+    rows, plan = sort_tokens(x, ids.to(DEV) if wide else ids.int().to(DEV), e, align=align)
+    assert _cabi.query(_cabi.QUERY_LAUNCH_COUNT) - before == (1 if t * k <= 16384 else 3)
+    flat = ids.reshape(-1)
+    counts = torch.bincount(flat[flat >= 0], minlength=e)
+    blocks = (counts + align - 1) // align * align
+    offsets = blocks.cumsum(0) - blocks
+    order = torch.sort(torch.where(flat < 0, e, flat), stable=True).indices[:int(counts.sum())]
+    key = flat[order]
+    dest = torch.full_like(flat, -1)
+    dest[order] = offsets[key] + torch.arange(order.numel()) - (counts.cumsum(0) - counts)[key]
+    m_indices = torch.full((sort_capacity(t * k, e, align),), -1)
+    m_indices[dest[order]] = key
+    assert torch.equal(plan.dest.cpu().long(), dest.view(t, k)) and torch.equal(plan.m_indices.cpu().long(), m_indices)
+    assert torch.equal(plan.counts.cpu().long(), counts) and torch.equal(plan.offsets.cpu().long(), offsets)
+    assert plan.m_total.item() == int(blocks.sum())
+    want = torch.zeros(m_indices.numel(), h, dtype=BF, device=DEV)
+    want[dest[order].to(DEV)] = x[(order // k).to(DEV)]
+    assert torch.equal(rows, want)
