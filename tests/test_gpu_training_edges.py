@@ -5,8 +5,9 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import deepgemm
-from deepgemm import (_cabi, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, silu_mul, silu_mul_checkpoint,
-                      silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort, unsort_tokens, unsort_tokens_grad)
+from deepgemm import (_cabi, clear_padding_rows, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, moe_forward_bf16,
+                      silu_mul, silu_mul_checkpoint, silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort, unsort_tokens,
+                      unsort_tokens_grad)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -238,3 +239,65 @@ def test_sort_on_both_sides_of_counting_ahead(t, k, wide):
     want = torch.zeros(m_indices.numel(), h, dtype=BF, device=DEV)
     want[dest[order].to(DEV)] = x[(order // k).to(DEV)]
     assert torch.equal(rows, want)
+
+
+@pytest.mark.parametrize("block_n", [128, 256, 512, 0])
+@pytest.mark.parametrize("last", [1, 40, 64, 100, 128])
+@pytest.mark.parametrize("n,k", [(16, 64), (336, 576), (256, 768)])
+def test_input_grad_of_any_number_of_rows(block_n, last, n, k):
+    """The last block cut short, in a result of its own (padding cleared) and in a given one."""
+    gen = torch.Generator().manual_seed(last)
+    counts = [130, 0, 128, 257, last]
+    m, g = 6 * 128 + last, len(counts)
+    mi = torch.cat([torch.cat([torch.full((c,), e), torch.full((-c % 128,), -1)]) for e, c in enumerate(counts)]).int()[:m]
+    if last > 40:
+        mi[-7:] = -1
+    dy, w = whole(gen, m, n), whole(gen, g, n, k, lim=2)
+    dy[mi < 0] = float("nan")
+    want = torch.zeros(m, k, dtype=BF)
+    for e in range(g):
+        r = mi == e
+        want[r] = (dy[r].double() @ w[e].double()).bfloat16()
+    dyd, wd, md = dy.to(DEV), packed(w).to(DEV), mi.to(DEV)
+    poison(((m, k), BF))
+    assert torch.equal(grouped_bf16_input_grad(dyd, wd, md, block_n=block_n).cpu(), want)
+    room = torch.full((m + 128, k), 3.0, dtype=BF, device=DEV)
+    grouped_bf16_input_grad(dyd, wd, md, room[:m], block_n=block_n)
+    want[mi < 0] = 3.0
+    assert torch.equal(room[:m].cpu(), want) and bool((room[m:] == 3.0).all())
+    deepgemm.check_device_status()
+
+
+@pytest.mark.parametrize("t,gone", [(0, False), (50, True)])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_a_layer_without_a_row(t, gone, kind):
+    """No tokens, or every pair at experts that live elsewhere: zeros, and gradients of zeros."""
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(t, 128, generator=gen).bfloat16().to(DEV)
+    ids = torch.full((t, 2), -1, device=DEV) if gone else torch.zeros(t, 2, dtype=torch.long, device=DEV)
+    w = torch.rand(t, 2, generator=gen).to(DEV)
+    w13, w2 = torch.randn(3, 2, 256, 64, generator=gen).bfloat16().to(DEV), torch.randn(3, 2, 192, 64, generator=gen).bfloat16().to(DEV)
+    leaves = [v.requires_grad_() for v in (x, w, w13, w2)]
+    poison((w13.shape, BF), (w2.shape, BF), ((t, 192), BF), ((t, 128), BF))
+    out = moe_forward_bf16(leaves[0], ids, *leaves[1:], checkpoint=kind)
+    assert out.shape == (t, 192) and not bool(out.any())
+    for v, d in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
+        assert d.shape == v.shape and d.dtype == v.dtype and bool((d == 0).all())
+    with torch.no_grad():
+        assert torch.equal(moe_forward_bf16(leaves[0], ids, *leaves[1:], checkpoint=kind), out)
+    deepgemm.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("m,h", [(0, 8), (1, 1), (130, 264), (300, 77), (5000, 16), (64, 2048)])
+def test_clear_padding_rows_clears_those_and_no_others(dtype, m, h):
+    gen = torch.Generator().manual_seed(m + h)
+    rows = torch.randn(m, h, generator=gen).to(dtype)
+    mi = torch.randint(-2, 3, (m,), generator=gen).int()
+    room = torch.full((m + 2, h), 5.0, dtype=dtype, device=DEV)
+    room[1:m + 1] = rows.to(DEV)
+    room[1:m + 1][(mi < 0).to(DEV)] = float("nan")
+    mid = room[1:m + 1]
+    assert clear_padding_rows(mid, mi.to(DEV)) is mid
+    rows[mi < 0] = 0
+    assert torch.equal(mid.cpu(), rows) and bool((room[0] == 5.0).all()) and bool((room[-1] == 5.0).all())
