@@ -86,6 +86,7 @@ struct WgradParams {
   int segment;               // most row blocks that are accumulated at once
   int split;                 // kSplit: blocks of a cluster
   void* dw;                  // kSplit: the output
+  int whole_blocks;          // every row with an entry >= 0 counts for its block's group (else those of that group)
   int dy_blocks;             // N % 64 == 0: dy's map counts 64-column blocks, as x's always does
 };
 
@@ -224,7 +225,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
       const int e = __shfl_sync(0xffffffffu, m[0], 0);
       uint32_t in_group[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) in_group[i] = __ballot_sync(0xffffffffu, m[i] == e);
+      for (int i = 0; i < 4; ++i) in_group[i] = __ballot_sync(0xffffffffu, p.whole_blocks ? m[i] >= 0 : m[i] == e);
       if (lane == 0) {
         const bool in = e >= 0 && e < p.G;
         bad |= e >= p.G;
@@ -519,7 +520,8 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_con
           uint32_t rows = (1u << (n & 15)) - 1u;  // rows of the step that count
           if (n == kWgIrregular) {
             const int row = row0 + lane;
-            rows = __ballot_sync(0xffffffffu, lane < 16 && row < p.M && __ldg(p.m_indices + row) == w.g);
+            const int e = lane < 16 && row < p.M ? __ldg(p.m_indices + row) : -1;
+            rows = __ballot_sync(0xffffffffu, p.whole_blocks ? e >= 0 : e == w.g);
           }
           uint4 dy[8], x[8];
 #pragma unroll

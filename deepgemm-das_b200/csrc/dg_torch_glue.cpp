@@ -470,7 +470,7 @@ py::object input_grad_impl(const Tensor& dy, const Tensor& w, const Tensor& m_in
 }
 
 py::object weight_grad_impl(const Tensor& dy, const Tensor& x, const Tensor& m_indices, int64_t groups, const OptTensor& out, bool f32,
-                            bool accumulate, int64_t tile) {
+                            bool accumulate, int64_t tile, bool whole_blocks) {
   const int dev = current(dy);
   if (dev < 0 || !operand_ok(dy, dev) || !operand_ok(x, dev) || x.size(0) != dy.size(0) || m_indices.dim() != 1 ||
       !ints_ok(m_indices, dev, dy.size(0)) || groups < 1 || groups > DG_MAX_GROUPS)
@@ -498,6 +498,7 @@ py::object weight_grad_impl(const Tensor& dy, const Tensor& x, const Tensor& m_i
   a.out_kind = dw.scalar_type() == at::kFloat ? DG_OUT_F32 : DG_OUT_BF16;
   a.accumulate = accumulate;
   a.tile = static_cast<int32_t>(tile);
+  a.whole_blocks = whole_blocks;
   a.status = status;
   if (dg_grouped_weight_grad(&a, stream_of(dev)) != DG_OK) return py::none();
   return py::cast(dw);
@@ -536,8 +537,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("input_grad", [](const Tensor& dy, const Tensor& w, const Tensor& mi, const OptTensor& out, int64_t bn) {
     return count_obj(input_grad_impl(dy, w, mi, out, bn));
   });
-  m.def("weight_grad", [](const Tensor& dy, const Tensor& x, const Tensor& mi, int64_t g, const OptTensor& out, bool f32, bool acc, int64_t tile) {
-    return count_obj(weight_grad_impl(dy, x, mi, g, out, f32, acc, tile));
+  m.def("weight_grad", [](const Tensor& dy, const Tensor& x, const Tensor& mi, int64_t g, const OptTensor& out, bool f32, bool acc, int64_t tile,
+                          bool whole) {
+    return count_obj(weight_grad_impl(dy, x, mi, g, out, f32, acc, tile, whole));
   });
   m.def("set_status_words", &set_status_words);
   m.def("stats", []() { return std::make_pair(g_accepted, g_declined); }, "(calls enqueued here, calls handed back)");

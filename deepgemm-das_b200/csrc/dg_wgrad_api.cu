@@ -121,6 +121,7 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   p.f32 = a->out_kind == DG_OUT_F32;
   p.add = a->accumulate != 0;
   p.dw = a->dw;
+  p.whole_blocks = a->whole_blocks != 0;
   p.segment = p.f32 ? kWgSegment : DG_MAX_CONTIG_ROWS / 128;
   // 256 x 256 tiles move half the operand bytes per product, which pays when a group has rows enough
   // and there are tiles enough; else 128 x 128 ones, whose epilogues are shorter and which reach more

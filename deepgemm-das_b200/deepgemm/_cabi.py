@@ -348,7 +348,7 @@ class WeightGradArgs(C.Structure):
         ("out_kind", C.c_int32),
         ("accumulate", C.c_int32),
         ("tile", C.c_int32),
-        ("reserved", C.c_int32),
+        ("whole_blocks", C.c_int32),
         ("status", C.c_void_p),
     ]
 

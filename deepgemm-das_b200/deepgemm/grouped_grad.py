@@ -6,8 +6,12 @@
   layout ``[G, K/64, N, 64]`` of the weight, so that an optimiser steps over both element by element
   (``unpack_weight`` gives the plain ``[G, N, K]`` form).
 
-Both read ``m_indices`` as the forward product does: one group for every 128 rows, named by the first
-of them; rows with ``m_indices < 0`` stand for nothing, whatever they hold.  CUDA tensors only.
+Both read one group for every 128 rows from ``m_indices``, named by the first of them, as the forward
+product does; rows with ``m_indices < 0`` stand for nothing, whatever they hold.  They are the
+product's gradients for blocks whose other entries are that group's or negative, as ``sort_tokens``
+lays them out.  Where an entry names another group, the forward product and the input gradient take
+the row with the block's group all the same; the weight gradient leaves it out, unless it is asked to
+take ``whole_blocks``.  CUDA tensors only.
 """
 from __future__ import annotations
 
@@ -68,13 +72,15 @@ def grouped_bf16_input_grad(dy: torch.Tensor, weight: torch.Tensor, m_indices: t
 
 def grouped_bf16_weight_grad(dy: torch.Tensor, x: torch.Tensor, m_indices: torch.Tensor, num_groups: int, *,
                              out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
-                             accumulate: bool = False, tile: int = 0) -> torch.Tensor:
+                             accumulate: bool = False, tile: int = 0, whole_blocks: bool = False) -> torch.Tensor:
     """dy bf16 ``[M, N]``, x bf16 ``[M, K]`` -> dW ``[G, K/64, N, 64]`` in bf16 or fp32 (``dtype``, or the
-    type of ``out``), summed in fp32.  ``accumulate`` adds to a given fp32 ``out``, for micro-batches;
-    otherwise groups without rows give zeros."""
+    type of ``out``), summed in fp32 over the rows whose entry is the group of their block.  ``accumulate`` adds to a given fp32 ``out``, for micro-batches;
+    otherwise groups without rows give zeros.  ``whole_blocks``: rows with any entry >= 0 count for the group
+    of their block, as in the forward product."""
     what = "grouped_bf16_weight_grad"
     if _glue is not None and dtype in (torch.bfloat16, torch.float32) and \
-            (made := _glue.weight_grad(dy, x, m_indices, num_groups, out, dtype == torch.float32, accumulate, tile)) is not None:
+            (made := _glue.weight_grad(dy, x, m_indices, num_groups, out, dtype == torch.float32, accumulate, tile,
+                                      whole_blocks)) is not None:
         return made
     _bf16_rows(dy, "dy", what)
     _bf16_rows(x, "x", what)
@@ -97,6 +103,7 @@ def grouped_bf16_weight_grad(dy: torch.Tensor, x: torch.Tensor, m_indices: torch
     args = _cabi.WeightGradArgs(dy=dy.data_ptr(), x=x.data_ptr(), dw=out.data_ptr(), m_indices=m_indices.data_ptr(),
                                 num_groups=int(num_groups), m_total=m, n=n, k=k,
                                 out_kind=_cabi.OUT_F32 if out.dtype == torch.float32 else _cabi.OUT_BF16,
-                                accumulate=int(accumulate), tile=int(tile), status=device_status_words(dy.device).data_ptr())
+                                accumulate=int(accumulate), tile=int(tile), whole_blocks=int(whole_blocks),
+                                status=device_status_words(dy.device).data_ptr())
     _launch(_cabi.lib.dg_grouped_weight_grad, args, dy.device, what)
     return out

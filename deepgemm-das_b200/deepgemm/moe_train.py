@@ -55,9 +55,10 @@ class _ExpertMlp(torch.autograd.Function):
         dh, act = silu_mul_checkpoint_grad(Checkpoint(q, scale, torch.bfloat16), dact, m_indices=m_indices, need_act=need_w2)
         del dact
         if need_w2:
-            dw2 = grouped_bf16_weight_grad(dy, act, m_indices, w2.shape[0])
+            dw2 = grouped_bf16_weight_grad(dy, act, m_indices, w2.shape[0], whole_blocks=True)
         if need_w13:
-            dw13 = grouped_bf16_weight_grad(dh, restore_rows(Checkpoint(rows_q, rows_scale, torch.bfloat16)), m_indices, w13.shape[0])
+            dw13 = grouped_bf16_weight_grad(dh, restore_rows(Checkpoint(rows_q, rows_scale, torch.bfloat16)), m_indices, w13.shape[0],
+                                            whole_blocks=True)
         if need_rows:
             drows = grouped_bf16_input_grad(dh, w13, m_indices)
         return drows, dw13, dw2, None, None, None
@@ -66,7 +67,7 @@ class _ExpertMlp(torch.autograd.Function):
 def expert_mlp_bf16(rows: torch.Tensor, m_indices: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *,
                     checkpoint: str = "fp8") -> torch.Tensor:
     """Both GEMMs of the experts with the activation between them, on rows sorted by expert
-    (``sort_tokens`` with ``align`` 128 or 256): rows bf16 ``[M, K]``, w13 the packed bf16
+    (``sort_tokens`` with ``align`` 128 or 256; the first entry of 128 rows names the expert of them all): rows bf16 ``[M, K]``, w13 the packed bf16
     ``[E, K/64, 2 I, 64]`` (gate rows, then up rows), w2 the packed ``[E, I/64, K_out, 64]`` -> bf16
     ``[M, K_out]``, zero in rows with ``m_indices < 0`` and in blocks of 128 rows whose first entry names
     no expert.  Differentiable in rows, w13 and w2 (their

@@ -606,7 +606,9 @@ DG_API int dg_grouped_input_grad(const dg_input_grad_args* args, void* stream);
  * in fp32, rounded once (DG_OUT_BF16) or not at all (DG_OUT_F32; there `accumulate` adds to what dw
  * holds, every value once, so the result does not depend on an order).  m_indices names one group
  * for every 128 rows (the group of their first row); rows of them with another entry count for
- * nothing, whatever they hold.  Groups without rows give zeros. */
+ * nothing, whatever they hold.  (dg_contig_gemm and dg_grouped_input_grad take such rows, unless the
+ * entry is negative, with their block's group; so does `whole_blocks`, with which dW is the product's
+ * gradient for any entries.)  Groups without rows give zeros. */
 typedef struct dg_weight_grad_args {
   const void*    dy;        /* [m_total][n] bf16 */
   const void*    x;         /* [m_total][k] bf16 */
@@ -619,7 +621,7 @@ typedef struct dg_weight_grad_args {
   int32_t out_kind;         /* DG_OUT_BF16 or DG_OUT_F32 */
   int32_t accumulate;       /* DG_OUT_F32 only */
   int32_t tile;             /* 0 = choose; 128 / 256 = that tile; 1 = 128 with every tile split over four blocks */
-  int32_t reserved;
+  int32_t whole_blocks;     /* 0: as above; else every row with an entry >= 0 counts for its block's group */
   int32_t*       status;    /* NULL, or int32[DG_STATUS_WORDS] */
 } dg_weight_grad_args;
 DG_API int dg_grouped_weight_grad(const dg_weight_grad_args* args, void* stream);

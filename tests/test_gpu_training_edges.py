@@ -5,9 +5,9 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import deepgemm
-from deepgemm import (_cabi, clear_padding_rows, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, moe_forward_bf16,
-                      silu_mul, silu_mul_checkpoint, silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort, unsort_tokens,
-                      unsort_tokens_grad)
+from deepgemm import (_cabi, clear_padding_rows, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, grouped_grad,
+                      moe_forward_bf16, silu_mul, silu_mul_checkpoint, silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort,
+                      unsort_tokens, unsort_tokens_grad)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -301,3 +301,52 @@ def test_clear_padding_rows_clears_those_and_no_others(dtype, m, h):
     assert clear_padding_rows(mid, mi.to(DEV)) is mid
     rows[mi < 0] = 0
     assert torch.equal(mid.cpu(), rows) and bool((room[0] == 5.0).all()) and bool((room[-1] == 5.0).all())
+
+
+@pytest.mark.parametrize("block_n,tile", [(128, 128), (512, 256)])
+def test_entries_beside_the_first_of_a_block(block_n, tile):
+    """What the documentation says of a block that holds entries of two groups: the product and the gradient
+    of the rows take all of them with the first one's weights, the gradient of the weights leaves the
+    others out."""
+    gen = torch.Generator().manual_seed(4)
+    g, n, k = 3, 128, 256
+    mi = torch.full((256,), 1, dtype=torch.int32)
+    mi[30:40], mi[200:256] = 2, -1
+    dy, x, w = whole(gen, 256, n), whole(gen, 256, k), whole(gen, g, n, k, lim=2)
+    dyd, wd, md = dy.to(DEV), packed(w).to(DEV), mi.to(DEV)
+    y = torch.zeros(256, n, dtype=BF, device=DEV)
+    deepgemm.m_grouped_bf16_gemm_nt_contiguous(x.to(DEV), wd, y, md)
+    used = mi >= 0
+    assert torch.equal(y.cpu()[used], (x.double() @ w[1].double().T).bfloat16()[used])
+    dx = grouped_bf16_input_grad(dyd, wd, md, block_n=block_n).cpu()
+    assert torch.equal(dx[used], (dy.double() @ w[1].double()).bfloat16()[used])
+    dw = grouped_bf16_weight_grad(dyd, x.to(DEV), md, g, dtype=F32, tile=tile).cpu()
+    one = mi == 1
+    assert torch.equal(dw[1], packed((dy[one].double().T @ x[one].double())[None])[0].float())
+    assert not bool(dw[0].any()) and not bool(dw[2].any())
+    whole_blocks = grouped_bf16_weight_grad(dyd, x.to(DEV), md, g, dtype=F32, tile=tile, whole_blocks=True).cpu()
+    assert torch.equal(whole_blocks[1], packed((dy[used].double().T @ x[used].double())[None])[0].float())
+    assert not bool(whole_blocks[0].any()) and not bool(whole_blocks[2].any())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_the_gradients_of_the_layer_are_those_of_its_result(native, monkeypatch):
+    """Whatever the entries behind a block's first one name: the product takes the first's weights for all
+    rows, and so do all three gradients."""
+    if not native:
+        monkeypatch.setattr(grouped_grad, "_glue", None)
+    gen = torch.Generator().manual_seed(6)
+    mi = torch.randint(-1, 3, (5 * 128 + 17,), generator=gen).int()
+    mi[::128] = torch.tensor([2, 0, 2, 1, 1, 0]).int()
+    rows, g = torch.randn(mi.numel(), 128, generator=gen).bfloat16().to(DEV), torch.randn(mi.numel(), 128, generator=gen).bfloat16().to(DEV)
+    w13, w2 = (torch.randn(3, 2, 256, 64, generator=gen) / 11).bfloat16().to(DEV), (torch.randn(3, 2, 128, 64, generator=gen) / 11).bfloat16().to(DEV)
+    first = mi[::128].repeat_interleave(128)[:mi.numel()]
+
+    def run(m_indices):
+        leaves = [t.clone().requires_grad_() for t in (rows, w13, w2)]
+        y = expert_mlp_bf16(leaves[0], m_indices.to(DEV), *leaves[1:])
+        return [y.detach(), *torch.autograd.grad(y, leaves, g)]
+
+    for a, b in zip(run(mi), run(torch.where(mi < 0, mi, first))):
+        assert torch.equal(a, b)
+    deepgemm.check_device_status()
