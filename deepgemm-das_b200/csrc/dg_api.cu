@@ -706,6 +706,12 @@ int validate_and_launch(Problem& pr, cudaStream_t stream) {
     return DG_ERR_BAD_ARGUMENT;
   if ((pr.block_n == 32 || pr.block_n == 64) && (pr.mode == MODE_CONTIG || pr.kind == DG_KIND_W4A8))
     return DG_ERR_BAD_ARGUMENT;
+  if (pr.b_trans) {
+    const long long d_bytes = 2LL * pr.M * pr.N;
+    if (overlap(pr.d, d_bytes, pr.a, 2LL * pr.M * pr.K) || overlap(pr.d, d_bytes, pr.b, 2LL * pr.G * pr.N * pr.K) ||
+        overlap(pr.d, d_bytes, pr.sched, 4LL * pr.M))
+      return DG_ERR_BAD_ARGUMENT;
+  }
 
   const DeviceInfo* dev = nullptr;
   int rc = device_info(&dev);

@@ -35,6 +35,17 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* b
 // Adds to dg_query(DG_QUERY_LAUNCH_COUNT).
 void count_launches(int n);
 
+// Whether a buffer of `n` bytes and one of `m` share any: a result must not lie on what it is made of,
+// which other blocks may still be reading.
+inline bool overlap(const void* a, long long n, const void* b, long long m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && n > 0 && m > 0 && (x < y ? y - x < static_cast<uintptr_t>(n) : x - y < static_cast<uintptr_t>(m));
+}
+// Bytes from the first to behind the last of `rows` rows of `h` elements, `stride` apart.
+inline long long row_span(long long rows, long long stride, long long h, long long elem_bytes) {
+  return rows > 0 ? ((rows - 1) * stride + h) * elem_bytes : 0;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace host

@@ -109,6 +109,10 @@ int dg_token_sort(const dg_token_sort_args* a, void* stream) {
   if (need > 0 && (!a->scratch || a->scratch_bytes < need)) return DG_ERR_BAD_ARGUMENT;
   if (!aligned_to(a->x, a->elem_bytes) || !aligned_to(a->rows, a->elem_bytes) || !aligned_to(a->ids, a->ids64 ? 8 : 4))
     return DG_ERR_BAD_ALIGNMENT;
+  const long long rows_bytes = (long long)a->cap * a->hidden * a->elem_bytes;
+  if (overlap(a->rows, rows_bytes, a->x, row_span(a->num_tokens, a->x_stride, a->hidden, a->elem_bytes)) ||
+      overlap(a->rows, rows_bytes, a->ids, pairs * (a->ids64 ? 8 : 4)))
+    return DG_ERR_BAD_ARGUMENT;
   const DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc != DG_OK) return rc;
@@ -174,6 +178,10 @@ int dg_token_unsort(const dg_token_unsort_args* a, void* stream) {
   if (!a->dest || !a->out || (a->num_rows > 0 && !a->y)) return DG_ERR_NULL_POINTER;
   const size_t es = elem_size(a->elem);
   if (!aligned_to(a->y, es) || !aligned_to(a->out, es)) return DG_ERR_BAD_ALIGNMENT;
+  const long long out_bytes = (long long)es * a->num_tokens * a->hidden, pair_bytes = 4LL * a->num_tokens * a->top_k;
+  if (overlap(a->out, out_bytes, a->y, row_span(a->num_rows, a->y_stride, a->hidden, es)) ||
+      overlap(a->out, out_bytes, a->dest, pair_bytes) || overlap(a->out, out_bytes, a->weights, pair_bytes))
+    return DG_ERR_BAD_ARGUMENT;
   const DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc != DG_OK) return rc;
@@ -221,6 +229,10 @@ int dg_token_unsort_grad(const dg_token_unsort_grad_args* a, void* stream) {
   if (a->num_rows > 0 && (!a->dy || (a->dw && !a->y) || (a->clear && !a->m_indices))) return DG_ERR_NULL_POINTER;
   const size_t es = elem_size(a->elem);
   if (!aligned_to(a->y, es) || !aligned_to(a->dy, es) || !aligned_to(a->dout, es)) return DG_ERR_BAD_ALIGNMENT;
+  const long long dy_bytes = (long long)es * a->num_rows * a->hidden;
+  if (overlap(a->dy, dy_bytes, a->dout, row_span(a->num_tokens, a->dout_stride, a->hidden, es)) ||
+      (a->dw && overlap(a->dy, dy_bytes, a->y, row_span(a->num_rows, a->y_stride, a->hidden, es))))
+    return DG_ERR_BAD_ARGUMENT;
   const DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc != DG_OK) return rc;

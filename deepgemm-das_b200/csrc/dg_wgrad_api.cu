@@ -105,6 +105,10 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   if (!a->dw || (a->m_total > 0 && (!a->dy || !a->x || !a->m_indices))) return DG_ERR_NULL_POINTER;
   if (!aligned16(a->dy) || !aligned16(a->x) || !aligned16(a->dw)) return DG_ERR_BAD_ALIGNMENT;
   if (a->m_total == 0 && a->accumulate) return DG_OK;
+  const long long dw_bytes = (a->out_kind == DG_OUT_F32 ? 4LL : 2LL) * a->num_groups * a->n * a->k;
+  if (overlap(a->dw, dw_bytes, a->dy, 2LL * a->m_total * a->n) || overlap(a->dw, dw_bytes, a->x, 2LL * a->m_total * a->k) ||
+      overlap(a->dw, dw_bytes, a->m_indices, 4LL * a->m_total))
+    return DG_ERR_BAD_ARGUMENT;
   const DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc != DG_OK) return rc;

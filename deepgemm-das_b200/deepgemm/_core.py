@@ -135,6 +135,24 @@ def _launch(entry, args, device: torch.device, what: str) -> None:
         _cabi.check(entry(C.byref(args), C.c_void_p(stream)), what)
 
 
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte of a tensor's elements and the one behind their last."""
+    first = t.data_ptr()
+    if t.numel() == 0:
+        return first, first
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _apart(out: torch.Tensor, what: str, **inputs: Optional[torch.Tensor]) -> None:
+    """A result must not lie on what it is made of, which other thread blocks may still be reading."""
+    first, end = _span(out)
+    for name, t in inputs.items():
+        if t is not None:
+            a, b = _span(t)
+            if first < b and a < end and a < b:
+                raise ValueError(f"{what}: out must not overlap {name}")
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

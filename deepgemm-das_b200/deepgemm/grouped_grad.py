@@ -11,7 +11,7 @@ product does; rows with ``m_indices < 0`` stand for nothing, whatever they hold.
 product's gradients for blocks whose other entries are that group's or negative, as ``sort_tokens``
 lays them out.  Where an entry names another group, the forward product and the input gradient take
 the row with the block's group all the same; the weight gradient leaves it out, unless it is asked to
-take ``whole_blocks``.  CUDA tensors only.
+take ``whole_blocks``.  An ``out`` must not overlap an input.  CUDA tensors only.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ import torch
 
 from . import _cabi
 from ._cabi import KIND_BF16
-from ._core import _glue, _launch, device_status_words, packed_weight_dims
+from ._core import _apart, _glue, _launch, device_status_words, packed_weight_dims
 
 
 def _bf16_rows(t: torch.Tensor, name: str, what: str) -> torch.Tensor:
@@ -62,6 +62,7 @@ def grouped_bf16_input_grad(dy: torch.Tensor, weight: torch.Tensor, m_indices: t
         _bf16_rows(out, "out", what)
         if out.device != dy.device or tuple(out.shape) != (m, k):
             raise RuntimeError(f"{what}: out must be {(m, k)} on {dy.device}, got {tuple(out.shape)} on {out.device}")
+        _apart(out, what, dy=dy, weight=weight, m_indices=m_indices)
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device) if out is None else out
     args = _cabi.InputGradArgs(dy=dy.data_ptr(), w_packed=weight.data_ptr(), dx=dx.data_ptr(), m_indices=m_indices.data_ptr(),
                                num_groups=g, m_total=m, n=n, k=k, block_n=int(block_n), clear=int(out is None),
@@ -100,6 +101,7 @@ def grouped_bf16_weight_grad(dy: torch.Tensor, x: torch.Tensor, m_indices: torch
                            f"{dy.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
     if accumulate and out.dtype != torch.float32:
         raise ValueError(f"{what}: a gradient is added to in fp32, got {out.dtype}")
+    _apart(out, what, dy=dy, x=x, m_indices=m_indices)
     args = _cabi.WeightGradArgs(dy=dy.data_ptr(), x=x.data_ptr(), dw=out.data_ptr(), m_indices=m_indices.data_ptr(),
                                 num_groups=int(num_groups), m_total=m, n=n, k=k,
                                 out_kind=_cabi.OUT_F32 if out.dtype == torch.float32 else _cabi.OUT_BF16,

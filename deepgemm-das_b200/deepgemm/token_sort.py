@@ -8,7 +8,7 @@ points, ``align=1`` with ``plan.counts`` / ``plan.offsets`` for the compact one.
 
 Rows that stand for no pair (an expert's padding, everything behind the last expert;
 ``plan.m_indices < 0``) are zero in what these functions allocate and are left as they are in a
-buffer that the caller passes as ``out``.  No function here synchronises, and each can be captured
+buffer that the caller passes as ``out`` (which must not overlap an input).  No function here synchronises, and each can be captured
 into a CUDA graph.  Gradients are those of reverse mode; forward-mode differentiation is refused.
 """
 from __future__ import annotations
@@ -20,7 +20,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
-from ._core import _glue, _launch, device_status_words
+from ._core import _apart, _glue, _launch, device_status_words
 
 _ELEM = {torch.bfloat16: _cabi.OUT_BF16, torch.float16: _cabi.OUT_F16, torch.float32: _cabi.OUT_F32}
 
@@ -97,6 +97,8 @@ def _sort(x, topk_ids, num_experts, align, out):
     ids = topk_ids if topk_ids.is_contiguous() else topk_ids.contiguous()
     dev = x.device
     rows = torch.empty((cap, h), dtype=x.dtype, device=dev) if out is None else _out_arg(out, x, (cap, h), what)
+    if out is not None:
+        _apart(out, what, x=x, topk_ids=ids)
     # tensors of their own (views of one buffer would share a version: writing counts would spoil the saved dest)
     dest, m_indices, counts, offsets, m_total = (torch.empty(size, dtype=torch.int32, device=dev)
                                                  for size in ((t, k), cap, num_experts, num_experts, 1))
@@ -115,7 +117,10 @@ def _sort(x, topk_ids, num_experts, align, out):
 def _unsort(y, dest, weights, out, what):
     t, k = (int(v) for v in dest.shape)
     h = int(y.shape[1])
-    out = torch.empty((t, h), dtype=y.dtype, device=y.device) if out is None else _out_arg(out, y, (t, h), what)
+    if out is None:
+        out = torch.empty((t, h), dtype=y.dtype, device=y.device)
+    else:
+        _apart(_out_arg(out, y, (t, h), what), what, y=y, dest=dest, weights=weights)
     args = _cabi.TokenUnsortArgs(
         elem=_ELEM[y.dtype], num_tokens=t, top_k=k, hidden=h, num_rows=int(y.shape[0]),
         y_stride=y.stride(0) if y.shape[0] > 1 else h, y=y.data_ptr(), dest=dest.data_ptr(),

@@ -350,3 +350,35 @@ def test_the_gradients_of_the_layer_are_those_of_its_result(native, monkeypatch)
     for a, b in zip(run(mi), run(torch.where(mi < 0, mi, first))):
         assert torch.equal(a, b)
     deepgemm.check_device_status()
+
+
+def test_results_that_lie_on_their_inputs_are_refused():
+    x = torch.randn(256, 128, device=DEV).bfloat16()
+    ids = torch.randint(0, 2, (128, 2), dtype=torch.int32, device=DEV)
+    room = torch.randn(1024, 128, device=DEV).bfloat16()
+    w = torch.rand(128, 2, device=DEV)
+    rows, plan = sort_tokens(x[:128], ids, 2, align=1)
+    mi = torch.zeros(256, dtype=torch.int32, device=DEV)
+    square = torch.randn(1, 2, 128, 64, device=DEV).bfloat16()
+    grad = torch.zeros(1, 2, 128, 64, dtype=BF, device=DEV)
+    bad = [
+        lambda: sort_tokens(room[100:228], ids, 2, align=1, out=room[:256]),
+        lambda: unsort_tokens(room[:256], plan, w, out=room[255:383]),
+        lambda: grouped_bf16_input_grad(x, square, mi, out=x),
+        lambda: grouped_bf16_input_grad(room[:256], square, mi, out=room[255:511]),
+        lambda: grouped_bf16_input_grad(x, room[:128].view(1, 2, 128, 64), mi, out=room[:256]),
+        lambda: grouped_bf16_weight_grad(x, room[:256], mi, 1, out=room[:128].view(1, 2, 128, 64)),
+        lambda: grouped_bf16_weight_grad(room[:256], x, mi, 1, out=room[200:328].view(1, 2, 128, 64)),
+    ]
+    before = room.clone()
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError), match="overlap"):
+            call()
+            print("accepted:", i)
+    assert torch.equal(room, before)
+    # neighbours in one buffer are not concerned
+    assert torch.equal(sort_tokens(room[256:384], ids, 2, align=1, out=room[:256])[0], sort_tokens(room[256:384], ids, 2, align=1)[0])
+    unsort_tokens(room[:256], plan, w, out=room[256:384])
+    grouped_bf16_input_grad(room[:256], square, mi, out=room[256:512])
+    grouped_bf16_weight_grad(room[:256], room[256:512], mi, 1, out=grad)
+    deepgemm.check_device_status()
