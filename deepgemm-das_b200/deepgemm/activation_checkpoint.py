@@ -7,10 +7,10 @@ pass of the activation computes from the checkpoint directly.  ``silu_mul_quant`
 counterpart: it quantises the activation for the next GEMM and keeps nothing.  CUDA tensors only.
 
 ``"fp8"`` (e4m3): the scale is the smallest power of two that brings a block's largest value to 448
-or less, so a value comes back within 2^-4 of itself, or, where it is more than 2^-14 below the
-largest, within 2^-10 scales; taking rows out again in bf16 adds no rounding.  ``"int8"``: the scale is a 127th of the
-largest value, and a value comes back within half of that.  A block that holds a NaN or an infinity
-comes back as NaN.
+or less, and a value comes back within 2^-4 of itself or 2^-10 scales, whichever is more (codes are
+subnormal below 2^-6 scales, i.e. 2^-13.8 to 2^-14.8 of the largest); taking rows out again in bf16
+adds no rounding.  ``"int8"``: the scale is a 127th of the largest value, and a value comes back within
+half of that.  A block that holds a NaN or an infinity comes back as NaN.
 """
 from __future__ import annotations
 

@@ -5,9 +5,9 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import deepgemm
-from deepgemm import (_cabi, clear_padding_rows, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad, grouped_grad,
-                      moe_forward_bf16, silu_mul, silu_mul_checkpoint, silu_mul_checkpoint_grad, sort_capacity, sort_tokens, token_sort,
-                      unsort_tokens, unsort_tokens_grad)
+from deepgemm import (_cabi, checkpoint_rows, clear_padding_rows, expert_mlp_bf16, grouped_bf16_input_grad, grouped_bf16_weight_grad,
+                      grouped_grad, moe_forward_bf16, restore_rows, silu_mul, silu_mul_checkpoint, silu_mul_checkpoint_grad, sort_capacity,
+                      sort_tokens, token_sort, unsort_tokens, unsort_tokens_grad)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -382,3 +382,18 @@ def test_results_that_lie_on_their_inputs_are_refused():
     grouped_bf16_input_grad(room[:256], square, mi, out=room[256:512])
     grouped_bf16_weight_grad(room[:256], room[256:512], mi, 1, out=grad)
     deepgemm.check_device_status()
+
+
+def test_where_codes_become_subnormal():
+    """The bound on what e4m3 holds, on both sides of 2^-6 scales: 2^-4 of the value or 2^-10 scales,
+    whichever is more.  Beside a block's 225 (scale 1) 7.5 / 512 is further off than 2^-4 of itself."""
+    x = torch.zeros(3, 128, device=DEV)
+    x[0, :2] = torch.tensor([225.0, 7.5 / 512])
+    x[1] = torch.linspace(0, 2.0 ** -5, 128)
+    x[1, 0] = 448.0
+    x[2] = torch.exp2(torch.linspace(-16, 0, 128)) * 224.0
+    c = checkpoint_rows(x)
+    assert c.scale.flatten().tolist() == [1.0, 1.0, 0.5]
+    off, v = (restore_rows(c).double() - x.double()).abs(), x.double().abs()
+    assert float(off[0, 1]) > float(v[0, 1]) * 2.0 ** -4
+    assert bool((off <= torch.maximum(v * 2.0 ** -4, c.scale.double() * 2.0 ** -10)).all())
