@@ -81,7 +81,7 @@ struct CkValues<T, false> {
 };
 template <bool VEC>
 struct CkCodes {
-  EightBytes<true, 8> h[2];
+  EightBytes h[2];
   __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on) {
     h[0].load(row, c0, lane, cols, on);
     h[1].load(row, c0 + 64, lane, cols, on);

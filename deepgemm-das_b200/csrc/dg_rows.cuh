@@ -142,39 +142,21 @@ struct Eight {
   }
 };
 
-// The same for 8-bit codes: one 8-byte access, or byte by byte.
-template <bool VEC, int LANES>
+// Eight 8-bit codes, columns c0 + 8 * lane + i, in one 8-byte access.
 struct EightBytes {
   union {
     uint2 raw;
     uint32_t word[2];
     uint16_t half[4];
-    uint8_t val[8];
   };
   __device__ __forceinline__ EightBytes() { raw = make_uint2(0u, 0u); }
-  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on = true) {
-    if constexpr (VEC) {
-      const int c = c0 + 8 * lane;
-      raw = load_once8(row + c, on && c < cols);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = c0 + lane + LANES * i;
-        val[i] = on && c < cols ? row[c] : uint8_t(0);
-      }
-    }
+  __device__ __forceinline__ void load(const uint8_t* row, int c0, int lane, int cols, bool on) {
+    const int c = c0 + 8 * lane;
+    raw = load_once8(row + c, on && c < cols);
   }
   __device__ __forceinline__ void store(uint8_t* row, int c0, int lane, int cols) const {
-    if constexpr (VEC) {
-      const int c = c0 + 8 * lane;
-      if (c < cols) __stcs(reinterpret_cast<uint2*>(row + c), raw);  // not read again soon
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = c0 + lane + LANES * i;
-        if (c < cols) row[c] = val[i];
-      }
-    }
+    const int c = c0 + 8 * lane;
+    if (c < cols) __stcs(reinterpret_cast<uint2*>(row + c), raw);  // not read again soon
   }
 };
 
