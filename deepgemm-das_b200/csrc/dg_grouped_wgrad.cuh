@@ -12,7 +12,8 @@
 // tcgen05.mma.cta_group::2, block r owning rows [128 r, 128 r + 128) of the tile (its part of dY, its
 // accumulator, its epilogue) and holding 128 of the 256 columns of X.  CL = 1: one block, 128 x 128,
 // for problems with few tiles.  Either way a ring stage holds 64 rows of 128 columns of each
-// operand (32 KB), six stages.  A work item is (group, tile); its contraction walks the 128-row
+// operand (32 KB); six stages, five where eight epilogue warps (below) need the room, and one fewer
+// where the table of very many rows does.  A work item is (group, tile); its contraction walks the 128-row
 // blocks of the group in ascending order, 64 rows (a chunk) at a time.
 //   warp 0      TMA producer (each block its own copies)
 //   warp 1      UMMA issuer (leader)
@@ -43,7 +44,10 @@
 // of at most kWgSegment row blocks, each accumulated by itself and added to the ones before it with
 // correct rounding, in order, in the epilogue's registers: eight epilogue warps (kWide), each with
 // half of a tile's columns, hold a lane's 128 sums.  32 groups of 1024 rows, 4096 x 7168, i.e. two segments
-// each, fp32: 1.78 ms, added to what is there 2.29; with four warps and the segments added in memory by the
+// each, fp32: 1.79 ms, added to what is there 2.05 to 2.31 (cards differ): about as if
+// what a bf16 result does not move (1.9 GB, added 5.6) came on top of its 1.44 ms at the copy rate.  The
+// 256-wide form has 168 registers for its sums and all else (384 threads leave no more) and spills 80
+// bytes.  With four warps and the segments added in memory by the
 // TMA's reduce-add 2.2 and 2.7; 8 groups of 4096 rows 1.71 instead of 2.07.  Groups of one segment are on
 // average where they were (768 rows 1.58 and 1.60 ms, 896 rows 1.72 and 1.51, 512 rows, 4096 x 4096, 361 and
 // 404 us); bf16 results (1.44 ms) need no segments and keep four warps and the sixth ring stage.
@@ -58,7 +62,7 @@
 
 namespace dg {
 
-constexpr int kWgStages = 6;                       // five where the table below needs the room
+constexpr int kWgStages = 6;                       // less one with eight epilogue warps, less one for a large table
 constexpr int kWgThreads = 256;
 constexpr int kWgWideThreads = 384;                // kWide: warps 8..11 are a second set of epilogue warps
 constexpr uint32_t kWgBoxBytes = 64 * 128;         // 64 columns x 64 rows

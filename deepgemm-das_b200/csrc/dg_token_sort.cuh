@@ -104,10 +104,12 @@ struct BytesOf<2> { using type = uint16_t; };
 // Plan and copy in one launch.  Every block counts all pairs itself (their ids stay in L2; where they
 // are many, the two kernels above have counted), so no block waits for another; it then places the
 // pairs of its own tokens and copies their rows, each read once and written top_k times.  blockIdx.y
-// splits the columns of a row when there are few tokens.  Nine tenths of the bytes are written, and
-// HBM takes writes at 3.9 TB/s (a plain fill) where it copies at 6.5: 4096 tokens x top-8 x 7168 bf16 in
-// 32 experts padded to 128 rows, 586 MB: 122 us = 4.8 TB/s, 108 us without padding.  (Streaming
-// stores: 1024 tokens 32 -> 28 us, 4096 x top-4 67 -> 63.)
+// splits the columns of a row when there are few tokens.  Nine tenths of the bytes are written: 4096
+// tokens x top-8 x 7168 bf16 in 32 experts padded to 128 rows, 586 MB: 122 us = 4.8 TB/s, 110 us without
+// padding.  HBM takes more (a plain fp32 fill of as many bytes writes 7.1 TB/s) and issue slots are 20 %
+// busy; with one block of 32 warps on an SM, each reading a piece before it writes it, latency is the
+// likely rest, but it was not isolated.  (Streaming stores: 1024 tokens 32 -> 28 us, 4096 x top-4
+// 67 -> 63.)
 template <int VB>
 __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const TokenSortParams p) {
   using V = typename BytesOf<VB>::type;
@@ -410,7 +412,8 @@ __device__ __forceinline__ void clear_rows_block(T* out, const int32_t* m_indice
 // above, what a lane holds is kept to 64 registers (VEC; 48 if not): blocks of eight warps with up to 128
 // took 129 us instead of 105 for 16384 tokens x top-1 x 7168 bf16 (6.7 TB/s), 289 instead of 206 for fp32,
 // 425 instead of 337 for 4096 x top-8 x 7168 fp32, 55 instead of 46 for 4096 x top-4 x 1002 fp32.  Streaming
-// stores are 3 to 5 % of that.
+// stores are 3 to 5 % of that.  Six of the forms spill for it: 16-bit with eight pairs 28 bytes stored and 36
+// loaded, with four 8 and 8; fp32 with four pairs 16 and 28, with two 8 and 16.
 constexpr int kUnsortGradWarps = 4;
 __host__ __device__ constexpr int grad_pairs(bool vec, int bytes, int pairs) {  // at most
   const int most = !vec ? 2 : (bytes == 4 ? 4 : 8);

@@ -150,7 +150,7 @@ int dg_grouped_weight_grad(const dg_weight_grad_args* a, void* stream) {
   auto go = [&](auto stages) {
     constexpr int S = decltype(stages)::value;
     if (splits) return launch_wgrad<1, S, true, true>(a, p, *dev, st);
-    // (a stage's room for the strips of four more epilogue warps)
+    // (fp32: a stage's room goes to the strips of four more epilogue warps)
     if (p.f32) return tile == 256 ? launch_wgrad<2, S - 1, true>(a, p, *dev, st) : launch_wgrad<1, S - 1, true>(a, p, *dev, st);
     return tile == 256 ? launch_wgrad<2, S, false>(a, p, *dev, st) : launch_wgrad<1, S, false>(a, p, *dev, st);
   };

@@ -94,7 +94,8 @@ def restore_rows(checkpoint: Checkpoint) -> torch.Tensor:
 def silu_mul_checkpoint(x: torch.Tensor, *, kind: str = "fp8", m_indices: Optional[torch.Tensor] = None
                         ) -> Tuple[torch.Tensor, Checkpoint]:
     """x ``[M, 2 H]``, gate in the first H columns, up in the others -> ``(act [M, H], checkpoint of x)``:
-    ``act = gate * sigmoid(gate) * up`` in fp32 from x itself, rounded once.  Rows with ``m_indices < 0``
+    ``act = gate * sigmoid(gate) * up`` in fp32 from x itself, rounded once (16-bit types: a sigmoid below
+    2^-126, i.e. of a gate below -87.3, counts as zero).  Rows with ``m_indices < 0``
     are not read; their ``act`` is zero and their checkpoint holds zeros."""
     what = "silu_mul_checkpoint"
     code, qdtype = _kind(kind, what)
