@@ -75,9 +75,10 @@ def grouped_bf16_weight_grad(dy: torch.Tensor, x: torch.Tensor, m_indices: torch
                              out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
                              accumulate: bool = False, tile: int = 0, whole_blocks: bool = False) -> torch.Tensor:
     """dy bf16 ``[M, N]``, x bf16 ``[M, K]`` -> dW ``[G, K/64, N, 64]`` in bf16 or fp32 (``dtype``, or the
-    type of ``out``), summed in fp32 over the rows whose entry is the group of their block.  ``accumulate`` adds to a given fp32 ``out``, for micro-batches;
-    otherwise groups without rows give zeros.  ``whole_blocks``: rows with any entry >= 0 count for the group
-    of their block, as in the forward product."""
+    type of ``out``), summed in fp32 over the rows whose entry is the group of their block.
+    ``accumulate`` adds to a given fp32 ``out``, for micro-batches; otherwise groups without rows give
+    zeros.  ``whole_blocks``: rows with any entry >= 0 count for the group of their block, as in the
+    forward product."""
     what = "grouped_bf16_weight_grad"
     if _glue is not None and dtype in (torch.bfloat16, torch.float32) and \
             (made := _glue.weight_grad(dy, x, m_indices, num_groups, out, dtype == torch.float32, accumulate, tile,

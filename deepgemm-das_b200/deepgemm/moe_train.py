@@ -67,8 +67,8 @@ class _ExpertMlp(torch.autograd.Function):
 def expert_mlp_bf16(rows: torch.Tensor, m_indices: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *,
                     checkpoint: str = "fp8") -> torch.Tensor:
     """Both GEMMs of the experts with the activation between them, on rows sorted by expert
-    (``sort_tokens`` with ``align`` 128 or 256; the first entry of 128 rows names the expert of them all): rows bf16 ``[M, K]``, w13 the packed bf16
-    ``[E, K/64, 2 I, 64]`` (gate rows, then up rows), w2 the packed ``[E, I/64, K_out, 64]`` -> bf16
+    (``sort_tokens`` with ``align`` 128 or 256; the first entry of 128 rows names the expert of them
+    all): rows bf16 ``[M, K]``, w13 the packed bf16 ``[E, K/64, 2 I, 64]`` (gate rows, then up rows), w2 the packed ``[E, I/64, K_out, 64]`` -> bf16
     ``[M, K_out]``, zero in rows with ``m_indices < 0`` and in blocks of 128 rows whose first entry names
     no expert.  Differentiable in rows, w13 and w2 (their
     gradients have the packed layout); ``checkpoint`` ("fp8" or "int8") is what the rows and the

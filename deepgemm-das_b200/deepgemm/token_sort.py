@@ -8,8 +8,9 @@ points, ``align=1`` with ``plan.counts`` / ``plan.offsets`` for the compact one.
 
 Rows that stand for no pair (an expert's padding, everything behind the last expert;
 ``plan.m_indices < 0``) are zero in what these functions allocate and are left as they are in a
-buffer that the caller passes as ``out`` (which must not overlap an input).  No function here synchronises, and each can be captured
-into a CUDA graph.  Gradients are those of reverse mode; forward-mode differentiation is refused.
+buffer that the caller passes as ``out`` (which must not overlap an input).  No function here
+synchronises, and each can be captured into a CUDA graph.  Gradients are those of reverse mode;
+forward-mode differentiation is refused.
 """
 from __future__ import annotations
 
@@ -186,8 +187,8 @@ def unsort_tokens_grad(dout: torch.Tensor, y: Optional[torch.Tensor], plan: Toke
     args = _cabi.TokenUnsortGradArgs(
         elem=_ELEM[dout.dtype], num_tokens=t, top_k=k, hidden=h, num_rows=rows, clear=1,
         y_stride=y.stride(0) if y is not None and rows > 1 else h, dout_stride=dout.stride(0) if t > 1 else h,
-        dout=dout.data_ptr(), y=y.data_ptr() if y is not None else None, dest=dest.data_ptr(), weights=weights.data_ptr() if weights is not None else None,
-        m_indices=m_indices.data_ptr(), dy=dy.data_ptr(), dw=dw.data_ptr() if dw is not None else None)
+        dout=dout.data_ptr(), y=y.data_ptr() if y is not None else None, dest=dest.data_ptr(),
+        weights=weights.data_ptr() if weights is not None else None, m_indices=m_indices.data_ptr(), dy=dy.data_ptr(), dw=dw.data_ptr() if dw is not None else None)
     _launch(_cabi.lib.dg_token_unsort_grad, args, dout.device, what)
     return dy, dw
 

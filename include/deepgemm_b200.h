@@ -632,7 +632,8 @@ DG_API int dg_grouped_weight_grad(const dg_weight_grad_args* args, void* stream)
  * library is forward only; these are additions of this library.
  * Element types (`elem`): DG_OUT_BF16, DG_OUT_F16 or DG_OUT_F32.  Rows may lie apart (`*_stride`,
  * in elements); any row length is taken, multiples of 8 on 16-byte boundaries are fastest.
- * Results must not overlap inputs (DG_ERR_BAD_ARGUMENT); the same holds for the two gradients above.
+ * Results must not overlap inputs, here and in the two gradients above; those and the dg_token_*
+ * functions look, and return DG_ERR_BAD_ARGUMENT.
  * "Rows that stand for no pair" are those with m_indices < 0: `clear` != 0 sets them to zero in the
  * outputs, `clear` == 0 leaves them as they are.
  * --------------------------------------------------------------------------------------- */
